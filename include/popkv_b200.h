@@ -634,6 +634,143 @@ POPKV_API int popkv_norm_lm_head_argmax(const void* w, int64_t vocab, int64_t k,
                                         void* hidden_out, void* logits, unsigned long long* argmax_state,
                                         int64_t* token_next, int64_t* position_dev, void* stream);
 
+/*
+ * A KV cache held in 4 bits, in pages.  The reference keeps its cache in the
+ * model's 16-bit type, contiguous, for one sequence (popkv.py:965-972); this
+ * cache has no counterpart there.  head_dim is 128.
+ *
+ * A group of G = dim_group_size dims of one token and head is stored as numbers
+ * n in 0..15 and an fp16 pair (low, delta); n stands for low + n * delta.
+ *   pages    [layers, num_pages, kv_heads, page_bytes], 16-byte aligned, with
+ *            page_bytes = page_size * (128 + 8 * 128 / G).  A (page, head) is
+ *            page_size / 16 tiles of 16 tokens; a tile is 16 x 64 key bytes, 16 x 64
+ *            value bytes, then per token 128 / G key pairs and 128 / G value pairs
+ *            (low, delta).  Natural byte b of a row holds dim 2b in its low and 2b + 1
+ *            in its high nibble.  Key rows store the natural 4-byte word w at word
+ *            (w % 4) * 4 + w / 4; value rows the natural byte b at byte
+ *            (b % 8) * 8 + b / 8.
+ *   refs     [num_pages] sequences that hold each page; 0: the page is free
+ *   lengths  [max_seqs] tokens of each sequence (the same for every layer)
+ *   table    [max_seqs, max_pages] the page of each page_size tokens, -1 past the end
+ *   status   [4]: [0] sticky error bits (POPKV_KV4_*), [1] live pages and [2] pages moved
+ *            by the last popkv_kv4_compact
+ * page_size is 16, 32, 64, 128 or 256; G is 32, 64 or 128.  A page id or a sequence
+ * id that is out of range is never followed: such tokens do not exist.  Sequence
+ * lists (`seqs`, int32 [n]) may hold -1 for a padding slot without tokens.
+ */
+typedef struct popkv_kv4_cache {
+    uint8_t* pages;
+    int32_t* refs;
+    int32_t* lengths;
+    int32_t* table;
+    int32_t* status;
+    int64_t layers;
+    int64_t num_pages;
+    int64_t kv_heads;
+    int64_t page_size;
+    int64_t dim_group_size;
+    int64_t max_seqs;
+    int64_t max_pages;
+} popkv_kv4_cache;
+
+#define POPKV_KV4_FULL 1     /* an extend found too few free pages or table columns, and did nothing */
+#define POPKV_KV4_SEQUENCE 2 /* a sequence id was out of range or repeated; its entry was skipped */
+
+/*
+ * Quantise keys and values of the LAST counts[i] (NULL: `tokens`) tokens of each
+ * listed sequence into its pages of `layer`.  keys[i, t, h, d] is read at keys +
+ * i*k_seq_stride + t*k_token_stride + h*k_head_stride + d (elements); likewise the
+ * values.  low is the group's least value and delta a fifteenth of its range, both
+ * rounded to fp16; n = rint((x - low) * (1 / delta)) in fp32, within 0..15.  NaN is
+ * stored as 0 and magnitudes past 65504 as 65504.  The pages must belong to the
+ * sequence alone (popkv_kv4_extend sees to it).
+ */
+POPKV_API int popkv_kv4_write(const popkv_kv4_cache* cache, int64_t layer, const int32_t* seqs, int64_t n,
+                              const int32_t* counts, const void* keys, const void* values, int dtype,
+                              int64_t tokens, int64_t k_seq_stride, int64_t k_token_stride, int64_t k_head_stride,
+                              int64_t v_seq_stride, int64_t v_token_stride, int64_t v_head_stride, void* stream);
+
+/*
+ * Cached tokens [start, start + tokens) of each listed sequence, as the values they
+ * stand for: keys and values [n, tokens, kv_heads, 128] of `dtype`, contiguous, 16-byte
+ * aligned; rows past a sequence's end are zeros.
+ */
+POPKV_API int popkv_kv4_read(const popkv_kv4_cache* cache, int64_t layer, const int32_t* seqs, int64_t n,
+                             int64_t start, int64_t tokens, void* keys, void* values, int dtype, void* stream);
+
+/*
+ * Attention of the last counts[i] (NULL: q_len) tokens of each listed sequence over all
+ * its tokens, causal among them: query row j sees cached tokens 0 .. length - counts[i] + j.
+ * queries[i, j, h, d] is read at queries + i*q_seq_stride + j*q_token_stride +
+ * h*q_head_stride + d, fp16 or bf16; query head h reads KV head h / (q_heads / kv_heads).
+ * out [n, q_len, q_heads, 128] of the same type; rows j >= counts[i], and rows that see no
+ * token, are zeros.
+ */
+POPKV_API int popkv_kv4_attention(const popkv_kv4_cache* cache, int64_t layer, const int32_t* seqs, int64_t n,
+                                  const int32_t* counts, const void* queries, int dtype, int64_t q_heads,
+                                  int64_t q_len, int64_t q_seq_stride, int64_t q_token_stride,
+                                  int64_t q_head_stride, float scale, void* out, void* stream);
+
+/*
+ * Attention of one token's query heads over the cached tokens that each selected:
+ * indices int64 [n, q_heads, selected] (popkv_topk's, any order), valid uint8 of the same
+ * shape or NULL.  A slot that is masked, negative or past the sequence's end contributes
+ * nothing.  out [n, q_heads, 128]; otherwise as popkv_kv4_attention.
+ */
+POPKV_API int popkv_kv4_attention_selected(const popkv_kv4_cache* cache, int64_t layer, const int32_t* seqs,
+                                           int64_t n, const void* queries, int dtype, int64_t q_heads,
+                                           int64_t q_seq_stride, int64_t q_head_stride, const int64_t* indices,
+                                           int64_t selected, const uint8_t* valid, float scale, void* out,
+                                           void* stream);
+
+/*
+ * Page operations: they change the tables on the device, in stream order, without
+ * a host round trip.  New pages are the lowest free ones, in the order of the
+ * entries.  At most 4096 sequences a call; workspaces are int32 scratch.
+ *
+ * popkv_kv4_extend: room for counts[i] (NULL: `count`) more tokens of each listed
+ *   sequence; lengths grow.  A last page that is partly filled and shared is copied
+ *   first, in every layer.  All or nothing: with too few free pages or table columns it
+ *   sets POPKV_KV4_FULL and changes nothing else.  workspace: num_pages + 3 n.
+ * popkv_kv4_fork: children take their parents' tokens, sharing the pages, and give back
+ *   their own; every parent is read before any child changes, so one call can reorder
+ *   beams.  workspace: n * (1 + max_pages).
+ * popkv_kv4_truncate: shorten to lengths[i] tokens (NULL: free the sequence).
+ * popkv_kv4_compact: move the live pages past the number of live pages, in order, to the
+ *   free pages below it, in order; table, refs and pages of every layer follow.
+ *   workspace: 3 num_pages.
+ * popkv_kv4_copy_pages: page sources[i] to page targets[i] in every layer (entries out of
+ *   range are skipped; no target may be a source or repeat).
+ */
+POPKV_API int popkv_kv4_extend(const popkv_kv4_cache* cache, const int32_t* seqs, int64_t n, const int32_t* counts,
+                               int64_t count, int32_t* workspace, void* stream);
+POPKV_API int popkv_kv4_fork(const popkv_kv4_cache* cache, const int32_t* parents, const int32_t* children,
+                             int64_t n, int32_t* workspace, void* stream);
+POPKV_API int popkv_kv4_truncate(const popkv_kv4_cache* cache, const int32_t* seqs, int64_t n,
+                                 const int32_t* lengths, void* stream);
+POPKV_API int popkv_kv4_compact(const popkv_kv4_cache* cache, int32_t* workspace, void* stream);
+POPKV_API int popkv_kv4_copy_pages(const popkv_kv4_cache* cache, const int32_t* sources, const int32_t* targets,
+                                   int64_t count, void* stream);
+
+/*
+ * Verification of drafted tokens.  target: the target model's probabilities after each
+ * accepted prefix, element (i, j, v) at target + i*t_seq_stride + j*t_place_stride + v for
+ * j in 0..drafts; draft: the proposal's, j in 0..drafts-1, or NULL where the drafts were not
+ * drawn at random (probability 1).  Draft j of sequence i is accepted while
+ * uniforms[i, j] * q(tokens[i, j]) < p(tokens[i, j]) (fp32) and j < counts[i] (NULL: drafts).
+ * The next token is the argmax (lowest index among equals) of weight(v) / noise[i, v] in
+ * fp32, over weight > 0: weight = max(p - q, 0) at the first refusal (p where that is zero
+ * everywhere), p when none was refused.  With noise ~ Exp(1), uniforms ~ U[0, 1) the tokens
+ * are distributed as the target's.  A drafted id out of range is refused.
+ * out_tokens int64 [n, drafts + 1]: the accepted drafts, the next token, then -1;
+ * accepted int32 [n].  The reference decodes one token per call and has no counterpart.
+ */
+POPKV_API int popkv_verify_drafts(const void* target, int64_t t_seq_stride, int64_t t_place_stride,
+                                  const void* draft, int64_t d_seq_stride, int64_t d_place_stride, int dtype,
+                                  int64_t n, int64_t drafts, int64_t vocab, const int64_t* tokens,
+                                  const int32_t* counts, const float* uniforms, const float* noise,
+                                  int64_t* out_tokens, int32_t* accepted, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,366 @@
+// Pages of the 4-bit cache: share, extend (with copy on write), truncate, copy
+// and compact, all from device-resident tables, so that a captured graph or a
+// serving loop needs no host round trip.
+//
+// A page is free exactly when its reference count is 0; new pages are the lowest
+// free ones, so the result depends on the tables alone.
+#include "kv4.cuh"
+
+namespace popkv {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kCopyThreads = 256;
+constexpr int kRowThreads = 128;
+
+// Whether entry i names a sequence in range that no earlier entry names.
+__device__ bool first_of(const Kv4View& view, const int32_t* seqs, int i) {
+    const int s = seqs[i];
+    if (!view.has_sequence(s)) return false;
+    for (int j = 0; j < i; ++j)
+        if (seqs[j] == s) return false;
+    return true;
+}
+
+// Exclusive prefix sum over the block (kPlanThreads threads); *total for everybody.
+__device__ int block_scan(int value, int* total) {
+    __shared__ int sums[kPlanThreads / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int inclusive = value;
+#pragma unroll
+    for (int step = 1; step < 32; step *= 2) {
+        const int other = __shfl_up_sync(0xFFFFFFFFu, inclusive, step);
+        if (lane >= step) inclusive += other;
+    }
+    if (lane == 31) sums[warp] = inclusive;
+    __syncthreads();
+    if (warp == 0) {
+        int s = sums[lane];
+#pragma unroll
+        for (int step = 1; step < 32; step *= 2) {
+            const int other = __shfl_up_sync(0xFFFFFFFFu, s, step);
+            if (lane >= step) s += other;
+        }
+        sums[lane] = s;
+    }
+    __syncthreads();
+    const int before = warp ? sums[warp - 1] : 0;
+    *total = sums[kPlanThreads / 32 - 1];
+    __syncthreads();
+    return before + inclusive - value;
+}
+
+// One CTA.  workspace: found [num_pages] | first [n] | source [n] | target [n].
+__global__ void __launch_bounds__(kPlanThreads) extend_kernel(Kv4View view, const int32_t* __restrict__ seqs, int n,
+                                                              const int32_t* __restrict__ counts, int count,
+                                                              int32_t* __restrict__ workspace) {
+    int32_t* found = workspace;
+    int32_t* first = found + view.num_pages;
+    int32_t* source = first + n;
+    int32_t* target = source + n;
+    const int size = view.page_size();
+    __shared__ int short_of_columns;
+    if (threadIdx.x == 0) short_of_columns = 0;
+    __syncthreads();
+
+    // Pages that each entry needs: those its tokens reach, and one for the copy of
+    // a last page that is partly filled and shared.
+    int needed = 0;
+    for (int base = 0; base < n; base += kPlanThreads) {
+        const int i = base + threadIdx.x;
+        int need = 0, copied = -1;
+        if (i < n) {
+            if (first_of(view, seqs, i)) {
+                const int s = seqs[i], held = view.length_of(s);
+                const int more = max(0, counts ? counts[i] : count);
+                // 64 bits: a count near the int limit must not wrap past the check.
+                const int64_t columns = (static_cast<int64_t>(held) + more + size - 1) >> view.page_shift;
+                if (columns > view.max_pages) {
+                    short_of_columns = 1;
+                } else {
+                    need = static_cast<int>(columns) - view.pages_of(held);
+                    if (more > 0 && (held & (size - 1))) {
+                        const int last = view.page_at(s, held - 1);
+                        if (last >= 0 && view.refs[last] > 1) {
+                            copied = last;
+                            ++need;
+                        }
+                    }
+                }
+            } else {
+                need = -1;
+                if (seqs[i] != -1) atomicOr(view.status, kKv4StatusSequence);
+            }
+        }
+        int total;
+        const int before = block_scan(max(need, 0), &total);
+        if (i < n) {
+            first[i] = needed + before;
+            source[i] = copied;
+            target[i] = need;  // until the pages are known; -1: not an entry to extend
+        }
+        needed = min(needed + total, view.num_pages + 1);
+    }
+
+    // The lowest free pages, in order.
+    int free_pages = 0;
+    for (int base = 0; base < view.num_pages && free_pages < needed; base += kPlanThreads) {
+        const int p = base + threadIdx.x;
+        const bool is_free = p < view.num_pages && view.refs[p] == 0;
+        int total;
+        const int at = free_pages + block_scan(is_free, &total);
+        if (is_free && at < needed) found[at] = p;
+        free_pages += total;
+    }
+    __syncthreads();
+    if (short_of_columns || free_pages < needed) {  // all or nothing
+        for (int i = threadIdx.x; i < n; i += kPlanThreads) source[i] = -1;
+        if (threadIdx.x == 0) atomicOr(view.status, kKv4StatusFull);
+        return;
+    }
+
+    // Hand them out, a warp per entry.
+    for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {
+        const int lane = threadIdx.x & 31;
+        const int need = target[i], at = first[i], copied = source[i];
+        const int s = seqs[i];
+        __syncwarp();
+        if (need < 0) continue;
+        const int held = view.length_of(s), more = max(0, counts ? counts[i] : count);
+        int column = view.pages_of(held) - (copied >= 0);
+        for (int j = lane; j < need; j += 32) {
+            const int page = found[at + j];
+            view.table[static_cast<int64_t>(s) * view.max_pages + column + j] = page;
+            view.refs[page] = 1;
+        }
+        if (lane == 0) {
+            if (copied >= 0) {
+                atomicSub(view.refs + copied, 1);
+                target[i] = found[at];
+            }
+        }
+        __syncwarp();
+        if (lane == 0) view.lengths[s] = held + more;
+    }
+}
+
+// fork, first half: the parents' rows as they are, and a reference more for each page.
+__global__ void __launch_bounds__(kRowThreads) fork_read_kernel(Kv4View view, const int32_t* __restrict__ parents,
+                                                                const int32_t* __restrict__ children, int n,
+                                                                int32_t* __restrict__ workspace) {
+    const int i = blockIdx.x;
+    const int parent = parents[i];
+    const bool fine = view.has_sequence(parent) && first_of(view, children, i);
+    if (threadIdx.x == 0) {
+        workspace[i] = fine ? view.length_of(parent) : -1;
+        if (!fine && children[i] != -1) atomicOr(view.status, kKv4StatusSequence);
+    }
+    if (!fine) return;
+    int32_t* row = workspace + n + static_cast<int64_t>(i) * view.max_pages;
+    const int pages = view.pages_of(view.length_of(parent));
+    for (int j = threadIdx.x; j < pages; j += kRowThreads) {
+        const int page = view.table[static_cast<int64_t>(parent) * view.max_pages + j];
+        row[j] = page;
+        if (page >= 0 && page < view.num_pages) atomicAdd(view.refs + page, 1);
+    }
+}
+
+// fork, second half: each child gives its pages back and takes the rows read.
+__global__ void __launch_bounds__(kRowThreads) fork_write_kernel(Kv4View view, const int32_t* __restrict__ children,
+                                                                 int n, const int32_t* __restrict__ workspace) {
+    const int i = blockIdx.x;
+    const int length = workspace[i];
+    if (length < 0) return;
+    const int child = children[i];
+    const int before = view.pages_of(view.length_of(child)), after = view.pages_of(length);
+    const int32_t* row = workspace + n + static_cast<int64_t>(i) * view.max_pages;
+    int32_t* to = view.table + static_cast<int64_t>(child) * view.max_pages;
+    for (int j = threadIdx.x; j < max(before, after); j += kRowThreads) {
+        if (j < before) {
+            const int page = to[j];
+            if (page >= 0 && page < view.num_pages) atomicSub(view.refs + page, 1);
+        }
+        to[j] = j < after ? row[j] : -1;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) view.lengths[child] = length;
+}
+
+__global__ void __launch_bounds__(kRowThreads) truncate_kernel(Kv4View view, const int32_t* __restrict__ seqs,
+                                                               const int32_t* __restrict__ lengths) {
+    const int i = blockIdx.x;
+    if (!first_of(view, seqs, i)) {
+        if (threadIdx.x == 0 && seqs[i] != -1) atomicOr(view.status, kKv4StatusSequence);
+        return;
+    }
+    const int s = seqs[i], held = view.length_of(s);
+    const int kept = lengths ? min(held, max(0, lengths[i])) : 0;
+    int32_t* row = view.table + static_cast<int64_t>(s) * view.max_pages;
+    for (int j = view.pages_of(kept) + threadIdx.x; j < view.pages_of(held); j += kRowThreads) {
+        const int page = row[j];
+        if (page >= 0 && page < view.num_pages) atomicSub(view.refs + page, 1);
+        row[j] = -1;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) view.lengths[s] = kept;
+}
+
+// One CTA.  workspace: source [num_pages] | target [num_pages] | place [num_pages].
+__global__ void __launch_bounds__(kPlanThreads) compact_kernel(Kv4View view, int32_t* __restrict__ workspace) {
+    int32_t* source = workspace;
+    int32_t* target = source + view.num_pages;
+    int32_t* place = target + view.num_pages;
+    int live = 0;
+    for (int base = 0; base < view.num_pages; base += kPlanThreads) {
+        const int p = base + threadIdx.x;
+        int total;
+        block_scan(p < view.num_pages && view.refs[p] > 0, &total);
+        live += total;
+    }
+    int moved = 0, holes = 0;
+    for (int base = 0; base < view.num_pages; base += kPlanThreads) {
+        const int p = base + threadIdx.x;
+        const bool used = p < view.num_pages && view.refs[p] > 0;
+        const bool moves = used && p >= live, hole = p < live && !used;
+        int total;
+        const int at = moved + block_scan(moves, &total);
+        moved += total;
+        const int into = holes + block_scan(hole, &total);
+        holes += total;
+        if (moves) source[at] = p;
+        if (hole) target[into] = p;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < moved; i += kPlanThreads) {
+        place[source[i]] = target[i];
+        view.refs[target[i]] = view.refs[source[i]];
+        view.refs[source[i]] = 0;
+    }
+    if (threadIdx.x == 0) {
+        view.status[1] = live;
+        view.status[2] = moved;
+    }
+}
+
+__global__ void __launch_bounds__(kRowThreads) place_kernel(Kv4View view, const int32_t* __restrict__ workspace) {
+    const int s = blockIdx.x;
+    const int live = view.status[1];
+    const int32_t* place = workspace + 2 * static_cast<int64_t>(view.num_pages);
+    const int pages = view.pages_of(view.length_of(s));
+    for (int j = threadIdx.x; j < pages; j += kRowThreads) {
+        const int64_t at = static_cast<int64_t>(s) * view.max_pages + j;
+        const int page = view.table[at];
+        if (page >= live && page < view.num_pages) view.table[at] = place[page];
+    }
+}
+
+// Page i of layer blockIdx.z, one part of it per blockIdx.x.
+__global__ void __launch_bounds__(kCopyThreads) copy_kernel(Kv4View view, const int32_t* __restrict__ sources,
+                                                            const int32_t* __restrict__ targets, int64_t count,
+                                                            const int32_t* __restrict__ count_dev) {
+    if (count_dev) count = min(count, static_cast<int64_t>(*count_dev));
+    const int64_t units = view.page_bytes / 16;
+    for (int64_t i = blockIdx.y; i < count; i += gridDim.y) {
+        const int from = sources[i], to = targets[i];
+        if (from < 0 || from >= view.num_pages || to < 0 || to >= view.num_pages) continue;
+        const uint8_t* layer = view.pages + blockIdx.z * view.layer_bytes;
+        const auto* src = reinterpret_cast<const uint4*>(layer + from * view.page_bytes);
+        auto* dst = reinterpret_cast<uint4*>(const_cast<uint8_t*>(layer) + to * view.page_bytes);
+        for (int64_t u = blockIdx.x * static_cast<int64_t>(kCopyThreads) + threadIdx.x; u < units;
+             u += static_cast<int64_t>(gridDim.x) * kCopyThreads)
+            dst[u] = src[u];
+    }
+}
+
+}  // namespace
+
+int kv4_copy_launch(const char* what, const Kv4View& view, const int32_t* sources, const int32_t* targets,
+                    int64_t count, const int32_t* count_dev, cudaStream_t stream) {
+    if (count == 0) return POPKV_OK;
+    const int64_t units = view.page_bytes / 16;
+    const unsigned x = static_cast<unsigned>(units > 16 * kCopyThreads ? 16 : (units + kCopyThreads - 1) / kCopyThreads);
+    const unsigned y = static_cast<unsigned>(count > 4096 ? 4096 : count);
+    copy_kernel<<<dim3(x, y, view.layers), kCopyThreads, 0, stream>>>(view, sources, targets, count, count_dev);
+    return check_launch(what);
+}
+
+}  // namespace popkv
+
+extern "C" int popkv_kv4_copy_pages(const popkv_kv4_cache* cache, const int32_t* sources, const int32_t* targets,
+                                    int64_t count, void* stream) {
+    using namespace popkv;
+    Kv4View view;
+    if (int status = kv4_view("popkv_kv4_copy_pages", cache, &view)) return status;
+    if (count < 0 || count > (1 << 30)) return fail(POPKV_ERR_INVALID, "popkv_kv4_copy_pages: count out of range");
+    if (count == 0) return POPKV_OK;
+    if (!sources || !targets) return fail(POPKV_ERR_INVALID, "popkv_kv4_copy_pages: null pointer");
+    return kv4_copy_launch("popkv_kv4_copy_pages", view, sources, targets, count, nullptr,
+                           static_cast<cudaStream_t>(stream));
+}
+
+namespace popkv {
+namespace {
+int check_entries(const char* what, int64_t n) {
+    if (n < 0 || n > 4096) return fail(POPKV_ERR_INVALID, "%s: between 0 and 4096 sequences in one call", what);
+    return POPKV_OK;
+}
+}  // namespace
+}  // namespace popkv
+
+extern "C" int popkv_kv4_extend(const popkv_kv4_cache* cache, const int32_t* seqs, int64_t n, const int32_t* counts,
+                                int64_t count, int32_t* workspace, void* stream) {
+    using namespace popkv;
+    Kv4View view;
+    if (int status = kv4_view("popkv_kv4_extend", cache, &view)) return status;
+    if (int status = check_entries("popkv_kv4_extend", n)) return status;
+    if (count < 0 || count > (1 << 30)) return fail(POPKV_ERR_INVALID, "popkv_kv4_extend: count out of range");
+    if (n == 0) return POPKV_OK;
+    if (!seqs || !workspace) return fail(POPKV_ERR_INVALID, "popkv_kv4_extend: null pointer");
+    const auto s = static_cast<cudaStream_t>(stream);
+    extend_kernel<<<1, kPlanThreads, 0, s>>>(view, seqs, static_cast<int>(n), counts, static_cast<int>(count),
+                                             workspace);
+    if (int status = check_launch("popkv_kv4_extend")) return status;
+    const int32_t* source = workspace + view.num_pages + n;
+    return kv4_copy_launch("popkv_kv4_extend", view, source, source + n, n, nullptr, s);
+}
+
+extern "C" int popkv_kv4_fork(const popkv_kv4_cache* cache, const int32_t* parents, const int32_t* children,
+                              int64_t n, int32_t* workspace, void* stream) {
+    using namespace popkv;
+    Kv4View view;
+    if (int status = kv4_view("popkv_kv4_fork", cache, &view)) return status;
+    if (int status = check_entries("popkv_kv4_fork", n)) return status;
+    if (n == 0) return POPKV_OK;
+    if (!parents || !children || !workspace) return fail(POPKV_ERR_INVALID, "popkv_kv4_fork: null pointer");
+    const auto s = static_cast<cudaStream_t>(stream);
+    const int count = static_cast<int>(n);
+    fork_read_kernel<<<count, kRowThreads, 0, s>>>(view, parents, children, count, workspace);
+    fork_write_kernel<<<count, kRowThreads, 0, s>>>(view, children, count, workspace);
+    return check_launch("popkv_kv4_fork");
+}
+
+extern "C" int popkv_kv4_truncate(const popkv_kv4_cache* cache, const int32_t* seqs, int64_t n,
+                                  const int32_t* lengths, void* stream) {
+    using namespace popkv;
+    Kv4View view;
+    if (int status = kv4_view("popkv_kv4_truncate", cache, &view)) return status;
+    if (int status = check_entries("popkv_kv4_truncate", n)) return status;
+    if (n == 0) return POPKV_OK;
+    if (!seqs) return fail(POPKV_ERR_INVALID, "popkv_kv4_truncate: null pointer");
+    truncate_kernel<<<static_cast<unsigned>(n), kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(view, seqs,
+                                                                                                      lengths);
+    return check_launch("popkv_kv4_truncate");
+}
+
+extern "C" int popkv_kv4_compact(const popkv_kv4_cache* cache, int32_t* workspace, void* stream) {
+    using namespace popkv;
+    Kv4View view;
+    if (int status = kv4_view("popkv_kv4_compact", cache, &view)) return status;
+    if (!workspace) return fail(POPKV_ERR_INVALID, "popkv_kv4_compact: null pointer");
+    const auto s = static_cast<cudaStream_t>(stream);
+    compact_kernel<<<1, kPlanThreads, 0, s>>>(view, workspace);
+    place_kernel<<<view.max_seqs, kRowThreads, 0, s>>>(view, workspace);
+    if (int status = check_launch("popkv_kv4_compact")) return status;
+    return kv4_copy_launch("popkv_kv4_compact", view, workspace, workspace + view.num_pages, view.num_pages,
+                           view.status + 2, s);
+}

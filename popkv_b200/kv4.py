@@ -1,0 +1,361 @@
+"""A KV cache held in 4 bits, in pages, and the attention that reads it.
+
+``Kv4Cache`` holds keys and values of several sequences and layers as 4-bit numbers
+with an fp16 (low, delta) pair per group of 32, 64 or 128 dims: 160, 144 or 136 bytes a
+token and KV head instead of 512 in bf16.  Pages of 16 to 256 tokens are shared between
+sequences (parallel samples, beams, drafted branches) and copied when a shared one is
+written.  All tables live on the device; no call here synchronises except ``check`` and
+``free_pages``.
+
+A decode step, for the sequences ``seqs`` (int32 slots of the cache)::
+
+    cache.extend(seqs, 1)                               # room for the token, in every layer
+    for layer in ...:
+        cache.write(keys, values, seqs=seqs, layer=layer)
+        out = cache.attention(queries, seqs=seqs, layer=layer)              # dense layers
+        out = cache.attention_selected(queries, indices, seqs=seqs, layer=layer)  # sparse layers
+
+With drafted tokens, ``extend`` / ``write`` / ``attention`` take several tokens a sequence
+(``counts`` when the drafts are of uneven length), ``popkv_b200.speculative.verify_drafts``
+says how many stay, and ``truncate`` drops the rest.
+
+The reference keeps a contiguous 16-bit cache of one sequence (popkv.py:965-972) and has no
+counterpart.  The byte layout is documented in ``include/popkv_b200.h``.  Sequence ids of -1
+are padding; ids out of range or repeated set an error bit that ``check`` raises on.
+
+Streams: calls run on the current stream of the cache's device.  Calls on one cache that
+overlap in time must be ordered by the caller when one of them writes.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+
+HEAD_DIM = 128
+DIM_GROUP_SIZES = (32, 64, 128)
+PAGE_SIZES = (16, 32, 64, 128, 256)
+MAX_SEQUENCES_PER_CALL = 4096
+
+
+class _Descriptor(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("pages", "refs", "lengths", "table", "status")] + [
+        (name, ctypes.c_int64) for name in ("layers", "num_pages", "kv_heads", "page_size", "dim_group_size",
+                                            "max_seqs", "max_pages")]
+
+
+def page_bytes(page_size: int, dim_group_size: int) -> int:
+    """Bytes of one page of one KV head."""
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"page_size must be one of {PAGE_SIZES}")
+    if dim_group_size not in DIM_GROUP_SIZES:
+        raise ValueError(f"dim_group_size must be one of {DIM_GROUP_SIZES}")
+    return page_size * (HEAD_DIM + 8 * (HEAD_DIM // dim_group_size))
+
+
+class Kv4Cache:
+    """Pages, tables and operations of a 4-bit KV cache (head_dim 128).
+
+    Args:
+        num_pages: pages of the pool (of each layer).
+        kv_heads, layers: KV heads and layers of the model.
+        max_seqs: sequence slots.
+        max_tokens: most tokens of one sequence (rounded up to whole pages).
+        page_size: tokens of a page, one of 16, 32, 64, 128, 256.
+        dim_group_size: dims that share a (low, delta) pair, one of 32, 64, 128.
+    """
+
+    def __init__(self, num_pages: int, *, kv_heads: int, layers: int = 1, max_seqs: int = 1, max_tokens: int,
+                 page_size: int = 64, dim_group_size: int = 32, device="cuda") -> None:
+        size = page_bytes(page_size, dim_group_size)
+        if min(num_pages, kv_heads, layers, max_seqs, max_tokens) < 1:
+            raise ValueError("cache sizes must be positive")
+        max_pages = math.ceil(max_tokens / page_size)
+        pages = torch.zeros((layers, num_pages, kv_heads, size), dtype=torch.uint8, device=device)
+        tables = torch.zeros(num_pages + max_seqs * (1 + max_pages), dtype=torch.int32, device=device)
+        tables[num_pages + max_seqs:] = -1
+        self._bind(pages, tables, max_seqs, page_size, dim_group_size)
+
+    @classmethod
+    def from_tensors(cls, pages: torch.Tensor, tables: torch.Tensor, *, max_seqs: int, page_size: int,
+                     dim_group_size: int) -> "Kv4Cache":
+        """A cache over buffers that the caller holds.
+
+        pages: uint8 [layers, num_pages, kv_heads, page_bytes]; tables: int32, refs [num_pages],
+        lengths [max_seqs] and table [max_seqs, max_pages] one after another.  Both contiguous.
+        """
+        size = page_bytes(page_size, dim_group_size)
+        if pages.ndim != 4 or pages.dtype != torch.uint8 or not pages.is_contiguous() or pages.shape[3] != size:
+            raise ValueError(f"pages must be contiguous uint8 [layers, num_pages, kv_heads, {size}]")
+        if min(pages.shape) < 1:
+            raise ValueError("cache sizes must be positive")
+        if tables.ndim != 1 or tables.dtype != torch.int32 or not tables.is_contiguous():
+            raise ValueError("tables must be a contiguous int32 vector")
+        if tables.device != pages.device:
+            raise ValueError("pages and tables must share a device")
+        rest = tables.numel() - int(pages.shape[1]) - max_seqs
+        if max_seqs < 1 or rest < max_seqs or rest % max_seqs:
+            raise ValueError("tables must hold refs [num_pages], lengths [max_seqs] and table [max_seqs, max_pages]")
+        cache = cls.__new__(cls)
+        cache._bind(pages, tables, max_seqs, page_size, dim_group_size)
+        return cache
+
+    def _bind(self, pages, tables, max_seqs, page_size, dim_group_size) -> None:
+        self.pages, self.tables = pages, tables
+        self.layers, self.num_pages, self.kv_heads = (int(x) for x in pages.shape[:3])
+        self.max_seqs, self.page_size, self.dim_group_size = int(max_seqs), int(page_size), int(dim_group_size)
+        self.refs = tables[:self.num_pages]
+        self.lengths = tables[self.num_pages:self.num_pages + self.max_seqs]
+        self.table = tables[self.num_pages + self.max_seqs:].view(self.max_seqs, -1)
+        self.max_pages = int(self.table.shape[1])
+        self.device = pages.device
+        self.status = torch.zeros(4, dtype=torch.int32, device=pages.device)
+        self._descriptor = _Descriptor(
+            pages.data_ptr(), self.refs.data_ptr(), self.lengths.data_ptr(), self.table.data_ptr(),
+            self.status.data_ptr(), self.layers, self.num_pages, self.kv_heads, self.page_size,
+            self.dim_group_size, self.max_seqs, self.max_pages)
+        self._address = ctypes.addressof(self._descriptor)
+
+    # -- arguments -----------------------------------------------------------------
+    def _call(self, entry, *args) -> None:
+        device = self.device
+        if device.type != "cuda":
+            raise RuntimeError("the 4-bit cache must be on a CUDA device")
+        if torch.cuda.current_device() == device.index:
+            status = entry(self._address, *args, torch.cuda.current_stream(device).cuda_stream)
+        else:
+            with torch.cuda.device(device):
+                status = entry(self._address, *args, torch.cuda.current_stream(device).cuda_stream)
+        if status:
+            _lib.check(status)
+
+    def _ids(self, ids, name: str) -> torch.Tensor:
+        """int32 [n] on the cache's device, from a tensor or a sequence of ints."""
+        if not isinstance(ids, torch.Tensor):
+            ids = torch.tensor(ids, dtype=torch.int32, device=self.device)
+        if ids.dtype != torch.int32 or not ids.is_contiguous():
+            if ids.dtype not in (torch.int32, torch.int64):
+                raise ValueError(f"{name} must be int32 or int64")
+            ids = ids.to(torch.int32).contiguous()
+        if ids.ndim != 1:
+            raise ValueError(f"{name} must be one-dimensional")
+        if ids.device != self.device:
+            raise RuntimeError(f"{name} must be on the cache's device")
+        return ids
+
+    def _sequences(self, seqs, name: str = "seqs", most: int = MAX_SEQUENCES_PER_CALL) -> torch.Tensor:
+        seqs = self._ids(seqs, name)
+        if seqs.shape[0] > most:
+            raise ValueError(f"at most {most} sequences in one call")
+        return seqs
+
+    def _per_sequence(self, values, seqs: torch.Tensor, name: str) -> torch.Tensor:
+        values = self._ids(values, name)
+        if values.shape[0] != seqs.shape[0]:
+            raise ValueError(f"{name} must have one value per listed sequence")
+        return values
+
+    def _layer(self, layer: int) -> int:
+        if not 0 <= layer < self.layers:
+            raise ValueError(f"layer must be in [0, {self.layers})")
+        return layer
+
+    # -- rows ----------------------------------------------------------------------
+    def write(self, keys: torch.Tensor, values: torch.Tensor, *, seqs, layer: int = 0, counts=None) -> None:
+        """Quantise the keys and values of the last tokens of each listed sequence.
+
+        keys, values: fp32/fp16/bf16 [n, tokens, kv_heads, 128], or [n, kv_heads, 128] for one
+        token; any strides with contiguous dims (slices of a fused projection).  They are the
+        last ``tokens`` (or ``counts[i]`` <= tokens, the first of the row's) of sequence
+        ``seqs[i]``, for which ``extend`` has made room.
+        """
+        if keys.ndim == 3 and values.ndim == 3:
+            keys, values = keys.unsqueeze(1), values.unsqueeze(1)
+        seqs = self._sequences(seqs, most=1 << 30)
+        if (keys.ndim != 4 or keys.shape != values.shape or keys.shape[0] != seqs.shape[0]
+                or keys.shape[2] != self.kv_heads or keys.shape[3] != HEAD_DIM):
+            raise ValueError(f"keys and values must be [{seqs.shape[0]}, tokens, {self.kv_heads}, {HEAD_DIM}]")
+        if keys.dtype != values.dtype or keys.dtype not in _lib.DTYPE_CODES:
+            raise RuntimeError("keys and values must share an fp32/fp16/bf16 dtype")
+        if keys.device != self.device or values.device != self.device:
+            raise RuntimeError("keys and values must be on the cache's device")
+        keys, values = _rows(keys), _rows(values)
+        counts = None if counts is None else self._per_sequence(counts, seqs, "counts")
+        ks, vs = keys.stride(), values.stride()
+        self._call(_lib.lib().popkv_kv4_write, self._layer(layer), seqs.data_ptr(), seqs.shape[0],
+                   None if counts is None else counts.data_ptr(), keys.data_ptr(), values.data_ptr(),
+                   _lib.DTYPE_CODES[keys.dtype], keys.shape[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
+
+    def read(self, seqs, *, start: int = 0, tokens: int, layer: int = 0,
+             dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+        """Cached tokens [start, start + tokens) as keys and values [n, tokens, kv_heads, 128].
+
+        Rows past a sequence's end are zeros.
+        """
+        if dtype not in _lib.DTYPE_CODES:
+            raise RuntimeError("dtype must be fp32/fp16/bf16")
+        if start < 0 or tokens < 0:
+            raise ValueError("start and tokens must not be negative")
+        seqs = self._sequences(seqs, most=1 << 30)
+        shape = (seqs.shape[0], tokens, self.kv_heads, HEAD_DIM)
+        keys = torch.empty(shape, dtype=dtype, device=self.device)
+        values = torch.empty(shape, dtype=dtype, device=self.device)
+        self._call(_lib.lib().popkv_kv4_read, self._layer(layer), seqs.data_ptr(), seqs.shape[0], start, tokens,
+                   keys.data_ptr(), values.data_ptr(), _lib.DTYPE_CODES[dtype])
+        return keys, values
+
+    # -- attention -----------------------------------------------------------------
+    def _queries(self, queries: torch.Tensor, seqs: torch.Tensor) -> torch.Tensor:
+        if queries.shape[0] != seqs.shape[0] or queries.shape[-1] != HEAD_DIM:
+            raise ValueError(f"queries must be [{seqs.shape[0]}, ..., query heads, {HEAD_DIM}]")
+        if queries.shape[-2] < 1 or queries.shape[-2] % self.kv_heads:
+            raise ValueError("query heads must be a multiple of the cache's KV heads")
+        if queries.dtype not in (torch.float16, torch.bfloat16):
+            raise RuntimeError("queries must be fp16 or bf16")
+        if queries.device != self.device:
+            raise RuntimeError("queries must be on the cache's device")
+        return _rows(queries)
+
+    def attention(self, queries: torch.Tensor, *, seqs, layer: int = 0, counts=None,
+                  softmax_scale: float | None = None) -> torch.Tensor:
+        """Causal attention of each listed sequence's last tokens over all its tokens.
+
+        queries: fp16/bf16 [n, q_len, q_heads, 128], or [n, q_heads, 128] for one token; row j of
+        sequence i is its token ``lengths[seqs[i]] - counts[i] + j`` (``counts`` default q_len).
+        Returns the same shape and type; rows past ``counts[i]``, and rows that see no token, are
+        zeros.  ``softmax_scale`` defaults to 1 / sqrt(128).
+        """
+        if queries.ndim not in (3, 4):
+            raise ValueError("queries must be [n, q_len, query heads, 128] or [n, query heads, 128]")
+        seqs = self._sequences(seqs, most=65535)
+        queries = self._queries(queries, seqs)
+        counts = None if counts is None else self._per_sequence(counts, seqs, "counts")
+        out = torch.empty(queries.shape, dtype=queries.dtype, device=self.device)
+        strides = queries.stride()
+        self._call(_lib.lib().popkv_kv4_attention, self._layer(layer), seqs.data_ptr(), seqs.shape[0],
+                   None if counts is None else counts.data_ptr(), queries.data_ptr(),
+                   _lib.DTYPE_CODES[queries.dtype], queries.shape[-2],
+                   queries.shape[1] if queries.ndim == 4 else 1, strides[0], strides[1] if queries.ndim == 4 else 0,
+                   strides[-2], _scale(softmax_scale), out.data_ptr())
+        return out
+
+    def attention_selected(self, queries: torch.Tensor, indices: torch.Tensor, *, seqs, layer: int = 0,
+                           valid_mask: torch.Tensor | None = None,
+                           softmax_scale: float | None = None) -> torch.Tensor:
+        """Attention of one token's query heads over the cached tokens that each selected.
+
+        queries: fp16/bf16 [n, q_heads, 128]; indices: int64 [n, q_heads, selected] token positions
+        (``popkv_cuda.topk``'s); valid_mask: bool of the same shape.  A slot that is masked, negative
+        or past the sequence's end contributes nothing.  Returns [n, q_heads, 128].
+        """
+        if queries.ndim != 3:
+            raise ValueError("queries must be [n, query heads, 128]")
+        if indices.ndim != 3 or indices.shape[:2] != queries.shape[:2]:
+            raise ValueError("indices must be [n, query heads, selected tokens]")
+        if valid_mask is not None and valid_mask.shape != indices.shape:
+            raise ValueError("valid mask must match indices")
+        if indices.dtype != torch.int64:
+            raise ValueError("indices must be int64")
+        seqs = self._sequences(seqs, most=65535)
+        queries = self._queries(queries, seqs)
+        if indices.device != self.device or (valid_mask is not None and valid_mask.device != self.device):
+            raise RuntimeError("indices and valid mask must be on the cache's device")
+        indices = indices.contiguous()
+        if valid_mask is not None:
+            if valid_mask.dtype not in (torch.bool, torch.uint8):
+                raise ValueError("valid mask must be bool or uint8")
+            valid_mask = valid_mask.contiguous()
+        out = torch.empty(queries.shape, dtype=queries.dtype, device=self.device)
+        strides = queries.stride()
+        self._call(_lib.lib().popkv_kv4_attention_selected, self._layer(layer), seqs.data_ptr(), seqs.shape[0],
+                   queries.data_ptr(), _lib.DTYPE_CODES[queries.dtype], queries.shape[1], strides[0], strides[1],
+                   indices.data_ptr(), indices.shape[2], None if valid_mask is None else valid_mask.data_ptr(),
+                   _scale(softmax_scale), out.data_ptr())
+        return out
+
+    # -- pages ---------------------------------------------------------------------
+    def extend(self, seqs, tokens) -> None:
+        """Room for ``tokens`` (an int, or int32 [n]) more tokens of each listed sequence.
+
+        Takes the lowest free pages; a last page that is partly filled and shared with another
+        sequence is copied first, in every layer.  All or nothing: without enough free pages
+        nothing changes and ``check`` raises.
+        """
+        seqs = self._sequences(seqs)
+        counts, count = None, 0
+        if isinstance(tokens, int):
+            count = tokens
+            if count < 0:
+                raise ValueError("tokens must not be negative")
+        else:
+            counts = self._per_sequence(tokens, seqs, "tokens")
+        n = seqs.shape[0]
+        workspace = torch.empty(self.num_pages + 3 * n, dtype=torch.int32, device=self.device)
+        self._call(_lib.lib().popkv_kv4_extend, seqs.data_ptr(), n, None if counts is None else counts.data_ptr(),
+                   count, workspace.data_ptr())
+
+    def fork(self, parents, children) -> None:
+        """Sequence ``children[i]`` becomes a copy of ``parents[i]`` that shares its pages.
+
+        What a child held before is given back.  Every parent is read before any child changes,
+        so one call can reorder beams (children distinct, parents repeated at will).
+        """
+        parents, children = self._sequences(parents, "parents"), self._sequences(children, "children")
+        if parents.shape != children.shape:
+            raise ValueError("parents and children must have the same length")
+        n = parents.shape[0]
+        workspace = torch.empty(n * (1 + self.max_pages), dtype=torch.int32, device=self.device)
+        self._call(_lib.lib().popkv_kv4_fork, parents.data_ptr(), children.data_ptr(), n, workspace.data_ptr())
+
+    def truncate(self, seqs, lengths) -> None:
+        """Shorten each listed sequence to ``lengths[i]`` tokens (longer: unchanged)."""
+        seqs = self._sequences(seqs)
+        lengths = self._per_sequence(lengths, seqs, "lengths")
+        self._call(_lib.lib().popkv_kv4_truncate, seqs.data_ptr(), seqs.shape[0], lengths.data_ptr())
+
+    def free(self, seqs) -> None:
+        """Give back every page of the listed sequences."""
+        seqs = self._sequences(seqs)
+        self._call(_lib.lib().popkv_kv4_truncate, seqs.data_ptr(), seqs.shape[0], None)
+
+    def compact(self) -> None:
+        """Move the live pages to the front of the pool (``status[1]`` then counts them).
+
+        Live pages past the number of live pages move, in order, to the free pages below it, in
+        order; the tables follow.  The tail of the pool is then free.
+        """
+        workspace = torch.empty(3 * self.num_pages, dtype=torch.int32, device=self.device)
+        self._call(_lib.lib().popkv_kv4_compact, workspace.data_ptr())
+
+    def copy_pages(self, sources, targets) -> None:
+        """Copy page ``sources[i]`` to page ``targets[i]`` in every layer (no table changes)."""
+        sources, targets = self._ids(sources, "sources"), self._ids(targets, "targets")
+        if sources.shape != targets.shape:
+            raise ValueError("sources and targets must have the same length")
+        self._call(_lib.lib().popkv_kv4_copy_pages, sources.data_ptr(), targets.data_ptr(), sources.shape[0])
+
+    # -- state ---------------------------------------------------------------------
+    def check(self) -> None:
+        """Raise if a page operation failed since the last check (synchronises)."""
+        bits = int(self.status[0].item())
+        if not bits:
+            return
+        self.status[0] = 0
+        reasons = [text for bit, text in ((1, "too few free pages or table columns for an extend"),
+                                          (2, "a sequence id was out of range or repeated")) if bits & bit]
+        raise RuntimeError("4-bit cache: " + "; ".join(reasons))
+
+    def free_pages(self) -> int:
+        """Free pages of the pool (synchronises)."""
+        return int((self.refs == 0).sum().item())
+
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    return x if x.stride(-1) == 1 else x.contiguous()
+
+
+def _scale(softmax_scale: float | None) -> float:
+    return HEAD_DIM ** -0.5 if softmax_scale is None else float(softmax_scale)
