@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kWarps * 32) rows_kernel(
     for (int w = 0; w < kWarps; ++w) best = fmaxf(best, tops[w]);
     float total = 0.0f, value = 0.0f;
     for (int w = 0; w < kWarps; ++w) {
-        if (tops[w] == -INFINITY) continue;
+        if (sums[w] == 0.0f) continue;  // saw no token (a NaN sum goes on into the output)
         const float keep = __expf(tops[w] - best);
         total = __fmaf_rn(sums[w], keep, total);
         value = __fmaf_rn(accs[w][threadIdx.x], keep, value);
