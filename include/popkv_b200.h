@@ -675,6 +675,7 @@ typedef struct popkv_kv4_cache {
 
 #define POPKV_KV4_FULL 1     /* an extend found too few free pages or table columns, and did nothing */
 #define POPKV_KV4_SEQUENCE 2 /* a sequence id was out of range or repeated; its entry was skipped */
+#define POPKV_KV4_WAIT 4     /* an attention's bounded wait for its copies gave up: its output is incomplete */
 
 /*
  * Quantise keys and values of the LAST counts[i] (NULL: `tokens`) tokens of each
@@ -704,12 +705,19 @@ POPKV_API int popkv_kv4_read(const popkv_kv4_cache* cache, int64_t layer, const 
  * queries[i, j, h, d] is read at queries + i*q_seq_stride + j*q_token_stride +
  * h*q_head_stride + d, fp16 or bf16; query head h reads KV head h / (q_heads / kv_heads).
  * out [n, q_len, q_heads, 128] of the same type; rows j >= counts[i], and rows that see no
- * token, are zeros.
+ * token, are zeros.  Query rows are 16-byte aligned (strides multiples of 8).
+ * workspace: popkv_kv4_attention_workspace bytes, 16-byte aligned, zero before the first call;
+ * every call leaves it usable for the next, of any size that it holds.  Calls that overlap in
+ * time need a workspace each.
  */
 POPKV_API int popkv_kv4_attention(const popkv_kv4_cache* cache, int64_t layer, const int32_t* seqs, int64_t n,
                                   const int32_t* counts, const void* queries, int dtype, int64_t q_heads,
                                   int64_t q_len, int64_t q_seq_stride, int64_t q_token_stride,
-                                  int64_t q_head_stride, float scale, void* out, void* stream);
+                                  int64_t q_head_stride, float scale, void* workspace, int64_t workspace_bytes,
+                                  void* out, void* stream);
+
+/* Bytes of the workspace of either attention (q_len 1 for the selected one); -1 for invalid sizes. */
+POPKV_API int64_t popkv_kv4_attention_workspace(int64_t n, int64_t kv_heads, int64_t q_heads, int64_t q_len);
 
 /*
  * Attention of one token's query heads over the cached tokens that each selected:
@@ -720,8 +728,8 @@ POPKV_API int popkv_kv4_attention(const popkv_kv4_cache* cache, int64_t layer, c
 POPKV_API int popkv_kv4_attention_selected(const popkv_kv4_cache* cache, int64_t layer, const int32_t* seqs,
                                            int64_t n, const void* queries, int dtype, int64_t q_heads,
                                            int64_t q_seq_stride, int64_t q_head_stride, const int64_t* indices,
-                                           int64_t selected, const uint8_t* valid, float scale, void* out,
-                                           void* stream);
+                                           int64_t selected, const uint8_t* valid, float scale, void* workspace,
+                                           int64_t workspace_bytes, void* out, void* stream);
 
 /*
  * Page operations: they change the tables on the device, in stream order, without

@@ -74,8 +74,10 @@ _SIGNATURES = {
     "popkv_norm_gate_up_swiglu": ([_P, _L, _L, _L, _P, _P, _P, ctypes.c_float, _P, _P, _P], _I),
     "popkv_kv4_write": ([_P, _L, _P, _L, _P, _P, _P, _I, _L, _L, _L, _L, _L, _L, _L, _P], _I),
     "popkv_kv4_read": ([_P, _L, _P, _L, _L, _L, _P, _P, _I, _P], _I),
-    "popkv_kv4_attention": ([_P, _L, _P, _L, _P, _P, _I, _L, _L, _L, _L, _L, ctypes.c_float, _P, _P], _I),
-    "popkv_kv4_attention_selected": ([_P, _L, _P, _L, _P, _I, _L, _L, _L, _P, _L, _P, ctypes.c_float, _P, _P], _I),
+    "popkv_kv4_attention": ([_P, _L, _P, _L, _P, _P, _I, _L, _L, _L, _L, _L, ctypes.c_float, _P, _L, _P, _P], _I),
+    "popkv_kv4_attention_selected": ([_P, _L, _P, _L, _P, _I, _L, _L, _L, _P, _L, _P, ctypes.c_float, _P, _L, _P,
+                                      _P], _I),
+    "popkv_kv4_attention_workspace": ([_L, _L, _L, _L], _L),
     "popkv_kv4_extend": ([_P, _P, _L, _P, _L, _P, _P], _I),
     "popkv_kv4_fork": ([_P, _P, _P, _L, _P, _P], _I),
     "popkv_kv4_truncate": ([_P, _P, _L, _P, _P], _I),

@@ -118,6 +118,7 @@ class Kv4Cache:
             self.status.data_ptr(), self.layers, self.num_pages, self.kv_heads, self.page_size,
             self.dim_group_size, self.max_seqs, self.max_pages)
         self._address = ctypes.addressof(self._descriptor)
+        self._workspaces = {}  # of each stream: the attention's scratch and the sizes it holds
 
     # -- arguments -----------------------------------------------------------------
     def _call(self, entry, *args) -> None:
@@ -208,6 +209,33 @@ class Kv4Cache:
         return keys, values
 
     # -- attention -----------------------------------------------------------------
+    def workspace(self, n: int, q_heads: int, q_len: int = 1) -> torch.Tensor:
+        """Scratch for attention calls of up to these sizes, zeroed, for the ``workspace`` arguments.
+
+        Without one, calls keep one per stream; inside a graph capture, where that cannot be, each
+        call would allocate and clear its own.  Calls that overlap in time need one each.
+        """
+        size = _lib.lib().popkv_kv4_attention_workspace(n, self.kv_heads, q_heads, q_len)
+        if size < 0:
+            raise ValueError("query heads must be a multiple of the cache's KV heads")
+        return torch.zeros(size, dtype=torch.uint8, device=self.device)
+
+    def _workspace(self, given, n: int, q_heads: int, q_len: int) -> torch.Tensor:
+        if given is not None:
+            if given.dtype != torch.uint8 or not given.is_contiguous() or given.device != self.device:
+                raise ValueError("workspace must be a tensor of workspace()")
+            return given
+        key = torch.cuda.current_stream(self.device).cuda_stream
+        held = self._workspaces.get(key)
+        if held is not None and held[1] >= n and held[2] >= q_heads and held[3] >= q_len:
+            return held[0]
+        if torch.cuda.is_current_stream_capturing():
+            return self.workspace(n, q_heads, q_len)
+        sizes = (n, q_heads, q_len) if held is None else (max(n, held[1]), max(q_heads, held[2]), max(q_len, held[3]))
+        made = self.workspace(*sizes)
+        self._workspaces[key] = (made, *sizes)
+        return made
+
     def _queries(self, queries: torch.Tensor, seqs: torch.Tensor) -> torch.Tensor:
         if queries.shape[0] != seqs.shape[0] or queries.shape[-1] != HEAD_DIM:
             raise ValueError(f"queries must be [{seqs.shape[0]}, ..., query heads, {HEAD_DIM}]")
@@ -217,10 +245,14 @@ class Kv4Cache:
             raise RuntimeError("queries must be fp16 or bf16")
         if queries.device != self.device:
             raise RuntimeError("queries must be on the cache's device")
-        return _rows(queries)
+        if queries.stride(-1) != 1 or queries.data_ptr() % 16 or any(s % 8 for s in queries.stride()[:-1]):
+            queries = queries.contiguous()
+            if queries.data_ptr() % 16:
+                queries = queries.clone()
+        return queries
 
     def attention(self, queries: torch.Tensor, *, seqs, layer: int = 0, counts=None,
-                  softmax_scale: float | None = None) -> torch.Tensor:
+                  softmax_scale: float | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
         """Causal attention of each listed sequence's last tokens over all its tokens.
 
         queries: fp16/bf16 [n, q_len, q_heads, 128], or [n, q_heads, 128] for one token; row j of
@@ -235,16 +267,18 @@ class Kv4Cache:
         counts = None if counts is None else self._per_sequence(counts, seqs, "counts")
         out = torch.empty(queries.shape, dtype=queries.dtype, device=self.device)
         strides = queries.stride()
-        self._call(_lib.lib().popkv_kv4_attention, self._layer(layer), seqs.data_ptr(), seqs.shape[0],
+        n, q_heads, q_len = seqs.shape[0], queries.shape[-2], queries.shape[1] if queries.ndim == 4 else 1
+        scratch = self._workspace(workspace, n, q_heads, q_len)
+        self._call(_lib.lib().popkv_kv4_attention, self._layer(layer), seqs.data_ptr(), n,
                    None if counts is None else counts.data_ptr(), queries.data_ptr(),
-                   _lib.DTYPE_CODES[queries.dtype], queries.shape[-2],
-                   queries.shape[1] if queries.ndim == 4 else 1, strides[0], strides[1] if queries.ndim == 4 else 0,
-                   strides[-2], _scale(softmax_scale), out.data_ptr())
+                   _lib.DTYPE_CODES[queries.dtype], q_heads, q_len, strides[0],
+                   strides[1] if queries.ndim == 4 else 0, strides[-2], _scale(softmax_scale), scratch.data_ptr(),
+                   scratch.numel(), out.data_ptr())
         return out
 
     def attention_selected(self, queries: torch.Tensor, indices: torch.Tensor, *, seqs, layer: int = 0,
-                           valid_mask: torch.Tensor | None = None,
-                           softmax_scale: float | None = None) -> torch.Tensor:
+                           valid_mask: torch.Tensor | None = None, softmax_scale: float | None = None,
+                           workspace: torch.Tensor | None = None) -> torch.Tensor:
         """Attention of one token's query heads over the cached tokens that each selected.
 
         queries: fp16/bf16 [n, q_heads, 128]; indices: int64 [n, q_heads, selected] token positions
@@ -270,10 +304,11 @@ class Kv4Cache:
             valid_mask = valid_mask.contiguous()
         out = torch.empty(queries.shape, dtype=queries.dtype, device=self.device)
         strides = queries.stride()
+        scratch = self._workspace(workspace, seqs.shape[0], queries.shape[1], 1)
         self._call(_lib.lib().popkv_kv4_attention_selected, self._layer(layer), seqs.data_ptr(), seqs.shape[0],
                    queries.data_ptr(), _lib.DTYPE_CODES[queries.dtype], queries.shape[1], strides[0], strides[1],
                    indices.data_ptr(), indices.shape[2], None if valid_mask is None else valid_mask.data_ptr(),
-                   _scale(softmax_scale), out.data_ptr())
+                   _scale(softmax_scale), scratch.data_ptr(), scratch.numel(), out.data_ptr())
         return out
 
     # -- pages ---------------------------------------------------------------------
@@ -345,7 +380,8 @@ class Kv4Cache:
             return
         self.status[0] = 0
         reasons = [text for bit, text in ((1, "too few free pages or table columns for an extend"),
-                                          (2, "a sequence id was out of range or repeated")) if bits & bit]
+                                          (2, "a sequence id was out of range or repeated"),
+                                          (4, "an attention gave up waiting for its copies")) if bits & bit]
         raise RuntimeError("4-bit cache: " + "; ".join(reasons))
 
     def free_pages(self) -> int:
