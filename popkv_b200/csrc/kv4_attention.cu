@@ -26,7 +26,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kChunk = 32;    // tokens of one stage of a warp: two tiles
-constexpr int kStages = 3;
+constexpr int kStages = 2;
 constexpr int kDim = kKv4Dim;
 constexpr int kMergeStride = kDim + 4;  // floats of a row in the warps' merge: conflict-free float2 stores
 constexpr float kNothing = -1e30f;      // `top` before any token
@@ -79,6 +79,12 @@ __device__ __forceinline__ float2 floats_of(uint32_t pair) {
     return __half22float2(h);
 }
 
+__device__ __forceinline__ float high_of(uint32_t pair) {
+    __half2 h;
+    memcpy(&h, &pair, 4);
+    return __high2float(h);
+}
+
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -91,6 +97,15 @@ __device__ __forceinline__ void mma(float* c, uint32_t a0, uint32_t a1, uint32_t
         "{%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// The same with zeros for c.
+__device__ __forceinline__ void mma_new(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
 // The pairs of one token, NG words of fp16 (low, delta).
@@ -108,6 +123,7 @@ __device__ __forceinline__ void load_pairs(const uint8_t* p, uint32_t* pairs) {
 }
 
 constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;  // n and 16 n of two numbers, as fp16 denormals
+constexpr uint32_t kMinusEven = 0x80088008u, kMinusOdd = 0x80808080u;  // -8 and -16 * 8 likewise
 
 // A warp's running state for NT blocks of 8 query rows.  Lane (g = lane / 4, t = lane % 4)
 // holds, of each block, columns 2t and 2t + 1 of the results and column g of the
@@ -115,7 +131,7 @@ constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;  // n and 16 n of tw
 template <int NG, int NT>
 struct State {
     uint32_t q[NT][16];       // queries as fp16, scaled by a power of two per row
-    float q_sum[NT][NG][2];   // their sums over each group, times 2^-24
+    uint32_t q_sum[NT][2];    // their sums over group t, times 2^-6, in two fp16 terms
     float factor[NT][2];      // logits (times log2 e) of the scaled sums
     float top[NT][2];         // p = 2^(logit - top)
     float sum[NT][2];         // this lane's tokens
@@ -157,7 +173,7 @@ __device__ __forceinline__ void load_queries(const Params& p, State<NG, NT>& s, 
         const int exponent = static_cast<int>(__float_as_uint(most) >> 23) - 127;  // -127 for 0 and denormals
         const int up = most == 0.0f || exponent == 128 ? 0 : min(13 - exponent, 126);
         const float by = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
-        float sums[4];
+        float sum = 0.0f;  // of the group that this lane's q_sum is for
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             float total = 0.0f;
@@ -168,25 +184,22 @@ __device__ __forceinline__ void load_queries(const Params& p, State<NG, NT>& s, 
             }
             total += __shfl_xor_sync(0xFFFFFFFFu, total, 1);
             total += __shfl_xor_sync(0xFFFFFFFFu, total, 2);
-            sums[w] = total * 0x1p-24f;
+            if (w / (4 / NG) == t) sum += total;
             // Numbers i and i + 4 of a word share a register; odd ones come as 16 n.
             s.q[b][4 * w] = half2_of(x[w][0], x[w][4]);
             s.q[b][4 * w + 1] = half2_of(x[w][1] * 0.0625f, x[w][5] * 0.0625f);
             s.q[b][4 * w + 2] = half2_of(x[w][2], x[w][6]);
             s.q[b][4 * w + 3] = half2_of(x[w][3] * 0.0625f, x[w][7] * 0.0625f);
         }
+        sum *= 0x1p-6f;
+        const float high = __half2float(__float2half_rn(sum));
+        s.q_sum[b][0] = half2_of(high, 0.0f);
+        s.q_sum[b][1] = half2_of(sum - high, 0.0f);
         const float back = p.scale * __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * 0x1p24f;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const int from = (2 * t + c) * 4;
             s.factor[b][c] = __shfl_sync(0xFFFFFFFFu, back, from);
-#pragma unroll
-            for (int k = 0; k < NG; ++k) {
-                float total = 0.0f;
-#pragma unroll
-                for (int w = 0; w < 4 / NG; ++w) total += sums[k * (4 / NG) + w];
-                s.q_sum[b][k][c] = __shfl_sync(0xFFFFFFFFu, total, from);
-            }
             s.top[b][c] = kNothing;
             s.sum[b][c] = 0.0f;
 #pragma unroll
@@ -204,7 +217,7 @@ __device__ __forceinline__ void load_queries(const Params& p, State<NG, NT>& s, 
 // share their banks).
 __device__ __forceinline__ int token_at(int j) { return j ^ (j >> 1 & 1); }
 
-// Scaled logits of a tile's tokens token_at(g) (results 0, 1) and 8 + token_at(g) (2, 3).
+// Scaled sums of a tile's tokens token_at(g) (results 0, 1) and 8 + token_at(g) (2, 3).
 template <int NG, int NT>
 __device__ __forceinline__ void tile_logits(const State<NG, NT>& s, const uint8_t* tile, float (*x)[4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -212,33 +225,41 @@ __device__ __forceinline__ void tile_logits(const State<NG, NT>& s, const uint8_
     const uint4 a4 = *reinterpret_cast<const uint4*>(tile + token * kKv4RowBytes + 16 * t);
     const uint4 b4 = *reinterpret_cast<const uint4*>(tile + (token + 8) * kKv4RowBytes + 16 * t);
     const uint32_t wa[4] = {a4.x, a4.y, a4.z, a4.w}, wb[4] = {b4.x, b4.y, b4.z, b4.w};
+    const uint8_t* pairs = tile + kKv4PairOffset + token * 8 * NG;
     uint32_t pa[NG], pb[NG];
-    load_pairs<NG>(tile + kKv4PairOffset + token * 8 * NG, pa);
-    load_pairs<NG>(tile + kKv4PairOffset + (token + 8) * 8 * NG, pb);
+    load_pairs<NG>(pairs, pa);
+    load_pairs<NG>(pairs + 64 * NG, pb);
+    // The lows' share: rows (low, delta) of group t against (sum, 0), a product for all groups.
+    const uint32_t la = *reinterpret_cast<const uint32_t*>(pairs + 4 * (t & (NG - 1)));
+    const uint32_t lb = *reinterpret_cast<const uint32_t*>(pairs + 64 * NG + 4 * (t & (NG - 1)));
 #pragma unroll
-    for (int b = 0; b < NT; ++b)
+    for (int r = 0; r < NT; ++r) {
+        mma_new(x[r], la, lb, la, lb, s.q_sum[r][0], s.q_sum[r][1]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) x[b][c] = 0.0f;
+        for (int c = 0; c < 4; ++c) x[r][c] *= 0x1p-18f;
+    }
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
-        float dots[NT][4] = {};
+        float dots[NT][4];
 #pragma unroll
         for (int w = k * (4 / NG); w < (k + 1) * (4 / NG); ++w) {
             const uint32_t a = wa[w], b = wb[w], a8 = a >> 8, b8 = b >> 8;
 #pragma unroll
             for (int r = 0; r < NT; ++r) {
-                mma(dots[r], a & kEven, b & kEven, a & kOdd, b & kOdd, s.q[r][4 * w], s.q[r][4 * w + 1]);
+                if (w == k * (4 / NG))
+                    mma_new(dots[r], a & kEven, b & kEven, a & kOdd, b & kOdd, s.q[r][4 * w], s.q[r][4 * w + 1]);
+                else
+                    mma(dots[r], a & kEven, b & kEven, a & kOdd, b & kOdd, s.q[r][4 * w], s.q[r][4 * w + 1]);
                 mma(dots[r], a8 & kEven, b8 & kEven, a8 & kOdd, b8 & kOdd, s.q[r][4 * w + 2], s.q[r][4 * w + 3]);
             }
         }
-        const float2 fa = floats_of(pa[k]), fb = floats_of(pb[k]);
+        const float fa = high_of(pa[k]), fb = high_of(pb[k]);
 #pragma unroll
         for (int r = 0; r < NT; ++r) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                x[r][c] = __fmaf_rn(fa.y, dots[r][c], __fmaf_rn(fa.x, s.q_sum[r][k][c], x[r][c]));
-                x[r][2 + c] = __fmaf_rn(fb.y, dots[r][2 + c], __fmaf_rn(fb.x, s.q_sum[r][k][c], x[r][2 + c]));
-            }
+            x[r][0] = __fmaf_rn(fa, dots[r][0], x[r][0]);
+            x[r][1] = __fmaf_rn(fa, dots[r][1], x[r][1]);
+            x[r][2] = __fmaf_rn(fb, dots[r][2], x[r][2]);
+            x[r][3] = __fmaf_rn(fb, dots[r][3], x[r][3]);
         }
     }
 }
@@ -246,13 +267,17 @@ __device__ __forceinline__ void tile_logits(const State<NG, NT>& s, const uint8_
 // log2 of the largest value delta of a token (at least fp16's smallest).
 template <int NG>
 __device__ __forceinline__ float log2_delta(const uint32_t* pairs) {
-    float most = 0x1p-24f;
+    __half2 most, other;
+    memcpy(&most, pairs, 4);
 #pragma unroll
-    for (int k = 0; k < NG; ++k) most = fmaxf(most, floats_of(pairs[k]).y);
-    return log2_of(most);
+    for (int k = 1; k < NG; ++k) {
+        memcpy(&other, pairs + k, 4);
+        most = __hmax2(most, other);
+    }
+    return log2_of(fmaxf(__high2float(most), 0x1p-24f));
 }
 
-// Which tokens of a chunk a masked pass takes: bit j of `tokens`, and of those, for column
+// Which tokens of a tile a masked pass takes: bit j of `tokens`, and of those, for column
 // c of block b, the ones before `limit`.
 template <int NT>
 struct Mask {
@@ -261,51 +286,50 @@ struct Mask {
     int limit[NT][2];
 };
 
-// One chunk of two tiles: logits, weights, outputs.
+// One tile: logits, weights, outputs.
 template <int NG, int NT, bool kMasked>
-__device__ __forceinline__ void chunk(State<NG, NT>& s, const uint8_t* data, const Mask<NT>& mask) {
+__device__ __forceinline__ void tile_pass(State<NG, NT>& s, const uint8_t* tile, const Mask<NT>& mask) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    constexpr int kTile = kKv4PairOffset + kKv4TileTokens * 8 * NG;
     const int token = token_at(g);
-    float x[2][NT][4];
+    float x[NT][4];
+    tile_logits<NG, NT>(s, tile, x);
+    const uint8_t* own_pairs = tile + kKv4PairOffset + token * 8 * NG + 4 * NG;
+    uint32_t pairs[2][NG];
+    bool there[2];
+    float size[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        load_pairs<NG>(own_pairs + half * 64 * NG, pairs[half]);
+        there[half] = !kMasked || (mask.tokens >> (token + 8 * half) & 1u);
+        size[half] = log2_delta<NG>(pairs[half]);
+    }
     bool above = false;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const uint8_t* tile = data + h * kTile;
-        tile_logits<NG, NT>(s, tile, x[h]);
+    for (int b = 0; b < NT; ++b)
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            uint32_t pairs[NG];
-            const int at = token + 8 * half;
-            load_pairs<NG>(tile + kKv4PairOffset + at * 8 * NG + 4 * NG, pairs);
-            const bool there = !kMasked || (mask.tokens >> (16 * h + at) & 1u);
-            const float size = log2_delta<NG>(pairs);
+        for (int c = 0; c < 2; ++c) {
+            if (kMasked) {
 #pragma unroll
-            for (int b = 0; b < NT; ++b)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    float& v = x[h][b][2 * half + c];
+                for (int half = 0; half < 2; ++half) {
+                    // A factor may be negative (a negative scale): -inf is put in after it.
+                    float& v = x[b][2 * half + c];
                     v *= s.factor[b][c];
-                    if (kMasked && !(there && mask.base + 16 * h + at < mask.limit[b][c])) v = -INFINITY;
-                    above |= v + size > s.top[b][c] + (kHeadroom + kSlack);
+                    if (!(there[half] && mask.base + token + 8 * half < mask.limit[b][c])) v = -INFINITY;
                 }
+                above |= fmaxf(x[b][c] + size[0], x[b][2 + c] + size[1]) > s.top[b][c] + (kHeadroom + kSlack);
+            } else {
+                above |= fmaxf(__fmaf_rn(x[b][c], s.factor[b][c], size[0]),
+                               __fmaf_rn(x[b][2 + c], s.factor[b][c], size[1])) > s.top[b][c] + (kHeadroom + kSlack);
+            }
         }
-    }
     if (__any_sync(0xFFFFFFFFu, above)) {
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
             float scale[2];
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float most = -INFINITY;
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        uint32_t pairs[NG];
-                        load_pairs<NG>(data + h * kTile + kKv4PairOffset + (token + 8 * half) * 8 * NG + 4 * NG, pairs);
-                        most = fmaxf(most, x[h][b][2 * half + c] + log2_delta<NG>(pairs));
-                    }
+                const float by = kMasked ? 1.0f : s.factor[b][c];
+                float most = fmaxf(__fmaf_rn(x[b][c], by, size[0]), __fmaf_rn(x[b][2 + c], by, size[1]));
 #pragma unroll
                 for (int step = 4; step < 32; step *= 2)
                     most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, step));
@@ -325,52 +349,69 @@ __device__ __forceinline__ void chunk(State<NG, NT>& s, const uint8_t* data, con
             }
         }
     }
+    // Weights p * delta of this lane's two tokens, turned to the products' operand.
+    uint32_t weights[NT][NG][2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const uint8_t* tile = data + h * kTile;
-        // Weights p * delta of this lane's two tokens, turned to the products' operand.
-        uint32_t weights[NT][NG][2];
+    for (int half = 0; half < 2; ++half) {
+        float p[NT][2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            uint32_t pairs[NG];
-            const int at = token + 8 * half;
-            load_pairs<NG>(tile + kKv4PairOffset + at * 8 * NG + 4 * NG, pairs);
-            const bool there = !kMasked || (mask.tokens >> (16 * h + at) & 1u);
+        for (int b = 0; b < NT; ++b)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const float v = x[b][2 * half + c];
+                p[b][c] = exp2_of(kMasked ? v - s.top[b][c] : __fmaf_rn(v, s.factor[b][c], -s.top[b][c]));
+                s.sum[b][c] += p[b][c];
+            }
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+            float2 pair = floats_of(pairs[half][k]);
+            if (kMasked && !there[half]) pair = make_float2(0.0f, 0.0f);  // what lies there may be NaN
+            const float centre = __fmaf_rn(8.0f, pair.y, pair.x);
 #pragma unroll
             for (int b = 0; b < NT; ++b) {
-                const float p0 = exp2_of(x[h][b][2 * half] - s.top[b][0]);
-                const float p1 = exp2_of(x[h][b][2 * half + 1] - s.top[b][1]);
-                s.sum[b][0] += p0;
-                s.sum[b][1] += p1;
-#pragma unroll
-                for (int k = 0; k < NG; ++k) {
-                    float2 pair = floats_of(pairs[k]);
-                    if (kMasked && !there) pair = make_float2(0.0f, 0.0f);  // what lies there may be NaN
-                    s.low_sum[b][k][0] = __fmaf_rn(p0, pair.x, s.low_sum[b][k][0]);
-                    s.low_sum[b][k][1] = __fmaf_rn(p1, pair.x, s.low_sum[b][k][1]);
-                    weights[b][k][half] = transposed(half2_of(p0 * pair.y, p1 * pair.y));
-                }
+                s.low_sum[b][k][0] = __fmaf_rn(p[b][0], centre, s.low_sum[b][k][0]);
+                s.low_sum[b][k][1] = __fmaf_rn(p[b][1], centre, s.low_sum[b][k][1]);
+                weights[b][k][half] = transposed(half2_of(p[b][0] * pair.y, p[b][1] * pair.y));
             }
         }
-        // Value numbers of tokens j, j + 1 (and + 8) side by side, 16 dims at a time.
-        const uint8_t* values = tile + kKv4ValueOffset + 8 * g;
-        const int j = token_at(2 * t), j1 = token_at(2 * t + 1);
-        const uint2 v0 = *reinterpret_cast<const uint2*>(values + j * kKv4RowBytes);
-        const uint2 v1 = *reinterpret_cast<const uint2*>(values + j1 * kKv4RowBytes);
-        const uint2 v2 = *reinterpret_cast<const uint2*>(values + (j + 8) * kKv4RowBytes);
-        const uint2 v3 = *reinterpret_cast<const uint2*>(values + (j1 + 8) * kKv4RowBytes);
+    }
+    // Value numbers of tokens j, j + 1 (and + 8) side by side, 16 dims at a time.  They enter
+    // as n - 8, the 8 in a product of its own: the sums stay near zero, so that neither the
+    // weights' rounding nor the tensor cores' truncated additions are multiplied by the
+    // numbers' offset (over 131072 tokens: error 3.5 times smaller).
+    const uint8_t* values = tile + kKv4ValueOffset + 8 * g;
+    const int j = token_at(2 * t), j1 = token_at(2 * t + 1);
+    const uint2 v0 = *reinterpret_cast<const uint2*>(values + j * kKv4RowBytes);
+    const uint2 v1 = *reinterpret_cast<const uint2*>(values + j1 * kKv4RowBytes);
+    const uint2 v2 = *reinterpret_cast<const uint2*>(values + (j + 8) * kKv4RowBytes);
+    const uint2 v3 = *reinterpret_cast<const uint2*>(values + (j1 + 8) * kKv4RowBytes);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t pick = i & 1 ? 0x7632u : 0x5410u;
-            const uint32_t a = __byte_perm(i < 2 ? v0.x : v0.y, i < 2 ? v1.x : v1.y, pick);
-            const uint32_t c = __byte_perm(i < 2 ? v2.x : v2.y, i < 2 ? v3.x : v3.y, pick);
-            const int k = i * NG / 4;
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t pick = i & 1 ? 0x7632u : 0x5410u;
+        const uint32_t a = __byte_perm(i < 2 ? v0.x : v0.y, i < 2 ? v1.x : v1.y, pick);
+        const uint32_t c = __byte_perm(i < 2 ? v2.x : v2.y, i < 2 ? v3.x : v3.y, pick);
+        const int k = i * NG / 4;
 #pragma unroll
-            for (int b = 0; b < NT; ++b) {
-                mma(s.out[b][2 * i], a & kEven, a & kOdd, c & kEven, c & kOdd, weights[b][k][0], weights[b][k][1]);
-                mma(s.out[b][2 * i + 1], a >> 8 & kEven, a >> 8 & kOdd, c >> 8 & kEven, c >> 8 & kOdd,
-                    weights[b][k][0], weights[b][k][1]);
-            }
+        for (int b = 0; b < NT; ++b) {
+            const uint32_t w0 = weights[b][k][0], w1 = weights[b][k][1];
+            mma(s.out[b][2 * i], kMinusEven, kMinusOdd, kMinusEven, kMinusOdd, w0, w1);
+            mma(s.out[b][2 * i + 1], kMinusEven, kMinusOdd, kMinusEven, kMinusOdd, w0, w1);
+            mma(s.out[b][2 * i], a & kEven, a & kOdd, c & kEven, c & kOdd, w0, w1);
+            mma(s.out[b][2 * i + 1], a >> 8 & kEven, a >> 8 & kOdd, c >> 8 & kEven, c >> 8 & kOdd, w0, w1);
+        }
+    }
+}
+
+// One chunk of two tiles, mask.tokens and mask.base those of the chunk.
+template <int NG, int NT, bool kMasked>
+__device__ __forceinline__ void chunk_pass(State<NG, NT>& s, const uint8_t* data, Mask<NT>& mask) {
+    constexpr int kTile = kKv4PairOffset + kKv4TileTokens * 8 * NG;
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {
+        tile_pass<NG, NT, kMasked>(s, data + h * kTile, mask);
+        if (kMasked) {
+            mask.tokens >>= 16;
+            mask.base += 16;
         }
     }
 }
@@ -478,7 +519,7 @@ __device__ __forceinline__ void copy8(uint8_t* to, const uint8_t* from, bool the
 }
 
 template <int NG, int NT, bool kSelected>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attention_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) attention_kernel(const __grid_constant__ Params p) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t full[kWarps][kStages];
     __shared__ float merge_top[kWarps][8 * NT], merge_sum[kWarps][8 * NT];
@@ -497,7 +538,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attention_kernel(co
     const int rows = kSelected ? 1 : p.q_len * group;
     const int segments = heads * p.tiles;
     Place place = find_place<kSelected>(p, segments);
-    uint32_t waits = 0;  // stages waited for so far (slot and phase of the next)
+    int next_slot = 0;  // the stage to wait for, and its phase
+    uint32_t phase = 0;
     bool failed = false;
 
     for (int64_t at = place.begin; at < place.end;) {
@@ -529,70 +571,77 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attention_kernel(co
         const int todo = !failed && chunk0 + warp < stop ? (stop - chunk0 - warp + kWarps - 1) / kWarps : 0;
 
         if constexpr (!kSelected) {
-            // Pages of the warp's chunks, 32 chunks to a register: this lane's of the current 32 and of
-            // the next, read ahead of their use.
+            // Where the warp's chunks lie, 32 chunks to a register: this lane's of the current 32 and
+            // of the next, read ahead of their use; 0 where there is no page.  Pages of 16 tokens need
+            // a second address for the chunk's second tile.
             const int32_t* table = p.view.table + static_cast<int64_t>(seq) * p.view.max_pages;
             const bool small = p.view.page_shift == 4;
-            auto page_of = [&](int j, int half) {
+            const uint64_t base = reinterpret_cast<uint64_t>(p.view.tile_at(p.layer, 0, kv_head, 0));
+            auto address_of = [&](int j, int half) -> uint64_t {
                 const int position = (chunk0 + warp + j * kWarps) * kChunk + 16 * half;
-                if (j >= todo || position >= length) return -1;
-                return table[position >> p.view.page_shift];
+                if (j >= todo || position >= length) return 0;
+                const int page = table[position >> p.view.page_shift];
+                if (page < 0 || page >= p.view.num_pages) return 0;
+                return base + page * p.view.page_bytes + ((position & (p.view.page_size() - 1)) >> 4) * kTile;
             };
-            int now0 = page_of(lane, 0), now1 = small ? page_of(lane, 1) : now0;
-            int next0 = page_of(lane + 32, 0), next1 = small ? page_of(lane + 32, 1) : next0;
-            uint32_t missing = 0;  // two bits a slot
-            auto issue = [&](int j) {
+            uint64_t now0 = address_of(lane, 0), now1 = small ? address_of(lane, 1) : 0;
+            uint64_t next0 = address_of(lane + 32, 0), next1 = small ? address_of(lane + 32, 1) : 0;
+            // Chunks without a page, of the 32 being read and of the 32 being copied.
+            uint32_t gone0 = __ballot_sync(0xFFFFFFFFu, !now0), gone1 = small ? __ballot_sync(0xFFFFFFFFu, !now1) : gone0;
+            uint32_t late0 = gone0, late1 = gone1;
+            auto issue = [&](int j, int slot) {
                 if (j && (j & 31) == 0) {
                     now0 = next0, now1 = next1;
-                    next0 = page_of(j + 32 + lane, 0);
-                    next1 = small ? page_of(j + 32 + lane, 1) : next0;
+                    next0 = address_of(j + 32 + lane, 0);
+                    next1 = small ? address_of(j + 32 + lane, 1) : 0;
+                    late0 = __ballot_sync(0xFFFFFFFFu, !now0);
+                    late1 = small ? __ballot_sync(0xFFFFFFFFu, !now1) : late0;
                 }
-                const int page0 = __shfl_sync(0xFFFFFFFFu, now0, j & 31), page1 = __shfl_sync(0xFFFFFFFFu, now1, j & 31);
-                const bool has0 = page0 >= 0 && page0 < p.view.num_pages, has1 = page1 >= 0 && page1 < p.view.num_pages;
-                const int slot = (waits + j) % kStages;
-                missing = (missing & ~(3u << (2 * slot))) | (has0 ? 0u : 1u) << (2 * slot) | (has1 ? 0u : 2u) << (2 * slot);
+                const uint64_t from0 = __shfl_sync(0xFFFFFFFFu, now0, j & 31);
+                const uint64_t from1 = small ? __shfl_sync(0xFFFFFFFFu, now1, j & 31) : 0;
                 if (lane == 0) {
-                    const int position = (chunk0 + warp + j * kWarps) * kChunk;
                     uint8_t* to = ring + slot * kStageBytes;
                     uint64_t* bar = &full[warp][slot];
-                    mbar_arrive_expect_tx(bar, ((has0 ? 1 : 0) + (has1 ? 1 : 0)) * kTile);
-                    if (!small) {
-                        if (has0) bulk_copy_g2s(to, p.view.tile_at(p.layer, page0, kv_head, position), kStageBytes, bar);
-                    } else {
-                        if (has0) bulk_copy_g2s(to, p.view.tile_at(p.layer, page0, kv_head, position), kTile, bar);
-                        if (has1)
-                            bulk_copy_g2s(to + kTile, p.view.tile_at(p.layer, page1, kv_head, position + 16), kTile, bar);
-                    }
+                    const uint32_t part = small ? kTile : kStageBytes;
+                    mbar_arrive_expect_tx(bar, (from0 ? part : 0) + (from1 ? part : 0));
+                    if (from0) bulk_copy_g2s(to, reinterpret_cast<const void*>(from0), part, bar);
+                    if (from1) bulk_copy_g2s(to + kTile, reinterpret_cast<const void*>(from1), part, bar);
                 }
             };
-            for (int j = 0; j < min(kStages, todo); ++j) issue(j);
+            int slot = next_slot;
+            for (int j = 0; j < min(kStages, todo); ++j) {
+                issue(j, slot);
+                slot = slot + 1 == kStages ? 0 : slot + 1;
+            }
             load_queries<NG, NT>(p, state, entry, head0, group, first_row, rows);
-            const uint32_t start = waits;
             for (int j = 0; j < todo; ++j) {
-                const int slot = (start + j) % kStages;
-                if (!mbar_wait(&full[warp][slot], (start + j) / kStages & 1u)) {
+                if (!mbar_wait(&full[warp][next_slot], phase)) {
                     // A copy did not arrive in time: no further copies, and a last chance for those in flight.
                     failed = true;
-                    for (int k = j + 1; k < min(j + kStages, todo); ++k)
-                        mbar_wait(&full[warp][(start + k) % kStages], (start + k) / kStages & 1u);
+                    for (int k = 0; k < kStages; ++k) mbar_wait(&full[warp][k], k > next_slot ? phase : phase ^ 1u);
                     break;
                 }
+                if ((j & 31) == 0) gone0 = late0, gone1 = late1;
                 const int position = (chunk0 + warp + j * kWarps) * kChunk;
-                const uint32_t gone = missing >> (2 * slot) & 3u;
-                if (position + kChunk <= seen_by_all && !gone) {
-                    chunk<NG, NT, false>(state, ring + slot * kStageBytes, mask);
+                const bool has0 = !(gone0 >> (j & 31) & 1u), has1 = !(gone1 >> (j & 31) & 1u);
+                const uint8_t* data = ring + next_slot * kStageBytes;
+                if (position + kChunk <= seen_by_all && has0 && has1) {
+                    chunk_pass<NG, NT, false>(state, data, mask);
                 } else {
                     const int left = length - position;  // > 0
                     mask.tokens = left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1u;
-                    if (gone & 1u) mask.tokens &= 0xFFFF0000u;
-                    if (gone & 2u) mask.tokens &= 0x0000FFFFu;
+                    if (!has0) mask.tokens &= 0xFFFF0000u;
+                    if (!has1) mask.tokens &= 0x0000FFFFu;
                     mask.base = position;
-                    chunk<NG, NT, true>(state, ring + slot * kStageBytes, mask);
+                    chunk_pass<NG, NT, true>(state, data, mask);
                 }
                 __syncwarp();
-                if (j + kStages < todo) issue(j + kStages);
+                if (j + kStages < todo) issue(j + kStages, next_slot);
+                if (++next_slot == kStages) {
+                    next_slot = 0;
+                    phase ^= 1u;
+                }
             }
-            waits = start + todo;
         } else {
             load_queries<NG, NT>(p, state, entry, head0, group, first_row, rows);
             const int64_t row_at = (static_cast<int64_t>(entry) * p.q_heads + head) * p.selected;
@@ -655,16 +704,16 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 3 : 2) attention_kernel(co
 #pragma unroll
             for (int j = 0; j < kStages - 1; ++j) live[j] = issue(j);  // past the end: nothing is there
             live[kStages - 1] = 0;
-            mask.base = 0;
             for (int j = 0; j < todo; ++j) {
                 const uint32_t issued = issue(j + kStages - 1);
                 asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
                 __syncwarp();
                 mask.tokens = live[0];
+                mask.base = 0;
 #pragma unroll
                 for (int i = 0; i + 2 < kStages; ++i) live[i] = live[i + 1];
                 live[kStages - 2] = issued;
-                chunk<NG, NT, true>(state, ring + (j % kStages) * kStageBytes, mask);
+                chunk_pass<NG, NT, true>(state, ring + (j % kStages) * kStageBytes, mask);
                 __syncwarp();
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -815,7 +864,7 @@ int launch(const char* what, const Params& p, int64_t most_chunks, cudaStream_t 
     static_assert(kWarps * 8 * NT * kMergeStride * 4 <= kSmem, "the merge fits the ring");
     auto kernel = attention_kernel<NG, NT, kSelected>;
     if (int status = allow_dynamic_smem(kernel, kSmem)) return status;
-    constexpr int kPerSm = NT == 1 ? 3 : 2;
+    constexpr int kPerSm = NT == 1 ? 4 : 2;
     const int64_t ctas = (most_chunks + kWarps - 1) / kWarps;
     const unsigned grid = static_cast<unsigned>(ctas < 148 * kPerSm ? ctas : 148 * kPerSm);
     const cudaError_t err = launch_pdl(kernel, dim3(grid), dim3(kThreads), kSmem, stream, 1, p);
