@@ -16,6 +16,7 @@
 // are the 8 columns of both.  One pass over the cache serves every query row of a KV
 // head, and a warp needs no exchange with others until its tokens are through.
 #include <cmath>
+#include <type_traits>
 
 #include "kv4.cuh"
 #include "mbarrier.cuh"
@@ -23,10 +24,14 @@
 namespace popkv {
 namespace {
 
-constexpr int kWarps = 4;
+#ifndef KV4_H
+#define KV4_H 2
+#define KV4_W 8
+#define KV4_S 4
+#endif
+constexpr int kWarps = KV4_W;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kChunk = 32;    // tokens of one stage of a warp: two tiles
-constexpr int kStages = 2;
 constexpr int kDim = kKv4Dim;
 constexpr int kMergeStride = kDim + 4;  // floats of a row in the warps' merge: conflict-free float2 stores
 constexpr float kNothing = -1e30f;      // `top` before any token
@@ -108,98 +113,118 @@ __device__ __forceinline__ void mma_new(float* c, uint32_t a0, uint32_t a1, uint
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 
-// The pairs of one token, NG words of fp16 (low, delta).
-template <int NG>
-__device__ __forceinline__ void load_pairs(const uint8_t* p, uint32_t* pairs) {
-    if constexpr (NG == 4) {
-        const uint4 v = *reinterpret_cast<const uint4*>(p);
-        pairs[0] = v.x, pairs[1] = v.y, pairs[2] = v.z, pairs[3] = v.w;
-    } else if constexpr (NG == 2) {
-        const uint2 v = *reinterpret_cast<const uint2*>(p);
-        pairs[0] = v.x, pairs[1] = v.y;
-    } else {
-        pairs[0] = *reinterpret_cast<const uint32_t*>(p);
-    }
-}
-
 constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;  // n and 16 n of two numbers, as fp16 denormals
 constexpr uint32_t kMinusEven = 0x80088008u, kMinusOdd = 0x80808080u;  // -8 and -16 * 8 likewise
 
-// A warp's running state for NT blocks of 8 query rows.  Lane (g = lane / 4, t = lane % 4)
-// holds, of each block, columns 2t and 2t + 1 of the results and column g of the
-// queries; of the outputs dims 16 i + 2 g (+ 1) in block i.
-template <int NG, int NT>
+// Columns of the products: NT blocks of 8, of which a lane (g = lane / 4, t = lane % 4) holds
+// columns 2t and 2t + 1 of the results and column g of the operands.  With NC = 2 each column
+// is a query row; with NC = 1 (at most 4 rows) only the even ones are, so that every lane works
+// on one row and none on padding.
+template <int NT, int NC>
+struct Columns {
+    static constexpr int kRows = NC == 2 ? 8 * NT : 4;
+    __device__ static int row_of(int b, int t, int c) { return NC == 2 ? 8 * b + 2 * t + c : t; }
+};
+
+// A warp's running state.  Of the outputs a lane holds dims 16 i + 2 g (+ 1) in block i.
+template <int NG, int NT, int NC>
 struct State {
-    uint32_t q[NT][16];       // queries as fp16, scaled by a power of two per row
-    uint32_t q_sum[NT][2];    // their sums over group t, times 2^-6, in two fp16 terms
-    float factor[NT][2];      // logits (times log2 e) of the scaled sums
-    float top[NT][2];         // p = 2^(logit - top)
-    float sum[NT][2];         // this lane's tokens
-    float low_sum[NT][NG][2];
+    uint32_t q_sum[NT][2];     // their sums over group t, times 2^-6, in two fp16 terms
+    float factor[NT][NC];      // logits (times log2 e) of the scaled sums
+    float top[NT][NC];         // p = 2^(logit - top)
+    float sum[NT][NC];         // this lane's tokens
+    float low_sum[NT][NG][NC];
     float out[NT][8][4];
 };
 
-// Query rows of the tile, from row `first` of the KV head's q_len * group rows.
+// The queries of one row tile as the products take them, made once per segment by the CTA.
+template <int NT>
+struct Queries {
+    uint32_t q[NT][4][32][4];
+    uint2 q_sum[NT][32];
+    float factor[NT][8];
+};
+
+// The part of one CTA's work inside one segment: chunks [chunk0, chunk1) of a row tile of a KV
+// head (or of a query head's selected slots).
+struct Segment {
+    int entry, head0, kv_head, first_row, last_row;  // last_row: the last one with a token of its own
+    int seq, length, count, seen, seen_by_all;       // tokens that the last row sees, that all rows see
+    int chunk0, chunk1, number;
+    bool whole;
+};
+
+// Query rows of the tile as they are: 16 threads a column, each with 8 dims.
+template <int NT, int NC>
+__device__ __forceinline__ void load_queries(const Params& p, const Segment& segment, int group, int rows,
+                                             uint4* raw) {
+#pragma unroll
+    for (int k = 0; k < (NT * 128 + kThreads - 1) / kThreads; ++k) {
+        const int item = threadIdx.x + k * kThreads, column = item >> 4, word = item & 15;
+        const int row = segment.first_row + (NC == 2 ? column : column >> 1);
+        raw[k] = make_uint4(0u, 0u, 0u, 0u);
+        if (item < NT * 128 && row < rows && (NC == 2 || (column & 1) == 0))
+            raw[k] = *reinterpret_cast<const uint4*>(p.queries + segment.entry * p.q_seq + (row / group) * p.q_token +
+                                                     (segment.head0 + row % group) * p.q_head + 8 * word);
+    }
+}
+
 template <int NG, int NT>
-__device__ __forceinline__ void load_queries(const Params& p, State<NG, NT>& s, int entry, int head0, int group,
-                                             int first, int rows) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+__device__ __forceinline__ void stage_queries(const Params& p, Queries<NT>& s, const uint4* rows_read) {
 #pragma unroll
-    for (int b = 0; b < NT; ++b) {
-        const int row = first + 8 * b + g;
-        float most = 0.0f;
-        uint4 raw[4] = {};
-        if (row < rows) {
-            const uint16_t* at = p.queries + entry * p.q_seq + (row / group) * p.q_token +
-                                 (head0 + row % group) * p.q_head;
+    for (int k = 0; k < (NT * 128 + kThreads - 1) / kThreads; ++k) {
+        const int item = threadIdx.x + k * kThreads, column = item >> 4, word = item & 15;
+        if (item >= NT * 128) break;  // whole warps
+        const int b = column >> 3, g = column & 7, w = word >> 2, t = word & 3;
+        const uint4 raw = rows_read[k];
+        float x[8], most = 0.0f;
+        const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-            for (int w = 0; w < 4; ++w) raw[w] = *reinterpret_cast<const uint4*>(at + 8 * (4 * w + t));
+        for (int i = 0; i < 4; ++i) {
+            const float2 h = p.bf16 ? make_float2(bf16_lo(words[i]), bf16_hi(words[i])) : floats_of(words[i]);
+            x[2 * i] = h.x;
+            x[2 * i + 1] = h.y;
+            most = fmaxf(most, fmaxf(fabsf(h.x), fabsf(h.y)));
         }
-        float x[4][8];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const uint32_t words[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 h = floats_of(words[i]);
-                x[w][2 * i] = p.bf16 ? bf16_lo(words[i]) : h.x;
-                x[w][2 * i + 1] = p.bf16 ? bf16_hi(words[i]) : h.y;
-                most = fmaxf(most, fmaxf(fabsf(x[w][2 * i]), fabsf(x[w][2 * i + 1])));
-            }
-        }
-        most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
-        most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+        for (int step = 1; step < 16; step *= 2) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, step));
         // The largest of the row to [2^13, 2^14): exact in fp16 down to 2^-38 of it.
         const int exponent = static_cast<int>(__float_as_uint(most) >> 23) - 127;  // -127 for 0 and denormals
         const int up = most == 0.0f || exponent == 128 ? 0 : min(13 - exponent, 126);
         const float by = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
-        float sum = 0.0f;  // of the group that this lane's q_sum is for
+        float sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            float total = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[w][i] = __half2float(__float2half_rn(x[w][i] * by));
-                total += x[w][i];
-            }
-            total += __shfl_xor_sync(0xFFFFFFFFu, total, 1);
-            total += __shfl_xor_sync(0xFFFFFFFFu, total, 2);
-            if (w / (4 / NG) == t) sum += total;
-            // Numbers i and i + 4 of a word share a register; odd ones come as 16 n.
-            s.q[b][4 * w] = half2_of(x[w][0], x[w][4]);
-            s.q[b][4 * w + 1] = half2_of(x[w][1] * 0.0625f, x[w][5] * 0.0625f);
-            s.q[b][4 * w + 2] = half2_of(x[w][2], x[w][6]);
-            s.q[b][4 * w + 3] = half2_of(x[w][3] * 0.0625f, x[w][7] * 0.0625f);
+        for (int i = 0; i < 8; ++i) {
+            x[i] = __half2float(__float2half_rn(x[i] * by));
+            sum += x[i];
         }
+        // Numbers i and i + 4 of a word share a register; odd ones come as 16 n.
+        *reinterpret_cast<uint4*>(s.q[b][w][g * 4 + t]) =
+            make_uint4(half2_of(x[0], x[4]), half2_of(x[1] * 0.0625f, x[5] * 0.0625f), half2_of(x[2], x[6]),
+                       half2_of(x[3] * 0.0625f, x[7] * 0.0625f));
+        constexpr int kWords = 16 / NG;  // words of a group
+#pragma unroll
+        for (int step = 1; step < kWords; step *= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, step);
         sum *= 0x1p-6f;
         const float high = __half2float(__float2half_rn(sum));
-        s.q_sum[b][0] = half2_of(high, 0.0f);
-        s.q_sum[b][1] = half2_of(sum - high, 0.0f);
-        const float back = p.scale * __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * 0x1p24f;
+        if (word % kWords == 0)
+            s.q_sum[b][g * 4 + word / kWords] = make_uint2(half2_of(high, 0.0f), half2_of(sum - high, 0.0f));
+        if (NG < 4 && word < 4 && word >= NG) s.q_sum[b][g * 4 + word] = make_uint2(0u, 0u);
+        if (word == 0)
+            s.factor[b][g] = p.scale * __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * 0x1p24f;
+    }
+}
+
+template <int NG, int NT, int NC>
+__device__ __forceinline__ void start_state(State<NG, NT, NC>& s, const Queries<NT>& from) {
+    const int lane = threadIdx.x & 31, t = lane & 3;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int from = (2 * t + c) * 4;
-            s.factor[b][c] = __shfl_sync(0xFFFFFFFFu, back, from);
+    for (int b = 0; b < NT; ++b) {
+        const uint2 sums = from.q_sum[b][lane];
+        s.q_sum[b][0] = sums.x, s.q_sum[b][1] = sums.y;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            s.factor[b][c] = from.factor[b][2 * t + c];
             s.top[b][c] = kNothing;
             s.sum[b][c] = 0.0f;
 #pragma unroll
@@ -217,119 +242,202 @@ __device__ __forceinline__ void load_queries(const Params& p, State<NG, NT>& s, 
 // share their banks).
 __device__ __forceinline__ int token_at(int j) { return j ^ (j >> 1 & 1); }
 
-// Scaled sums of a tile's tokens token_at(g) (results 0, 1) and 8 + token_at(g) (2, 3).
-template <int NG, int NT>
-__device__ __forceinline__ void tile_logits(const State<NG, NT>& s, const uint8_t* tile, float (*x)[4]) {
+// A lane's places in a tile, kept in registers (the compiler would compute them again for
+// each tile): its two tokens' keys, pairs and group-t pair, and its tokens' values.
+struct Lane {
+    uint32_t keys, pairs, low, values, queries;
+    uint32_t minus[4];  // the operand of -8: a register each, which the products want side by side
+};
+
+template <int NG>
+__device__ __forceinline__ Lane lane_places(const void* queries) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int token = token_at(g);
-    const uint4 a4 = *reinterpret_cast<const uint4*>(tile + token * kKv4RowBytes + 16 * t);
-    const uint4 b4 = *reinterpret_cast<const uint4*>(tile + (token + 8) * kKv4RowBytes + 16 * t);
+    Lane at;
+    at.keys = token_at(g) * kKv4RowBytes + 16 * t;
+    at.pairs = kKv4PairOffset + token_at(g) * 8 * NG;
+    at.low = at.pairs + 4 * (t & (NG - 1));
+    at.values = kKv4ValueOffset + token_at(2 * t) * kKv4RowBytes + 8 * g;
+    at.queries = smem_addr(queries) + 16 * lane;
+    at.minus[0] = at.minus[2] = kMinusEven;
+    at.minus[1] = at.minus[3] = kMinusOdd;
+    asm volatile("" : "+r"(at.keys), "+r"(at.pairs), "+r"(at.low), "+r"(at.values));
+    asm volatile("" : "+r"(at.minus[0]), "+r"(at.minus[1]), "+r"(at.minus[2]), "+r"(at.minus[3]));
+    return at;
+}
+
+template <typename T>
+__device__ __forceinline__ T shared_load(uint32_t at);
+template <>
+__device__ __forceinline__ uint32_t shared_load(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+template <>
+__device__ __forceinline__ uint2 shared_load(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+    return v;
+}
+template <>
+__device__ __forceinline__ uint4 shared_load(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+
+// The pairs of one token, NG words of fp16 (low, delta).
+template <int NG>
+__device__ __forceinline__ void load_pairs(uint32_t at, uint32_t* pairs) {
+    if constexpr (NG == 4) {
+        const uint4 v = shared_load<uint4>(at);
+        pairs[0] = v.x, pairs[1] = v.y, pairs[2] = v.z, pairs[3] = v.w;
+    } else if constexpr (NG == 2) {
+        const uint2 v = shared_load<uint2>(at);
+        pairs[0] = v.x, pairs[1] = v.y;
+    } else {
+        pairs[0] = shared_load<uint32_t>(at);
+    }
+}
+
+// Numbers 2, 3 (and 6, 7) of a word where 0, 1 (and 4, 5) were.
+__device__ __forceinline__ uint32_t upper_numbers(uint32_t word) { return __byte_perm(word, 0u, 0x4341u); }
+
+// Scaled sums of a tile's tokens token_at(g) (results 0, 1) and 8 + token_at(g) (2, 3).
+template <int NG, int NT, int NC>
+__device__ __forceinline__ void tile_logits(const State<NG, NT, NC>& s, uint32_t tile, const Lane& at,
+                                            float (*x)[4]) {
+    const uint4 a4 = shared_load<uint4>(tile + at.keys), b4 = shared_load<uint4>(tile + at.keys + 8 * kKv4RowBytes);
     const uint32_t wa[4] = {a4.x, a4.y, a4.z, a4.w}, wb[4] = {b4.x, b4.y, b4.z, b4.w};
-    const uint8_t* pairs = tile + kKv4PairOffset + token * 8 * NG;
     uint32_t pa[NG], pb[NG];
-    load_pairs<NG>(pairs, pa);
-    load_pairs<NG>(pairs + 64 * NG, pb);
+    load_pairs<NG>(tile + at.pairs, pa);
+    load_pairs<NG>(tile + at.pairs + 64 * NG, pb);
     // The lows' share: rows (low, delta) of group t against (sum, 0), a product for all groups.
-    const uint32_t la = *reinterpret_cast<const uint32_t*>(pairs + 4 * (t & (NG - 1)));
-    const uint32_t lb = *reinterpret_cast<const uint32_t*>(pairs + 64 * NG + 4 * (t & (NG - 1)));
+    const uint32_t la = shared_load<uint32_t>(tile + at.low), lb = shared_load<uint32_t>(tile + at.low + 64 * NG);
 #pragma unroll
     for (int r = 0; r < NT; ++r) {
         mma_new(x[r], la, lb, la, lb, s.q_sum[r][0], s.q_sum[r][1]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) x[r][c] *= 0x1p-18f;
+        for (int c = 0; c < NC; ++c) {
+            x[r][c] *= 0x1p-18f;
+            x[r][2 + c] *= 0x1p-18f;
+        }
     }
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
         float dots[NT][4];
 #pragma unroll
         for (int w = k * (4 / NG); w < (k + 1) * (4 / NG); ++w) {
-            const uint32_t a = wa[w], b = wb[w], a8 = a >> 8, b8 = b >> 8;
+            const uint32_t a = wa[w], b = wb[w], a8 = upper_numbers(a), b8 = upper_numbers(b);
 #pragma unroll
             for (int r = 0; r < NT; ++r) {
+                const uint4 q = shared_load<uint4>(at.queries + (4 * r + w) * 512);
                 if (w == k * (4 / NG))
-                    mma_new(dots[r], a & kEven, b & kEven, a & kOdd, b & kOdd, s.q[r][4 * w], s.q[r][4 * w + 1]);
+                    mma_new(dots[r], a & kEven, b & kEven, a & kOdd, b & kOdd, q.x, q.y);
                 else
-                    mma(dots[r], a & kEven, b & kEven, a & kOdd, b & kOdd, s.q[r][4 * w], s.q[r][4 * w + 1]);
-                mma(dots[r], a8 & kEven, b8 & kEven, a8 & kOdd, b8 & kOdd, s.q[r][4 * w + 2], s.q[r][4 * w + 3]);
+                    mma(dots[r], a & kEven, b & kEven, a & kOdd, b & kOdd, q.x, q.y);
+                mma(dots[r], a8 & kEven, b8 & kEven, a8 & kOdd, b8 & kOdd, q.z, q.w);
             }
         }
         const float fa = high_of(pa[k]), fb = high_of(pb[k]);
 #pragma unroll
         for (int r = 0; r < NT; ++r) {
-            x[r][0] = __fmaf_rn(fa, dots[r][0], x[r][0]);
-            x[r][1] = __fmaf_rn(fa, dots[r][1], x[r][1]);
-            x[r][2] = __fmaf_rn(fb, dots[r][2], x[r][2]);
-            x[r][3] = __fmaf_rn(fb, dots[r][3], x[r][3]);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                x[r][c] = __fmaf_rn(fa, dots[r][c], x[r][c]);
+                x[r][2 + c] = __fmaf_rn(fb, dots[r][2 + c], x[r][2 + c]);
+            }
         }
     }
 }
 
-// log2 of the largest value delta of a token (at least fp16's smallest).
+// log2 of the largest value delta of two tokens (at least fp16's smallest).
 template <int NG>
-__device__ __forceinline__ float log2_delta(const uint32_t* pairs) {
+__device__ __forceinline__ float log2_delta(const uint32_t (*pairs)[NG]) {
     __half2 most, other;
-    memcpy(&most, pairs, 4);
+    memcpy(&most, pairs[0], 4);
 #pragma unroll
-    for (int k = 1; k < NG; ++k) {
-        memcpy(&other, pairs + k, 4);
+    for (int k = 1; k < 2 * NG; ++k) {
+        memcpy(&other, pairs[0] + k, 4);
         most = __hmax2(most, other);
     }
     return log2_of(fmaxf(__high2float(most), 0x1p-24f));
 }
 
-// Which tokens of a tile a masked pass takes: bit j of `tokens`, and of those, for column
+// Which tokens of a chunk a masked pass takes: bit j of `tokens`, and of those, for column
 // c of block b, the ones before `limit`.
-template <int NT>
+template <int NT, int NC>
 struct Mask {
     uint32_t tokens;
     int base;
-    int limit[NT][2];
+    int limit[NT][NC];
 };
 
-// One tile: logits, weights, outputs.
-template <int NG, int NT, bool kMasked>
-__device__ __forceinline__ void tile_pass(State<NG, NT>& s, const uint8_t* tile, const Mask<NT>& mask) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int token = token_at(g);
-    float x[NT][4];
-    tile_logits<NG, NT>(s, tile, x);
-    const uint8_t* own_pairs = tile + kKv4PairOffset + token * 8 * NG + 4 * NG;
-    uint32_t pairs[2][NG];
-    bool there[2];
-    float size[2];
+// With NC = 1 the odd columns of the weights are free: two groups share a register, one in the
+// even and one in the odd columns, and the outputs of a group's dims are taken from its columns.
+template <int NG, int NC>
+constexpr int kGroupsPerWeight = NC == 1 && NG > 1 ? 2 : 1;
+
+// Result column of block i's dims that holds column c's row.
+template <int NG, int NC>
+__device__ constexpr int out_column(int i, int c) {
+    return kGroupsPerWeight<NG, NC> == 2 ? (i * NG / 8) & 1 : c;
+}
+
+// H tiles of a chunk, the first being tile `number`: logits, weights, outputs.
+template <int NG, int NT, int NC, int H, bool kMasked>
+__device__ __forceinline__ void tiles_pass(State<NG, NT, NC>& s, uint32_t data, const Lane& at, int number,
+                                           const Mask<NT, NC>& mask) {
+    constexpr int kPer = kGroupsPerWeight<NG, NC>;
+    constexpr int kTile = kKv4PairOffset + kKv4TileTokens * 8 * NG;
+    float x[H][NT][4];
+    float size = -INFINITY;
+    bool there[H][2];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        load_pairs<NG>(own_pairs + half * 64 * NG, pairs[half]);
-        there[half] = !kMasked || (mask.tokens >> (token + 8 * half) & 1u);
-        size[half] = log2_delta<NG>(pairs[half]);
+    for (int h = 0; h < H; ++h) {
+        const uint32_t tile = data + h * kTile;
+        tile_logits<NG, NT, NC>(s, tile, at, x[h]);
+        uint32_t pairs[2][NG];
+        const int token = 16 * (number + h) + token_at((threadIdx.x & 31) >> 2);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            there[h][half] = !kMasked || (mask.tokens >> (token + 8 * half) & 1u);
+            load_pairs<NG>(tile + at.pairs + 4 * NG + half * 64 * NG, pairs[half]);
+            if (kMasked && !there[h][half]) {  // what lies there may be infinite or NaN
+#pragma unroll
+                for (int k = 0; k < NG; ++k) pairs[half][k] = 0u;
+            }
+        }
+        size = fmaxf(size, log2_delta<NG>(pairs));
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int b = 0; b < NT; ++b)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    float& v = x[h][b][2 * half + c];
+                    v *= s.factor[b][c];  // may be negative (a negative scale), so -inf comes after it
+                    if (kMasked && !(there[h][half] && token + 8 * half < mask.limit[b][c] - mask.base)) v = -INFINITY;
+                }
     }
+    auto largest = [&](int b, int c) {
+        float most = fmaxf(x[0][b][c], x[0][b][2 + c]);
+#pragma unroll
+        for (int h = 1; h < H; ++h) most = fmaxf(most, fmaxf(x[h][b][c], x[h][b][2 + c]));
+        return most + size;
+    };
     bool above = false;
 #pragma unroll
     for (int b = 0; b < NT; ++b)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            if (kMasked) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    // A factor may be negative (a negative scale): -inf is put in after it.
-                    float& v = x[b][2 * half + c];
-                    v *= s.factor[b][c];
-                    if (!(there[half] && mask.base + token + 8 * half < mask.limit[b][c])) v = -INFINITY;
-                }
-                above |= fmaxf(x[b][c] + size[0], x[b][2 + c] + size[1]) > s.top[b][c] + (kHeadroom + kSlack);
-            } else {
-                above |= fmaxf(__fmaf_rn(x[b][c], s.factor[b][c], size[0]),
-                               __fmaf_rn(x[b][2 + c], s.factor[b][c], size[1])) > s.top[b][c] + (kHeadroom + kSlack);
-            }
-        }
+        for (int c = 0; c < NC; ++c) above |= largest(b, c) > s.top[b][c] + (kHeadroom + kSlack);
     if (__any_sync(0xFFFFFFFFu, above)) {
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
-            float scale[2];
+            float scale[NC];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const float by = kMasked ? 1.0f : s.factor[b][c];
-                float most = fmaxf(__fmaf_rn(x[b][c], by, size[0]), __fmaf_rn(x[b][2 + c], by, size[1]));
+            for (int c = 0; c < NC; ++c) {
+                float most = largest(b, c);
 #pragma unroll
                 for (int step = 4; step < 32; step *= 2)
                     most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, step));
@@ -341,91 +449,109 @@ __device__ __forceinline__ void tile_pass(State<NG, NT>& s, const uint8_t* tile,
                 for (int k = 0; k < NG; ++k) s.low_sum[b][k][c] *= scale[c];
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                s.out[b][i][0] *= scale[0];
-                s.out[b][i][1] *= scale[1];
-                s.out[b][i][2] *= scale[0];
-                s.out[b][i][3] *= scale[1];
-            }
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    s.out[b][i][c] *= scale[NC == 1 ? 0 : c];
+                    s.out[b][i][2 + c] *= scale[NC == 1 ? 0 : c];
+                }
         }
     }
-    // Weights p * delta of this lane's two tokens, turned to the products' operand.
-    uint32_t weights[NT][NG][2];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        float p[NT][2];
+    for (int h = 0; h < H; ++h) {
+        const uint32_t tile = data + h * kTile;
+        // Weights p * delta of this lane's two tokens, turned to the products' operand.
+        uint32_t weights[NT][NG / kPer][2];
+        uint32_t pairs[2][NG];
+        load_pairs<NG>(tile + at.pairs + 4 * NG, pairs[0]);
+        load_pairs<NG>(tile + at.pairs + 4 * NG + 64 * NG, pairs[1]);
 #pragma unroll
-        for (int b = 0; b < NT; ++b)
+        for (int half = 0; half < 2; ++half) {
+            float p[NT][NC];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const float v = x[b][2 * half + c];
-                p[b][c] = exp2_of(kMasked ? v - s.top[b][c] : __fmaf_rn(v, s.factor[b][c], -s.top[b][c]));
-                s.sum[b][c] += p[b][c];
+            for (int b = 0; b < NT; ++b)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    p[b][c] = exp2_of(x[h][b][2 * half + c] - s.top[b][c]);
+                    s.sum[b][c] += p[b][c];
+                }
+            float delta[NG];
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+                float2 pair = floats_of(pairs[half][k]);
+                if (kMasked && !there[h][half]) pair = make_float2(0.0f, 0.0f);
+                const float centre = __fmaf_rn(8.0f, pair.y, pair.x);
+                delta[k] = pair.y;
+#pragma unroll
+                for (int b = 0; b < NT; ++b)
+#pragma unroll
+                    for (int c = 0; c < NC; ++c)
+                        s.low_sum[b][k][c] = __fmaf_rn(p[b][c], centre, s.low_sum[b][k][c]);
             }
 #pragma unroll
-        for (int k = 0; k < NG; ++k) {
-            float2 pair = floats_of(pairs[half][k]);
-            if (kMasked && !there[half]) pair = make_float2(0.0f, 0.0f);  // what lies there may be NaN
-            const float centre = __fmaf_rn(8.0f, pair.y, pair.x);
+            for (int k = 0; k < NG; k += kPer)
+#pragma unroll
+                for (int b = 0; b < NT; ++b)
+                    weights[b][k / kPer][half] =
+                        transposed(half2_of(p[b][0] * delta[k], NC == 2     ? p[b][NC - 1] * delta[k]
+                                                                : kPer == 2 ? p[b][0] * delta[k + kPer - 1]
+                                                                            : 0.0f));
+        }
+        // Value numbers of tokens j, j + 1 (and + 8) side by side, 16 dims at a time.  They enter
+        // as n - 8, the 8 in a product of its own: the sums stay near zero, so that neither the
+        // weights' rounding nor the tensor cores' truncated additions are multiplied by the
+        // numbers' offset (over 131072 tokens: error 3.5 times smaller).
+        const uint32_t values = tile + at.values, others = values ^ kKv4RowBytes;  // token_at(2t + 1) = token_at(2t) ^ 1
+        const uint2 v0 = shared_load<uint2>(values), v1 = shared_load<uint2>(others);
+        const uint2 v2 = shared_load<uint2>(values + 8 * kKv4RowBytes), v3 = shared_load<uint2>(others + 8 * kKv4RowBytes);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t pick = i & 1 ? 0x7632u : 0x5410u;
+            const uint32_t a = __byte_perm(i < 2 ? v0.x : v0.y, i < 2 ? v1.x : v1.y, pick);
+            const uint32_t c = __byte_perm(i < 2 ? v2.x : v2.y, i < 2 ? v3.x : v3.y, pick);
+            const uint32_t a8 = upper_numbers(a), c8 = upper_numbers(c);
+            const int k = i * NG / 4 / kPer;
 #pragma unroll
             for (int b = 0; b < NT; ++b) {
-                s.low_sum[b][k][0] = __fmaf_rn(p[b][0], centre, s.low_sum[b][k][0]);
-                s.low_sum[b][k][1] = __fmaf_rn(p[b][1], centre, s.low_sum[b][k][1]);
-                weights[b][k][half] = transposed(half2_of(p[b][0] * pair.y, p[b][1] * pair.y));
+                const uint32_t w0 = weights[b][k][0], w1 = weights[b][k][1];
+                mma(s.out[b][2 * i], at.minus[0], at.minus[1], at.minus[2], at.minus[3], w0, w1);
+                mma(s.out[b][2 * i + 1], at.minus[0], at.minus[1], at.minus[2], at.minus[3], w0, w1);
+                mma(s.out[b][2 * i], a & kEven, a & kOdd, c & kEven, c & kOdd, w0, w1);
+                mma(s.out[b][2 * i + 1], a8 & kEven, a8 & kOdd, c8 & kEven, c8 & kOdd, w0, w1);
             }
-        }
-    }
-    // Value numbers of tokens j, j + 1 (and + 8) side by side, 16 dims at a time.  They enter
-    // as n - 8, the 8 in a product of its own: the sums stay near zero, so that neither the
-    // weights' rounding nor the tensor cores' truncated additions are multiplied by the
-    // numbers' offset (over 131072 tokens: error 3.5 times smaller).
-    const uint8_t* values = tile + kKv4ValueOffset + 8 * g;
-    const int j = token_at(2 * t), j1 = token_at(2 * t + 1);
-    const uint2 v0 = *reinterpret_cast<const uint2*>(values + j * kKv4RowBytes);
-    const uint2 v1 = *reinterpret_cast<const uint2*>(values + j1 * kKv4RowBytes);
-    const uint2 v2 = *reinterpret_cast<const uint2*>(values + (j + 8) * kKv4RowBytes);
-    const uint2 v3 = *reinterpret_cast<const uint2*>(values + (j1 + 8) * kKv4RowBytes);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t pick = i & 1 ? 0x7632u : 0x5410u;
-        const uint32_t a = __byte_perm(i < 2 ? v0.x : v0.y, i < 2 ? v1.x : v1.y, pick);
-        const uint32_t c = __byte_perm(i < 2 ? v2.x : v2.y, i < 2 ? v3.x : v3.y, pick);
-        const int k = i * NG / 4;
-#pragma unroll
-        for (int b = 0; b < NT; ++b) {
-            const uint32_t w0 = weights[b][k][0], w1 = weights[b][k][1];
-            mma(s.out[b][2 * i], kMinusEven, kMinusOdd, kMinusEven, kMinusOdd, w0, w1);
-            mma(s.out[b][2 * i + 1], kMinusEven, kMinusOdd, kMinusEven, kMinusOdd, w0, w1);
-            mma(s.out[b][2 * i], a & kEven, a & kOdd, c & kEven, c & kOdd, w0, w1);
-            mma(s.out[b][2 * i + 1], a >> 8 & kEven, a >> 8 & kOdd, c >> 8 & kEven, c >> 8 & kOdd, w0, w1);
         }
     }
 }
 
-// One chunk of two tiles, mask.tokens and mask.base those of the chunk.
-template <int NG, int NT, bool kMasked>
-__device__ __forceinline__ void chunk_pass(State<NG, NT>& s, const uint8_t* data, Mask<NT>& mask) {
+// One chunk of two tiles, together where that leaves the registers for it.
+template <int NG, int NT, int NC, bool kMasked>
+__device__ __forceinline__ void chunk_pass(State<NG, NT, NC>& s, uint32_t data, const Lane& at,
+                                           const Mask<NT, NC>& mask) {
     constexpr int kTile = kKv4PairOffset + kKv4TileTokens * 8 * NG;
+    constexpr int kTogether = NT == 1 ? KV4_H : 1;
 #pragma unroll 1
-    for (int h = 0; h < 2; ++h) {
-        tile_pass<NG, NT, kMasked>(s, data + h * kTile, mask);
-        if (kMasked) {
-            mask.tokens >>= 16;
-            mask.base += 16;
-        }
-    }
+    for (int h = 0; h < 2; h += kTogether)
+        tiles_pass<NG, NT, NC, kTogether, kMasked>(s, data + h * kTile, at, h, mask);
 }
 
 __device__ __forceinline__ uint16_t rounded(float v, int bf16) {
     return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
 
-// The work of one CTA: chunks [begin, end) of the flat list of all (entry, head, row
-// tile) segments' chunks, of which `first` lie before the current entry.
+// The work of one CTA: chunks [begin, end) of the flat list of all (entry, head, row tile)
+// segments' chunks, of which `first` lie before the current entry.  With `parts` every
+// segment is cut into that many, one to a CTA; with 0 the list is cut into even shares, and
+// a CTA may end one segment and begin the next.
 struct Place {
-    int64_t begin, end, all, first;
-    int ctas, entry, chunks;
+    int64_t begin, end, first;
+    int share, parts, entry, chunks;
 };
+
+// a / b, a >= 0: by 32-bit division wherever that holds.
+__device__ __forceinline__ int64_t quotient(int64_t a, int b) {
+    if (a >> 32 == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
 
 template <bool kSelected>
 __device__ __forceinline__ int chunks_of(const Params& p, int entry) {
@@ -433,38 +559,81 @@ __device__ __forceinline__ int chunks_of(const Params& p, int entry) {
     return max(1, (tokens + kChunk - 1) / kChunk);  // one even if empty: it writes the zeros
 }
 
-// An even share of the chunks for each CTA, at least one per warp.  The lengths are in
-// device memory, so every CTA finds its share by itself.
+// The CTA's place.  The lengths are in device memory, so every CTA finds its own.
+//
+// Segments of one length (a single sequence, or selected slots) are cut into equal parts, one to a
+// CTA, where that costs no more than a quarter over even shares: each further segment that a CTA
+// enters costs it about 5 us of latency (queries, page lookups, first copies, merge).  At 32 x 8
+// heads x 32768 tokens on 296 CTAs: 37 parts a head against shares that straddle heads.
 template <bool kSelected>
 __device__ Place find_place(const Params& p, int segments) {
     __shared__ int64_t sums[kWarps];
+    __shared__ int extremes[2][kWarps];
     __shared__ int64_t found_first;
     __shared__ int found_entry, found_chunks;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     Place place;
     const int mine = threadIdx.x < p.n ? chunks_of<kSelected>(p, threadIdx.x) : 0;
+    int64_t all;
+    int least, most;
     if (kSelected) {
-        place.all = static_cast<int64_t>(p.n) * segments * max(1, (p.selected + kChunk - 1) / kChunk);
+        least = most = max(1, (p.selected + kChunk - 1) / kChunk);
+        all = static_cast<int64_t>(p.n) * segments * most;
     } else {
         int64_t total = mine;
-        for (int i = threadIdx.x + kThreads; i < p.n; i += kThreads) total += chunks_of<kSelected>(p, i);
+        least = mine ? mine : 0x7FFFFFFF;
+        most = mine;
+        for (int i = threadIdx.x + kThreads; i < p.n; i += kThreads) {
+            const int chunks = chunks_of<kSelected>(p, i);
+            total += chunks;
+            least = min(least, chunks);
+            most = max(most, chunks);
+        }
+        least = __reduce_min_sync(0xFFFFFFFFu, least);
+        most = __reduce_max_sync(0xFFFFFFFFu, most);
 #pragma unroll
         for (int step = 16; step > 0; step /= 2) total += __shfl_xor_sync(0xFFFFFFFFu, total, step);
-        if (lane == 0) sums[warp] = total;
+        if (lane == 0) {
+            sums[warp] = total;
+            extremes[0][warp] = least;
+            extremes[1][warp] = most;
+        }
         __syncthreads();
-        place.all = (sums[0] + sums[1] + sums[2] + sums[3]) * segments;
+        all = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            all += sums[w];
+            least = min(least, extremes[0][w]);
+            most = max(most, extremes[1][w]);
+        }
+        all *= segments;
         __syncthreads();
     }
-    place.ctas = static_cast<int>(min(static_cast<int64_t>(gridDim.x), (place.all + kWarps - 1) / kWarps));
-    place.begin = blockIdx.x * place.all / place.ctas;
-    place.end = (blockIdx.x + int64_t{1}) * place.all / place.ctas;
-    if (blockIdx.x >= static_cast<unsigned>(place.ctas)) {
-        place.begin = place.end = 0;
-        return place;
+    const int ctas = gridDim.x, number = p.n * segments;
+    const int floor_share = min(kWarps, static_cast<int>(quotient(all, number)));  // a chunk to each warp
+    place.share = max(floor_share, static_cast<int>(quotient(all + ctas - 1, ctas)));
+    place.parts = 0;
+    if (least == most && number <= ctas) {
+        const int parts = ctas / number;
+        const int share = max(floor_share, (most + parts - 1) / parts);
+        if (share - place.share <= place.share / 4) {
+            place.share = share;
+            place.parts = (most + share - 1) / share;
+            const int segment = blockIdx.x / place.parts, part = blockIdx.x - segment * place.parts;
+            place.chunks = most;
+            place.entry = segment / segments;
+            place.first = static_cast<int64_t>(place.entry) * segments * most;
+            place.begin = static_cast<int64_t>(segment) * most + part * share;
+            place.end = segment < number ? min(place.begin + share, static_cast<int64_t>(segment + 1) * most) : 0;
+            return place;
+        }
     }
+    place.begin = static_cast<int64_t>(blockIdx.x) * place.share;
+    place.end = min(place.begin + place.share, all);
+    if (place.begin >= all) return place;
     if (kSelected) {
-        place.chunks = max(1, (p.selected + kChunk - 1) / kChunk);
-        place.entry = static_cast<int>(place.begin / (static_cast<int64_t>(place.chunks) * segments));
+        place.chunks = most;
+        place.entry = static_cast<int>(quotient(place.begin, place.chunks) / segments);
         place.first = static_cast<int64_t>(place.entry) * place.chunks * segments;
         return place;
     }
@@ -488,7 +657,8 @@ __device__ Place find_place(const Params& p, int segments) {
             found_entry = i;
             found_chunks = chunks;
         }
-        before += sums[0] + sums[1] + sums[2] + sums[3];
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) before += sums[w];
         __syncthreads();
         if (place.begin < before * segments) break;
     }
@@ -496,16 +666,6 @@ __device__ Place find_place(const Params& p, int segments) {
     place.entry = found_entry;
     place.chunks = found_chunks;
     return place;
-}
-
-// The CTA whose share holds flat chunk `at`.
-__device__ __forceinline__ int owner_of(const Place& place, int64_t at) {
-    return static_cast<int>(((at + 1) * place.ctas - 1) / place.all);
-}
-
-template <int NG, int NT>
-constexpr int smem_bytes() {
-    return kWarps * kStages * 2 * (kKv4PairOffset + kKv4TileTokens * 8 * NG);
 }
 
 // 16-byte (or 8-byte) copy into shared memory, zeros where `there` is false.
@@ -518,16 +678,212 @@ __device__ __forceinline__ void copy8(uint8_t* to, const uint8_t* from, bool the
                  : "memory");
 }
 
-template <int NG, int NT, bool kSelected>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) attention_kernel(const __grid_constant__ Params p) {
+template <int NG, int NT, int NC>
+struct Sizes {
+    static constexpr int kTile = kKv4PairOffset + kKv4TileTokens * 8 * NG;
+    static constexpr int kStageBytes = 2 * kTile;
+    static constexpr int kStages = NT == 1 ? KV4_S : NT == 2 ? 3 : 2;  // chunks of a warp in flight: what fits
+    static constexpr int kRing = kWarps * kStages * kStageBytes;
+    static constexpr int kMerge = kWarps * Columns<NT, NC>::kRows * kMergeStride * 4;
+};
+
+template <bool kSelected, int kRows>
+__device__ __forceinline__ Segment segment_at(const Params& p, const Place& place, int64_t at, int segments, int group,
+                                              int rows) {
+    Segment s;
+    const int64_t offset = at - place.first;
+    s.number = static_cast<int>(quotient(offset, place.chunks));
+    s.chunk0 = static_cast<int>(offset - static_cast<int64_t>(s.number) * place.chunks);
+    s.chunk1 = static_cast<int>(min(static_cast<int64_t>(place.chunks), s.chunk0 + (place.end - at)));
+    s.whole = s.chunk0 == 0 && s.chunk1 == place.chunks;
+    s.entry = place.entry;
+    const int head = s.number / p.tiles;
+    s.first_row = (s.number - head * p.tiles) * kRows;
+    s.seq = p.seqs[s.entry];
+    s.length = p.view.length_of(s.seq);
+    s.count = kSelected ? 1 : p.counts ? min(p.counts[s.entry], p.q_len) : p.q_len;
+    s.kv_head = kSelected ? head / group : head;
+    s.head0 = kSelected ? head : head * group;
+    s.last_row = min(s.first_row + kRows, min(rows, s.count * group)) - 1;
+    s.seen = kSelected ? p.selected
+             : s.last_row < s.first_row ? 0 : max(0, s.length - s.count + s.last_row / group + 1);
+    s.seen_by_all = kSelected ? 0 : max(0, s.length - s.count + s.first_row / group + 1);
+    return s;
+}
+
+// Chunks of a warp: every kWarps-th of the segment's part.
+struct Share {
+    int first, todo;
+};
+
+__device__ __forceinline__ Share share_of(const Segment& s, bool none) {
+    const int warp = threadIdx.x >> 5, stop = min(s.chunk1, (s.seen + kChunk - 1) / kChunk);
+    Share share;
+    share.first = s.chunk0 + warp;
+    share.todo = !none && share.first < stop ? (stop - share.first + kWarps - 1) / kWarps : 0;
+    return share;
+}
+
+// Copies a warp's chunks of consecutive tokens: one bulk copy each (two where pages hold one
+// tile), issued by one lane, from addresses that the lanes look up 32 chunks at a time.
+template <int kTile>
+struct TokenCopies {
+    uint64_t now0, now1, next0, next1;  // of this lane's chunk of the 32, by tile; 0 where there is no page
+    uint32_t gone0, gone1;              // chunks without a page, of the 32 in use
+    uint32_t late0, late1;              // and of the 32 being copied
+    const int32_t* table;
+    uint64_t base;
+    Share share;
+    int length;
+    bool small;
+
+    __device__ __forceinline__ uint64_t address_of(const Params& p, int j, int half) const {
+        const int position = (share.first + j * kWarps) * kChunk + 16 * half;
+        if (j >= share.todo || position >= length) return 0;
+        const int page = table[position >> p.view.page_shift];
+        if (page < 0 || page >= p.view.num_pages) return 0;
+        return base + page * p.view.page_bytes + ((position & (p.view.page_size() - 1)) >> 4) * kTile;
+    }
+    __device__ __forceinline__ void start(const Params& p, const Segment& s, const Share& chunks) {
+        const int lane = threadIdx.x & 31;
+        share = chunks;
+        length = s.length;
+        small = p.view.page_shift == 4;
+        table = p.view.table + static_cast<int64_t>(p.view.has_sequence(s.seq) ? s.seq : 0) * p.view.max_pages;
+        base = reinterpret_cast<uint64_t>(p.view.tile_at(p.layer, 0, s.kv_head, 0));
+        now0 = address_of(p, lane, 0);
+        now1 = small ? address_of(p, lane, 1) : 0;
+        next0 = share.todo > 32 ? address_of(p, lane + 32, 0) : 0;
+        next1 = share.todo > 32 && small ? address_of(p, lane + 32, 1) : 0;
+        late0 = __ballot_sync(0xFFFFFFFFu, !now0);
+        late1 = small ? __ballot_sync(0xFFFFFFFFu, !now1) : late0;
+        gone0 = late0;
+        gone1 = late1;
+    }
+    __device__ __forceinline__ void issue(const Params& p, int j, uint8_t* to, uint64_t* bar) {
+        const int lane = threadIdx.x & 31;
+        if (j && (j & 31) == 0) {
+            now0 = next0, now1 = next1;
+            next0 = address_of(p, j + 32 + lane, 0);
+            next1 = small ? address_of(p, j + 32 + lane, 1) : 0;
+            late0 = __ballot_sync(0xFFFFFFFFu, !now0);
+            late1 = small ? __ballot_sync(0xFFFFFFFFu, !now1) : late0;
+        }
+        const uint64_t from0 = __shfl_sync(0xFFFFFFFFu, now0, j & 31);
+        const uint64_t from1 = small ? __shfl_sync(0xFFFFFFFFu, now1, j & 31) : 0;
+        if (lane == 0) {
+            const uint32_t part = small ? kTile : 2 * kTile;
+            mbar_arrive_expect_tx(bar, (from0 ? part : 0) + (from1 ? part : 0));
+            if (from0) bulk_copy_g2s(to, reinterpret_cast<const void*>(from0), part, bar);
+            if (from1) bulk_copy_g2s(to + kTile, reinterpret_cast<const void*>(from1), part, bar);
+        }
+    }
+};
+
+// Copies a warp's chunks of selected slots: lane l resolves slot l (indices are read two chunks
+// ahead of their copies, pages one), the copies of a row go over neighbouring lanes.
+template <int NG, int kTile>
+struct SlotCopies {
+    int64_t index0, index1;
+    int64_t row_at;
+    int page0, seq, length, kv_head;
+    Share share;
+
+    __device__ __forceinline__ int64_t index_of(const Params& p, int j) const {
+        const int slot = (share.first + j * kWarps) * kChunk + static_cast<int>(threadIdx.x & 31);
+        if (j >= share.todo || slot >= p.selected) return -1;
+        if (p.valid && !p.valid[row_at + slot]) return -1;
+        const int64_t index = p.indices[row_at + slot];
+        return index < length ? index : -1;
+    }
+    __device__ __forceinline__ int page_of(const Params& p, int64_t index) const {
+        return index < 0 ? -1 : p.view.page_at(seq, static_cast<int>(index));
+    }
+    __device__ __forceinline__ void start(const Params& p, const Segment& s, const Share& chunks) {
+        share = chunks;
+        seq = s.seq;
+        length = s.length;
+        kv_head = s.kv_head;
+        row_at = (static_cast<int64_t>(s.entry) * p.q_heads + s.head0) * p.selected;
+        index0 = index_of(p, 0);
+        index1 = index_of(p, 1);
+        page0 = page_of(p, index0);
+    }
+    // Returns the slots of chunk j that hold a token (past the end: none).
+    __device__ __forceinline__ uint32_t issue(const Params& p, int j, uint8_t* to) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+        const bool there = page0 >= 0;
+        const int position = static_cast<int>(index0), at = there ? position & 15 : 0;
+        const uint64_t tile = reinterpret_cast<uint64_t>(there ? p.view.tile_at(p.layer, page0, kv_head, position)
+                                                               : p.view.pages);
+        const uint64_t key_row = tile + at * kKv4RowBytes, pair_row = tile + kKv4PairOffset + at * 8 * NG;
+        const uint32_t live = __ballot_sync(0xFFFFFFFFu, there);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // 8 tokens, 4 lanes each
+            const int token = 8 * i + g;
+            const uint64_t from = __shfl_sync(0xFFFFFFFFu, key_row, token) + 16 * t;
+            uint8_t* line = to + (token >> 4) * kTile + (token & 15) * kKv4RowBytes + 16 * t;
+            const bool has = live >> token & 1u;
+            copy16(line, reinterpret_cast<const uint8_t*>(from), has);
+            copy16(line + kKv4ValueOffset, reinterpret_cast<const uint8_t*>(from) + kKv4ValueOffset, has);
+        }
+        uint8_t* pairs = to + kKv4PairOffset;
+        if constexpr (NG == 4) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int token = 16 * i + (lane >> 1);
+                const uint64_t from = __shfl_sync(0xFFFFFFFFu, pair_row, token) + 16 * (lane & 1);
+                copy16(pairs + i * kTile + (lane >> 1) * 32 + 16 * (lane & 1), reinterpret_cast<const uint8_t*>(from),
+                       live >> token & 1u);
+            }
+        } else {
+            uint8_t* line = pairs + (lane >> 4) * kTile + (lane & 15) * 8 * NG;
+            if constexpr (NG == 2)
+                copy16(line, reinterpret_cast<const uint8_t*>(pair_row), there);
+            else
+                copy8(line, reinterpret_cast<const uint8_t*>(pair_row), there);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        index0 = index1;
+        page0 = page_of(p, index0);
+        index1 = index_of(p, j + 2);
+        return live;
+    }
+};
+
+// A running softmax of one row over parts that were computed apart, 4 dims to a lane.
+struct Join {
+    float top = kNothing, sum = 0.0f;
+    float4 value = {0.0f, 0.0f, 0.0f, 0.0f};
+
+    __device__ __forceinline__ void add(float2 head, float4 v) {
+        const float both = fmaxf(top, head.x);
+        const float keep = exp2_of(top - both), take = exp2_of(head.x - both);
+        top = both;
+        sum = __fmaf_rn(sum, keep, head.y * take);
+        value.x = __fmaf_rn(value.x, keep, v.x * take);
+        value.y = __fmaf_rn(value.y, keep, v.y * take);
+        value.z = __fmaf_rn(value.z, keep, v.z * take);
+        value.w = __fmaf_rn(value.w, keep, v.w * take);
+    }
+};
+
+template <int NG, int NT, int NC, bool kSelected>
+__global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ Params p) {
+    using Size = Sizes<NG, NT, NC>;
+    constexpr int kTile = Size::kTile, kStageBytes = Size::kStageBytes, kStages = Size::kStages;
+    constexpr int kRows = Columns<NT, NC>::kRows;
+    constexpr int kPartFloats = kRows * (kDim + 2);
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ Queries<NT> staged;
     __shared__ uint64_t full[kWarps][kStages];
-    __shared__ float merge_top[kWarps][8 * NT], merge_sum[kWarps][8 * NT];
+    __shared__ float2 merge_heads[kWarps][kRows];
     __shared__ int is_last;
-    constexpr int kTile = kKv4PairOffset + kKv4TileTokens * 8 * NG;
-    constexpr int kStageBytes = 2 * kTile;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     uint8_t* ring = smem + warp * kStages * kStageBytes;
+    float* merged = reinterpret_cast<float*>(smem + Size::kRing);
+    const uint32_t ring_at = smem_addr(ring);
+    const Lane lanes = lane_places<NG>(staged.q);
     if (!kSelected && lane == 0)
         for (int i = 0; i < kStages; ++i) mbar_init(&full[warp][i], 1);
     pdl_wait();
@@ -538,195 +894,119 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) attention_kernel(co
     const int rows = kSelected ? 1 : p.q_len * group;
     const int segments = heads * p.tiles;
     Place place = find_place<kSelected>(p, segments);
+    if (place.begin >= place.end) return;
     int next_slot = 0;  // the stage to wait for, and its phase
     uint32_t phase = 0;
     bool failed = false;
+    uint32_t live[kStages];
+    using Copies = std::conditional_t<kSelected, SlotCopies<NG, kTile>, TokenCopies<kTile>>;
+    Copies copies;
+    uint4 raw[(NT * 128 + kThreads - 1) / kThreads];
 
-    for (int64_t at = place.begin; at < place.end;) {
-        const int64_t offset = at - place.first;
-        const int segment = static_cast<int>(offset / place.chunks);
-        const int chunk0 = static_cast<int>(offset - static_cast<int64_t>(segment) * place.chunks);
-        const int chunk1 = static_cast<int>(min(static_cast<int64_t>(place.chunks), chunk0 + (place.end - at)));
-        const int entry = place.entry, head = segment / p.tiles;
-        const int first_row = (segment - head * p.tiles) * 8 * NT;
-        const int seq = p.seqs[entry];
-        const int length = p.view.length_of(seq);
-        const int count = kSelected ? 1 : p.counts ? min(p.counts[entry], p.q_len) : p.q_len;
-        const int kv_head = kSelected ? head / group : head;
-        const int head0 = kSelected ? head : head * group;
-        // Tokens that the tile's last row sees, and those that all its rows see.
-        const int last_row = min(first_row + 8 * NT, min(rows, count * group)) - 1;
-        const int seen = kSelected ? p.selected : last_row < first_row ? 0 : max(0, length - count + last_row / group + 1);
-        const int seen_by_all = kSelected ? 0 : max(0, length - count + first_row / group + 1);
-        State<NG, NT> state;
-        Mask<NT> mask;
+    // The first copies of a segment's part, and its queries.
+    auto begin = [&](const Segment& s) {
+        copies.start(p, s, share_of(s, failed));
+        if constexpr (kSelected) {
+#pragma unroll
+            for (int j = 0; j < kStages - 1; ++j) live[j] = copies.issue(p, j, ring + j * kStageBytes);
+        } else {
+            int slot = next_slot;
+            for (int j = 0; j < min(kStages, copies.share.todo); ++j) {
+                copies.issue(p, j, ring + slot * kStageBytes, &full[warp][slot]);
+                slot = slot + 1 == kStages ? 0 : slot + 1;
+            }
+        }
+        load_queries<NT, NC>(p, s, group, rows, raw);
+    };
+
+    int64_t at = place.begin;
+    Segment segment = segment_at<kSelected, kRows>(p, place, at, segments, group, rows);
+    begin(segment);
+    stage_queries<NG, NT>(p, staged, raw);
+    __syncthreads();
+    while (true) {
+        State<NG, NT, NC> state;
+        start_state<NG, NT, NC>(state, staged);
+        Mask<NT, NC> mask;
 #pragma unroll
         for (int b = 0; b < NT; ++b)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const int row = first_row + 8 * b + 2 * t + c;
-                mask.limit[b][c] = kSelected || row > last_row ? 0x7FFFFFFF : length - count + row / group + 1;
+            for (int c = 0; c < NC; ++c) {
+                const int row = segment.first_row + Columns<NT, NC>::row_of(b, t, c);
+                mask.limit[b][c] =
+                    kSelected || row > segment.last_row ? 0x7FFFFFFF : segment.length - segment.count + row / group + 1;
             }
-        const int stop = min(chunk1, (seen + kChunk - 1) / kChunk);
-        const int todo = !failed && chunk0 + warp < stop ? (stop - chunk0 - warp + kWarps - 1) / kWarps : 0;
-
-        if constexpr (!kSelected) {
-            // Where the warp's chunks lie, 32 chunks to a register: this lane's of the current 32 and
-            // of the next, read ahead of their use; 0 where there is no page.  Pages of 16 tokens need
-            // a second address for the chunk's second tile.
-            const int32_t* table = p.view.table + static_cast<int64_t>(seq) * p.view.max_pages;
-            const bool small = p.view.page_shift == 4;
-            const uint64_t base = reinterpret_cast<uint64_t>(p.view.tile_at(p.layer, 0, kv_head, 0));
-            auto address_of = [&](int j, int half) -> uint64_t {
-                const int position = (chunk0 + warp + j * kWarps) * kChunk + 16 * half;
-                if (j >= todo || position >= length) return 0;
-                const int page = table[position >> p.view.page_shift];
-                if (page < 0 || page >= p.view.num_pages) return 0;
-                return base + page * p.view.page_bytes + ((position & (p.view.page_size() - 1)) >> 4) * kTile;
-            };
-            uint64_t now0 = address_of(lane, 0), now1 = small ? address_of(lane, 1) : 0;
-            uint64_t next0 = address_of(lane + 32, 0), next1 = small ? address_of(lane + 32, 1) : 0;
-            // Chunks without a page, of the 32 being read and of the 32 being copied.
-            uint32_t gone0 = __ballot_sync(0xFFFFFFFFu, !now0), gone1 = small ? __ballot_sync(0xFFFFFFFFu, !now1) : gone0;
-            uint32_t late0 = gone0, late1 = gone1;
-            auto issue = [&](int j, int slot) {
-                if (j && (j & 31) == 0) {
-                    now0 = next0, now1 = next1;
-                    next0 = address_of(j + 32 + lane, 0);
-                    next1 = small ? address_of(j + 32 + lane, 1) : 0;
-                    late0 = __ballot_sync(0xFFFFFFFFu, !now0);
-                    late1 = small ? __ballot_sync(0xFFFFFFFFu, !now1) : late0;
-                }
-                const uint64_t from0 = __shfl_sync(0xFFFFFFFFu, now0, j & 31);
-                const uint64_t from1 = small ? __shfl_sync(0xFFFFFFFFu, now1, j & 31) : 0;
-                if (lane == 0) {
-                    uint8_t* to = ring + slot * kStageBytes;
-                    uint64_t* bar = &full[warp][slot];
-                    const uint32_t part = small ? kTile : kStageBytes;
-                    mbar_arrive_expect_tx(bar, (from0 ? part : 0) + (from1 ? part : 0));
-                    if (from0) bulk_copy_g2s(to, reinterpret_cast<const void*>(from0), part, bar);
-                    if (from1) bulk_copy_g2s(to + kTile, reinterpret_cast<const void*>(from1), part, bar);
-                }
-            };
-            int slot = next_slot;
-            for (int j = 0; j < min(kStages, todo); ++j) {
-                issue(j, slot);
-                slot = slot + 1 == kStages ? 0 : slot + 1;
+        if constexpr (kSelected) {
+            mask.base = 0;
+            for (int j = 0; j < copies.share.todo; ++j) {
+                const uint32_t issued = copies.issue(p, j + kStages - 1, ring + ((j + kStages - 1) % kStages) * kStageBytes);
+                asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+                __syncwarp();
+                mask.tokens = live[0];
+#pragma unroll
+                for (int i = 0; i + 2 < kStages; ++i) live[i] = live[i + 1];
+                live[kStages - 2] = issued;
+                chunk_pass<NG, NT, NC, true>(state, ring_at + (j % kStages) * kStageBytes, lanes, mask);
+                __syncwarp();
             }
-            load_queries<NG, NT>(p, state, entry, head0, group, first_row, rows);
-            for (int j = 0; j < todo; ++j) {
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncwarp();
+        } else {
+            for (int j = 0; j < copies.share.todo; ++j) {
                 if (!mbar_wait(&full[warp][next_slot], phase)) {
                     // A copy did not arrive in time: no further copies, and a last chance for those in flight.
                     failed = true;
                     for (int k = 0; k < kStages; ++k) mbar_wait(&full[warp][k], k > next_slot ? phase : phase ^ 1u);
                     break;
                 }
-                if ((j & 31) == 0) gone0 = late0, gone1 = late1;
-                const int position = (chunk0 + warp + j * kWarps) * kChunk;
-                const bool has0 = !(gone0 >> (j & 31) & 1u), has1 = !(gone1 >> (j & 31) & 1u);
-                const uint8_t* data = ring + next_slot * kStageBytes;
-                if (position + kChunk <= seen_by_all && has0 && has1) {
-                    chunk_pass<NG, NT, false>(state, data, mask);
+                if ((j & 31) == 0) copies.gone0 = copies.late0, copies.gone1 = copies.late1;
+                const int position = (copies.share.first + j * kWarps) * kChunk;
+                const bool has0 = !(copies.gone0 >> (j & 31) & 1u), has1 = !(copies.gone1 >> (j & 31) & 1u);
+                const uint32_t data = ring_at + next_slot * kStageBytes;
+                if (position + kChunk <= segment.seen_by_all && has0 && has1) {
+                    chunk_pass<NG, NT, NC, false>(state, data, lanes, mask);
                 } else {
-                    const int left = length - position;  // > 0
+                    const int left = segment.length - position;  // > 0
                     mask.tokens = left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1u;
                     if (!has0) mask.tokens &= 0xFFFF0000u;
                     if (!has1) mask.tokens &= 0x0000FFFFu;
                     mask.base = position;
-                    chunk_pass<NG, NT, true>(state, data, mask);
+                    chunk_pass<NG, NT, NC, true>(state, data, lanes, mask);
                 }
                 __syncwarp();
-                if (j + kStages < todo) issue(j + kStages, next_slot);
+                if (j + kStages < copies.share.todo)
+                    copies.issue(p, j + kStages, ring + next_slot * kStageBytes, &full[warp][next_slot]);
                 if (++next_slot == kStages) {
                     next_slot = 0;
                     phase ^= 1u;
                 }
             }
-        } else {
-            load_queries<NG, NT>(p, state, entry, head0, group, first_row, rows);
-            const int64_t row_at = (static_cast<int64_t>(entry) * p.q_heads + head) * p.selected;
-            // Lane l resolves slot l of a chunk: the address of its key row, and its row in the tile.
-            // Indices are read two chunks ahead of their copies, pages one.
-            auto index_of = [&](int j) -> int64_t {
-                const int slot = (chunk0 + warp + j * kWarps) * kChunk + lane;
-                if (j >= todo || slot >= p.selected) return -1;
-                if (p.valid && !p.valid[row_at + slot]) return -1;
-                const int64_t index = p.indices[row_at + slot];
-                return index < length ? index : -1;
-            };
-            auto page_of = [&](int64_t index) {
-                return index < 0 ? -1 : p.view.page_at(seq, static_cast<int>(index));
-            };
-            int64_t index0 = index_of(0), index1 = index_of(1);
-            int page0 = page_of(index0);
-            auto issue = [&](int j) {
-                const bool there = page0 >= 0;
-                const int position = static_cast<int>(index0);
-                const uint8_t* tile = there ? p.view.tile_at(p.layer, page0, kv_head, position) : p.view.pages;
-                const uint64_t key_row = reinterpret_cast<uint64_t>(tile) + (there ? position & 15 : 0) * kKv4RowBytes;
-                const uint64_t pair_row =
-                    reinterpret_cast<uint64_t>(tile) + kKv4PairOffset + (there ? position & 15 : 0) * 8 * NG;
-                const uint32_t live = __ballot_sync(0xFFFFFFFFu, there);
-                const int slot = j % kStages;
-                uint8_t* to = ring + slot * kStageBytes;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {  // 8 tokens, 4 lanes each
-                    const int token = 8 * i + g;
-                    const uint64_t from = __shfl_sync(0xFFFFFFFFu, key_row, token) + 16 * t;
-                    uint8_t* line = to + (token >> 4) * kTile + (token & 15) * kKv4RowBytes + 16 * t;
-                    const bool has = live >> token & 1u;
-                    copy16(line, reinterpret_cast<const uint8_t*>(from), has);
-                    copy16(line + kKv4ValueOffset, reinterpret_cast<const uint8_t*>(from) + kKv4ValueOffset, has);
-                }
-                uint8_t* pairs = to + kKv4PairOffset;
-                if constexpr (NG == 4) {
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int token = 16 * i + (lane >> 1);
-                        const uint64_t from = __shfl_sync(0xFFFFFFFFu, pair_row, token) + 16 * (lane & 1);
-                        copy16(pairs + i * kTile + (lane >> 1) * 32 + 16 * (lane & 1),
-                               reinterpret_cast<const uint8_t*>(from), live >> token & 1u);
-                    }
-                } else {
-                    uint8_t* line = pairs + (lane >> 4) * kTile + (lane & 15) * 8 * NG;
-                    if constexpr (NG == 2)
-                        copy16(line, reinterpret_cast<const uint8_t*>(pair_row), there);
-                    else
-                        copy8(line, reinterpret_cast<const uint8_t*>(pair_row), there);
-                }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                index0 = index1;
-                page0 = page_of(index0);
-                index1 = index_of(j + 2);
-                return live;
-            };
-            uint32_t live[kStages];
-#pragma unroll
-            for (int j = 0; j < kStages - 1; ++j) live[j] = issue(j);  // past the end: nothing is there
-            live[kStages - 1] = 0;
-            for (int j = 0; j < todo; ++j) {
-                const uint32_t issued = issue(j + kStages - 1);
-                asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-                __syncwarp();
-                mask.tokens = live[0];
-                mask.base = 0;
-#pragma unroll
-                for (int i = 0; i + 2 < kStages; ++i) live[i] = live[i + 1];
-                live[kStages - 2] = issued;
-                chunk_pass<NG, NT, true>(state, ring + (j % kStages) * kStageBytes, mask);
-                __syncwarp();
-            }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
 
-        // The warps' states, row by row, through the ring's memory.
-        __syncthreads();
-        float* merged = reinterpret_cast<float*>(smem);
-        const int live_rows = min(rows - first_row, 8 * NT);
+        // The next segment's first copies fly while this one's states are merged.
+        const Segment done = segment;
+        const int64_t done_first = place.first;
+        const int done_chunks = place.chunks;
+        const bool is_first = at == place.begin;
+        at += done.chunk1 - done.chunk0;
+        const bool more = at < place.end;
+        if (more) {
+            const int64_t next = place.first + static_cast<int64_t>(place.chunks) * segments;
+            if (at >= next) {
+                place.first = next;
+                ++place.entry;
+                place.chunks = chunks_of<kSelected>(p, place.entry);
+            }
+            segment = segment_at<kSelected, kRows>(p, place, at, segments, group, rows);
+            begin(segment);
+        }
+
+        // The warps' states, row by row.
+        const int live_rows = min(rows - done.first_row, kRows);
 #pragma unroll
         for (int b = 0; b < NT; ++b) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int c = 0; c < NC; ++c) {
 #pragma unroll
                 for (int step = 4; step < 32; step *= 2) {
                     state.sum[b][c] += __shfl_xor_sync(0xFFFFFFFFu, state.sum[b][c], step);
@@ -734,114 +1014,116 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 2) attention_kernel(co
                     for (int k = 0; k < NG; ++k)
                         state.low_sum[b][k][c] += __shfl_xor_sync(0xFFFFFFFFu, state.low_sum[b][k][c], step);
                 }
-                const int row = 8 * b + 2 * t + c;
-                if (g == 0) {
-                    merge_top[warp][row] = state.top[b][c];
-                    merge_sum[warp][row] = state.sum[b][c];
-                }
-                float* line = merged + (warp * 8 * NT + row) * kMergeStride;
+                const int row = Columns<NT, NC>::row_of(b, t, c);
+                if (g == 0) merge_heads[warp][row] = make_float2(state.top[b][c], state.sum[b][c]);
+                if (row < live_rows) {
+                    float* line = merged + (warp * kRows + row) * kMergeStride;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float low = state.low_sum[b][i * NG / 8][c];
-                    *reinterpret_cast<float2*>(line + 16 * i + 2 * g) =
-                        make_float2(__fmaf_rn(state.out[b][i][c], 0x1p24f, low),
-                                    __fmaf_rn(state.out[b][i][2 + c], 0x1p20f, low));
+                    for (int i = 0; i < 8; ++i) {
+                        const float low = state.low_sum[b][i * NG / 8][c];
+                        *reinterpret_cast<float2*>(line + 16 * i + 2 * g) =
+                            make_float2(__fmaf_rn(state.out[b][i][out_column<NG, NC>(i, c)], 0x1p24f, low),
+                                        __fmaf_rn(state.out[b][i][2 + out_column<NG, NC>(i, c)], 0x1p20f, low));
+                    }
                 }
             }
         }
         __syncthreads();
-        const bool whole = chunk0 == 0 && chunk1 == place.chunks;
-        const int which = at == place.begin ? 0 : 1;  // a CTA has at most a first and a last part of a segment
-        float* part = p.partials + (blockIdx.x * 2 + which) * static_cast<int64_t>(8 * NT * (kDim + 2));
-        auto out_row = [&](int r) {
-            const int row = first_row + r;
-            return p.out + ((static_cast<int64_t>(entry) * p.q_len + (kSelected ? 0 : row / group)) * p.q_heads + head0 +
-                            (kSelected ? 0 : row % group)) * kDim;
+        // A CTA has at most a first and a last part of a segment.
+        float* part = p.partials + (blockIdx.x * 2 + (is_first ? 0 : 1)) * static_cast<int64_t>(kPartFloats);
+        auto write_row = [&](int r, const Join& row_of) {
+            const int row = done.first_row + r;
+            uint16_t* to = p.out + ((static_cast<int64_t>(done.entry) * p.q_len + (kSelected ? 0 : row / group)) * p.q_heads +
+                                    done.head0 + (kSelected ? 0 : row % group)) * kDim;
+            const bool none = row_of.sum == 0.0f || row > done.last_row;
+            const float by = none ? 0.0f : 1.0f / row_of.sum;
+            uint2 bits;
+            bits.x = rounded(none ? 0.0f : row_of.value.x * by, p.bf16) |
+                     static_cast<uint32_t>(rounded(none ? 0.0f : row_of.value.y * by, p.bf16)) << 16;
+            bits.y = rounded(none ? 0.0f : row_of.value.z * by, p.bf16) |
+                     static_cast<uint32_t>(rounded(none ? 0.0f : row_of.value.w * by, p.bf16)) << 16;
+            *(reinterpret_cast<uint2*>(to) + lane) = bits;
         };
-        for (int r = 0; r < live_rows; ++r) {
-            float top = merge_top[0][r], sum = 0.0f, value = 0.0f;
+        for (int r = warp; r < live_rows; r += kWarps) {
+            Join row;
 #pragma unroll
-            for (int w = 1; w < kWarps; ++w) top = fmaxf(top, merge_top[w][r]);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float keep = exp2_of(merge_top[w][r] - top);
-                sum = __fmaf_rn(merge_sum[w][r], keep, sum);
-                value = __fmaf_rn(merged[(w * 8 * NT + r) * kMergeStride + threadIdx.x], keep, value);
-            }
-            if (whole) {
-                const bool none = sum == 0.0f || first_row + r > last_row;
-                out_row(r)[threadIdx.x] = rounded(none ? 0.0f : value / sum, p.bf16);
+            for (int w = 0; w < kWarps; ++w)
+                row.add(merge_heads[w][r], *(reinterpret_cast<const float4*>(merged + (w * kRows + r) * kMergeStride) + lane));
+            if (done.whole) {
+                write_row(r, row);
             } else {
-                part[r * kDim + threadIdx.x] = value;
-                if (threadIdx.x == 0)
-                    *reinterpret_cast<float2*>(part + 8 * NT * kDim + 2 * r) = make_float2(top, sum);
+                *(reinterpret_cast<float4*>(part + r * kDim) + lane) = row.value;
+                if (lane == 0) *reinterpret_cast<float2*>(part + kRows * kDim + 2 * r) = make_float2(row.top, row.sum);
             }
         }
-        if (!whole) {
+        if (more) stage_queries<NG, NT>(p, staged, raw);
+        if (!done.whole) {
             // The CTA that completes the segment joins its parts, in their order.
-            const int64_t from = place.first + static_cast<int64_t>(segment) * place.chunks;
-            const int owner0 = owner_of(place, from), owner1 = owner_of(place, from + place.chunks - 1);
-            __threadfence();
-            __syncthreads();
+            const int64_t from = done_first + static_cast<int64_t>(done.number) * done_chunks;
+            int owner0, owner1;
+            bool second = false;  // whether the first owner's part is that CTA's last
+            if (place.parts) {
+                owner0 = blockIdx.x / place.parts * place.parts;
+                owner1 = owner0 + place.parts - 1;
+            } else {
+                owner0 = static_cast<int>(quotient(from, place.share));
+                owner1 = static_cast<int>(quotient(from + done_chunks - 1, place.share));
+                second = static_cast<int64_t>(owner0) * place.share < from;
+            }
+            __syncthreads();  // every thread's part is written: the atomic below releases them all
             if (threadIdx.x == 0) {
-                int32_t* counter = p.counters + static_cast<int64_t>(entry) * segments + segment;
-                is_last = atomicAdd(counter, 1) == owner1 - owner0;
+                int32_t* counter = p.counters + static_cast<int64_t>(done.entry) * segments + done.number;
+                int before;
+                asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+                is_last = before == owner1 - owner0;
                 if (is_last) *counter = 0;
             }
             __syncthreads();
             if (is_last) {
-                __threadfence();
-                const bool first_is_second = owner0 * place.all / place.ctas < from;  // the owner's last part
-                for (int r = warp; r < live_rows; r += kWarps) {
-                    float top = kNothing;
-                    auto part_of = [&](int owner) {
-                        const int slot = owner * 2 + (owner == owner0 && first_is_second ? 1 : 0);
-                        return p.partials + slot * static_cast<int64_t>(8 * NT * (kDim + 2));
-                    };
-                    for (int o = owner0 + lane; o <= owner1; o += 32)
-                        top = fmaxf(top, __ldcg(part_of(o) + 8 * NT * kDim + 2 * r));
+                // Few rows: several warps to a row, each with every few parts.
+                const int per_row = live_rows == 1 ? 8 : live_rows == 2 ? 4 : live_rows <= 4 ? 2 : 1;
+                const int sub = warp & (per_row - 1);
+                for (int r = warp / per_row; r < live_rows; r += kWarps / per_row) {
+                    Join row;
+                    constexpr int kBatch = 10;
+                    for (int o0 = owner0 + sub; o0 <= owner1; o0 += kBatch * per_row) {
+                        float2 heads_of[kBatch];
+                        float4 v[kBatch];
 #pragma unroll
-                    for (int step = 16; step > 0; step /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, step));
-                    float sum = 0.0f;
-                    float4 value = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-                    for (int o = owner0; o <= owner1; ++o) {
-                        const float* from_part = part_of(o);
-                        const float2 head_of = __ldcg(reinterpret_cast<const float2*>(from_part + 8 * NT * kDim + 2 * r));
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(from_part + r * kDim) + lane);
-                        const float keep = exp2_of(head_of.x - top);
-                        sum = __fmaf_rn(head_of.y, keep, sum);
-                        value.x = __fmaf_rn(v.x, keep, value.x);
-                        value.y = __fmaf_rn(v.y, keep, value.y);
-                        value.z = __fmaf_rn(v.z, keep, value.z);
-                        value.w = __fmaf_rn(v.w, keep, value.w);
+                        for (int i = 0; i < kBatch; ++i) {
+                            const int o = min(o0 + i * per_row, owner1);
+                            const float* from_part =
+                                p.partials + (o * 2 + (second && o == owner0 ? 1 : 0)) * static_cast<int64_t>(kPartFloats);
+                            heads_of[i] = __ldcg(reinterpret_cast<const float2*>(from_part + kRows * kDim + 2 * r));
+                            v[i] = __ldcg(reinterpret_cast<const float4*>(from_part + r * kDim) + lane);
+                        }
+#pragma unroll
+                        for (int i = 0; i < kBatch; ++i)
+                            if (o0 + i * per_row <= owner1) row.add(heads_of[i], v[i]);
                     }
-                    const bool none = sum == 0.0f || first_row + r > last_row;
-                    const float by = none ? 0.0f : 1.0f / sum;
-                    uint2 bits;
-                    bits.x = rounded(none ? 0.0f : value.x * by, p.bf16) |
-                             static_cast<uint32_t>(rounded(none ? 0.0f : value.y * by, p.bf16)) << 16;
-                    bits.y = rounded(none ? 0.0f : value.z * by, p.bf16) |
-                             static_cast<uint32_t>(rounded(none ? 0.0f : value.w * by, p.bf16)) << 16;
-                    *(reinterpret_cast<uint2*>(out_row(r)) + lane) = bits;
+                    if (per_row > 1) {
+                        float* line = merged + warp * kMergeStride;
+                        *(reinterpret_cast<float4*>(line) + lane) = row.value;
+                        if (lane == 0) *reinterpret_cast<float2*>(line + kDim) = make_float2(row.top, row.sum);
+                        asm volatile("bar.sync %0, %1;" ::"r"(1 + r), "r"(32 * per_row) : "memory");
+                        if (sub == 0)
+                            for (int w = 1; w < per_row; ++w)
+                                row.add(*reinterpret_cast<const float2*>(line + w * kMergeStride + kDim),
+                                        *(reinterpret_cast<const float4*>(line + w * kMergeStride) + lane));
+                    }
+                    if (sub == 0) write_row(r, row);
                 }
             }
         }
-        // The ring's next bulk copies come after these reads and writes of its memory.
-        fence_async_smem();
+        if (!more) break;
         __syncthreads();
-        at += chunk1 - chunk0;
-        const int64_t next = place.first + static_cast<int64_t>(place.chunks) * segments;
-        if (at >= next && at < place.end) {
-            place.first = next;
-            ++place.entry;
-            place.chunks = chunks_of<kSelected>(p, place.entry);
-        }
     }
     if (failed && lane == 0) atomicOr(p.view.status, kKv4StatusWait);
 }
 
-constexpr int kMostParts = 148 * 4 * 2;  // first and last parts of the largest grid
+constexpr int kMostCtas = 148;  // one to an SM
+constexpr int kMostRows = 24;
+constexpr int64_t kPartsBytes = int64_t{kMostCtas} * 2 * kMostRows * (kDim + 2) * 4;
 
 int check_queries(const char* what, const Kv4View& view, int64_t layer, int64_t n, int64_t q_heads, int64_t q_len,
                   int dtype, const void* queries, int64_t s0, int64_t s1, int64_t s2) {
@@ -858,33 +1140,34 @@ int check_queries(const char* what, const Kv4View& view, int64_t layer, int64_t 
     return POPKV_OK;
 }
 
-template <int NG, int NT, bool kSelected>
+template <int NG, int NT, int NC, bool kSelected>
 int launch(const char* what, const Params& p, int64_t most_chunks, cudaStream_t stream) {
-    constexpr int kSmem = smem_bytes<NG, NT>();
-    static_assert(kWarps * 8 * NT * kMergeStride * 4 <= kSmem, "the merge fits the ring");
-    auto kernel = attention_kernel<NG, NT, kSelected>;
+    using Size = Sizes<NG, NT, NC>;
+    constexpr int kSmem = Size::kRing + Size::kMerge;
+    static_assert(kSmem + sizeof(Queries<NT>) < 225 * 1024, "one CTA fits an SM");
+    auto kernel = attention_kernel<NG, NT, NC, kSelected>;
     if (int status = allow_dynamic_smem(kernel, kSmem)) return status;
-    constexpr int kPerSm = NT == 1 ? 4 : 2;
-    const int64_t ctas = (most_chunks + kWarps - 1) / kWarps;
-    const unsigned grid = static_cast<unsigned>(ctas < 148 * kPerSm ? ctas : 148 * kPerSm);
+    const unsigned grid = static_cast<unsigned>(most_chunks < kMostCtas ? most_chunks : kMostCtas);
     const cudaError_t err = launch_pdl(kernel, dim3(grid), dim3(kThreads), kSmem, stream, 1, p);
     if (err != cudaSuccess) return fail(POPKV_ERR_CUDA, "%s: %s", what, cudaGetErrorString(err));
     return check_launch(what);
 }
 
-template <int NT, bool kSelected>
+template <int NT, int NC, bool kSelected>
 int launch_groups(const char* what, const Params& p, int64_t most_chunks, cudaStream_t stream) {
-    if (p.view.groups == 4) return launch<4, NT, kSelected>(what, p, most_chunks, stream);
-    if (p.view.groups == 2) return launch<2, NT, kSelected>(what, p, most_chunks, stream);
-    return launch<1, NT, kSelected>(what, p, most_chunks, stream);
+    if (p.view.groups == 4) return launch<4, NT, NC, kSelected>(what, p, most_chunks, stream);
+    if (p.view.groups == 2) return launch<2, NT, NC, kSelected>(what, p, most_chunks, stream);
+    return launch<1, NT, NC, kSelected>(what, p, most_chunks, stream);
 }
 
 constexpr float kLog2E = 1.4426950408889634f;
 
-// Row tiles of a KV head: 8 rows when that is all, else 16 (one pass of the cache per tile).
-int64_t row_tiles(int64_t rows) { return rows <= 8 ? 1 : (rows + 15) / 16; }
-
-constexpr int64_t kPartFloats = 16 * (kDim + 2);
+// Row tiles of a KV head (each is a pass over its tokens), and the columns of 8 rows of one.
+int64_t row_tiles(int64_t rows) { return (rows + kMostRows - 1) / kMostRows; }
+int64_t column_blocks(int64_t rows) {
+    const int64_t tiles = row_tiles(rows);
+    return (rows + 8 * tiles - 1) / (8 * tiles);
+}
 
 }  // namespace
 }  // namespace popkv
@@ -893,21 +1176,20 @@ extern "C" int64_t popkv_kv4_attention_workspace(int64_t n, int64_t kv_heads, in
     using namespace popkv;
     if (n < 0 || kv_heads < 1 || q_heads < kv_heads || q_len < 0 || q_heads % kv_heads) return -1;
     const int64_t selected = n * q_heads, all = n * kv_heads * row_tiles(q_len * (q_heads / kv_heads));
-    const int64_t counters = (selected > all ? selected : all) * 4;
-    return (counters + 255) / 256 * 256 + kMostParts * kPartFloats * 4;
+    // Parts first: their place does not depend on the sizes, so one workspace serves calls of any.
+    return kPartsBytes + (selected > all ? selected : all) * 4;
 }
 
 namespace popkv {
 namespace {
 
-int bind_workspace(const char* what, Params& p, int64_t n, int64_t kv_heads, void* workspace, int64_t bytes) {
-    const int64_t need = popkv_kv4_attention_workspace(n, kv_heads, p.q_heads, p.q_len);
+int bind_workspace(const char* what, Params& p, int64_t n, void* workspace, int64_t bytes) {
+    const int64_t need = popkv_kv4_attention_workspace(n, p.view.kv_heads, p.q_heads, p.q_len);
     if (!workspace || !aligned(workspace, 16) || bytes < need)
         return fail(POPKV_ERR_INVALID, "%s: the workspace must be 16-byte aligned and hold %lld bytes", what,
                     static_cast<long long>(need));
-    // Parts first: their place does not depend on the sizes, so one workspace serves calls of any.
     p.partials = static_cast<float*>(workspace);
-    p.counters = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + kMostParts * kPartFloats * 4);
+    p.counters = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(workspace) + kPartsBytes);
     return POPKV_OK;
 }
 
@@ -941,13 +1223,16 @@ extern "C" int popkv_kv4_attention(const popkv_kv4_cache* cache, int64_t layer, 
     p.q_head = q_head_stride;
     p.scale = scale * kLog2E;
     p.out = static_cast<uint16_t*>(out);
-    const int64_t rows = q_len * (q_heads / p.view.kv_heads);
-    p.tiles = static_cast<int>(row_tiles(rows));
-    if (int status = bind_workspace(what, p, n, p.view.kv_heads, workspace, workspace_bytes)) return status;
+    const int64_t rows = q_len * (q_heads / p.view.kv_heads), blocks = column_blocks(rows);
+    p.tiles = static_cast<int>((rows + 8 * blocks - 1) / (8 * blocks));
+    if (int status = bind_workspace(what, p, n, workspace, workspace_bytes)) return status;
     const int64_t chunks = (static_cast<int64_t>(p.view.max_pages) * p.view.page_size() + kChunk - 1) / kChunk;
     const int64_t most = n * p.view.kv_heads * p.tiles * chunks;
     const auto s = static_cast<cudaStream_t>(stream);
-    return rows <= 8 ? launch_groups<1, false>(what, p, most, s) : launch_groups<2, false>(what, p, most, s);
+    if (rows <= 4) return launch_groups<1, 1, false>(what, p, most, s);
+    return blocks == 1   ? launch_groups<1, 2, false>(what, p, most, s)
+           : blocks == 2 ? launch_groups<2, 2, false>(what, p, most, s)
+                         : launch_groups<3, 2, false>(what, p, most, s);
 }
 
 extern "C" int popkv_kv4_attention_selected(const popkv_kv4_cache* cache, int64_t layer, const int32_t* seqs,
@@ -979,7 +1264,7 @@ extern "C" int popkv_kv4_attention_selected(const popkv_kv4_cache* cache, int64_
     p.valid = valid;
     p.out = static_cast<uint16_t*>(out);
     p.tiles = 1;
-    if (int status = bind_workspace(what, p, n, p.view.kv_heads, workspace, workspace_bytes)) return status;
-    const int64_t most = n * q_heads * ((selected + kChunk - 1) / kChunk > 0 ? (selected + kChunk - 1) / kChunk : 1);
-    return launch_groups<1, true>(what, p, most, static_cast<cudaStream_t>(stream));
+    if (int status = bind_workspace(what, p, n, workspace, workspace_bytes)) return status;
+    const int64_t chunks = (selected + kChunk - 1) / kChunk;
+    return launch_groups<1, 1, true>(what, p, n * q_heads * (chunks > 0 ? chunks : 1), static_cast<cudaStream_t>(stream));
 }

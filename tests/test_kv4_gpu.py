@@ -210,8 +210,9 @@ def test_attention_counts_padding_and_strides(cuda_device):
     close(one, want, most)
 
 
-def test_attention_ignores_what_lies_past_the_end(cuda_device):
-    """Stale bytes behind a sequence's end (NaN pairs among them) and page ids out of range."""
+@pytest.mark.parametrize("stale", (0x7FFF, 0x7C00, -0x400, 0x7BFF))  # NaN, inf, -inf, the largest value
+def test_attention_ignores_what_lies_past_the_end(cuda_device, stale):
+    """Stale bytes behind a sequence's end and page ids out of range."""
     cache = make(cuda_device, [21, 50], kv_heads=2, page=16)
     host = R.HostCache.like(cache)
     before = cache.attention(random_queries((2, 2, 4, 128), torch.float16, cuda_device, 8), seqs=[0, 1])
@@ -221,9 +222,14 @@ def test_attention_ignores_what_lies_past_the_end(cuda_device):
         for r in range(length % 16, 16):
             tile[:, r * 64:(r + 1) * 64] = 255
             tile[:, 1024 + r * 64:1024 + (r + 1) * 64] = 255
-            tile[:, 2048 + r * 32:2048 + (r + 1) * 32] = 255  # fp16 NaN
+            tile.view(torch.int16)[:, 1024 + r * 16:1024 + (r + 1) * 16] = stale
     queries = random_queries((2, 2, 4, 128), torch.float16, cuda_device, 8)
     assert torch.equal(before, cache.attention(queries, seqs=[0, 1]))
+    picked = torch.tensor([3, 20, 21, 22, 49, 50, 63], device=cuda_device).expand(2, 4, 7)
+    got = cache.attention_selected(queries[:, 0], picked, seqs=[0, 1])
+    want, most = expect(cache, host, queries[:, 0], lambda at: (at[0], [t for t in (3, 20, 21, 22, 49)
+                                                                        if t < (21, 50)[at[0]]]))
+    close(got, want, most)
     # Tokens of a missing page do not exist.
     cache.table[1, 1] = -1
     got = cache.attention(queries, seqs=[0, 1])
