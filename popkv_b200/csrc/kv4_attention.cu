@@ -24,13 +24,6 @@
 namespace popkv {
 namespace {
 
-#ifndef KV4_H
-#define KV4_H 2
-#define KV4_W 8
-#define KV4_S 4
-#endif
-constexpr int kWarps = KV4_W;
-constexpr int kThreads = 32 * kWarps;
 constexpr int kChunk = 32;    // tokens of one stage of a warp: two tiles
 constexpr int kDim = kKv4Dim;
 constexpr int kMergeStride = kDim + 4;  // floats of a row in the warps' merge: conflict-free float2 stores
@@ -90,6 +83,13 @@ __device__ __forceinline__ float high_of(uint32_t pair) {
     return __high2float(h);
 }
 
+// a - b of two fp16 pairs.
+__device__ __forceinline__ uint32_t minus2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t y;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -115,6 +115,7 @@ __device__ __forceinline__ void mma_new(float* c, uint32_t a0, uint32_t a1, uint
 
 constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;  // n and 16 n of two numbers, as fp16 denormals
 constexpr uint32_t kMinusEven = 0x80088008u, kMinusOdd = 0x80808080u;  // -8 and -16 * 8 likewise
+constexpr uint32_t kEightEven = 0x00080008u, kEightOdd = 0x00800080u;  // 8 and 16 * 8
 
 // Columns of the products: NT blocks of 8, of which a lane (g = lane / 4, t = lane % 4) holds
 // columns 2t and 2t + 1 of the results and column g of the operands.  With NC = 2 each column
@@ -155,7 +156,7 @@ struct Segment {
 };
 
 // Query rows of the tile as they are: 16 threads a column, each with 8 dims.
-template <int NT, int NC>
+template <int NT, int NC, int kThreads>
 __device__ __forceinline__ void load_queries(const Params& p, const Segment& segment, int group, int rows,
                                              uint4* raw) {
 #pragma unroll
@@ -169,7 +170,7 @@ __device__ __forceinline__ void load_queries(const Params& p, const Segment& seg
     }
 }
 
-template <int NG, int NT>
+template <int NG, int NT, int kThreads>
 __device__ __forceinline__ void stage_queries(const Params& p, Queries<NT>& s, const uint4* rows_read) {
 #pragma unroll
     for (int k = 0; k < (NT * 128 + kThreads - 1) / kThreads; ++k) {
@@ -498,9 +499,11 @@ __device__ __forceinline__ void tiles_pass(State<NG, NT, NC>& s, uint32_t data, 
                                                                             : 0.0f));
         }
         // Value numbers of tokens j, j + 1 (and + 8) side by side, 16 dims at a time.  They enter
-        // as n - 8, the 8 in a product of its own: the sums stay near zero, so that neither the
-        // weights' rounding nor the tensor cores' truncated additions are multiplied by the
-        // numbers' offset (over 131072 tokens: error 3.5 times smaller).
+        // as n - 8: the sums stay near zero, so that neither the weights' rounding nor the tensor
+        // cores' truncated additions are multiplied by the numbers' offset (over 131072 tokens:
+        // error 3.5 times smaller).  With one block of rows the 8 is a product of its own (8 more
+        // products a tile), with several it is taken off the operand that they share (32 more
+        // subtractions).
         const uint32_t values = tile + at.values, others = values ^ kKv4RowBytes;  // token_at(2t + 1) = token_at(2t) ^ 1
         const uint2 v0 = shared_load<uint2>(values), v1 = shared_load<uint2>(others);
         const uint2 v2 = shared_load<uint2>(values + 8 * kKv4RowBytes), v3 = shared_load<uint2>(others + 8 * kKv4RowBytes);
@@ -510,25 +513,34 @@ __device__ __forceinline__ void tiles_pass(State<NG, NT, NC>& s, uint32_t data, 
             const uint32_t a = __byte_perm(i < 2 ? v0.x : v0.y, i < 2 ? v1.x : v1.y, pick);
             const uint32_t c = __byte_perm(i < 2 ? v2.x : v2.y, i < 2 ? v3.x : v3.y, pick);
             const uint32_t a8 = upper_numbers(a), c8 = upper_numbers(c);
+            uint32_t n[2][4] = {{a & kEven, a & kOdd, c & kEven, c & kOdd},
+                                {a8 & kEven, a8 & kOdd, c8 & kEven, c8 & kOdd}};
             const int k = i * NG / 4 / kPer;
+            if constexpr (NT > 1) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) n[u][v] = minus2(n[u][v], v & 1 ? kEightOdd : kEightEven);
+            }
 #pragma unroll
             for (int b = 0; b < NT; ++b) {
                 const uint32_t w0 = weights[b][k][0], w1 = weights[b][k][1];
-                mma(s.out[b][2 * i], at.minus[0], at.minus[1], at.minus[2], at.minus[3], w0, w1);
-                mma(s.out[b][2 * i + 1], at.minus[0], at.minus[1], at.minus[2], at.minus[3], w0, w1);
-                mma(s.out[b][2 * i], a & kEven, a & kOdd, c & kEven, c & kOdd, w0, w1);
-                mma(s.out[b][2 * i + 1], a8 & kEven, a8 & kOdd, c8 & kEven, c8 & kOdd, w0, w1);
+                if constexpr (NT == 1) {
+                    mma(s.out[b][2 * i], at.minus[0], at.minus[1], at.minus[2], at.minus[3], w0, w1);
+                    mma(s.out[b][2 * i + 1], at.minus[0], at.minus[1], at.minus[2], at.minus[3], w0, w1);
+                }
+                mma(s.out[b][2 * i], n[0][0], n[0][1], n[0][2], n[0][3], w0, w1);
+                mma(s.out[b][2 * i + 1], n[1][0], n[1][1], n[1][2], n[1][3], w0, w1);
             }
         }
     }
 }
 
 // One chunk of two tiles, together where that leaves the registers for it.
-template <int NG, int NT, int NC, bool kMasked>
+template <int NG, int NT, int NC, int kTogether, bool kMasked>
 __device__ __forceinline__ void chunk_pass(State<NG, NT, NC>& s, uint32_t data, const Lane& at,
                                            const Mask<NT, NC>& mask) {
     constexpr int kTile = kKv4PairOffset + kKv4TileTokens * 8 * NG;
-    constexpr int kTogether = NT == 1 ? KV4_H : 1;
 #pragma unroll 1
     for (int h = 0; h < 2; h += kTogether)
         tiles_pass<NG, NT, NC, kTogether, kMasked>(s, data + h * kTile, at, h, mask);
@@ -538,10 +550,14 @@ __device__ __forceinline__ uint16_t rounded(float v, int bf16) {
     return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
 
-// The work of one CTA: chunks [begin, end) of the flat list of all (entry, head, row tile)
-// segments' chunks, of which `first` lie before the current entry.  With `parts` every
-// segment is cut into that many, one to a CTA; with 0 the list is cut into even shares, and
-// a CTA may end one segment and begin the next.
+// A segment costs a CTA about as much as this many chunks besides its own (queries, page
+// lookups, first copies, merge: 5 us against 0.3 us a chunk).
+constexpr int kSegmentCost = 16;
+
+// The work of one CTA: [begin, end) of the flat list of all (entry, head, row tile) segments,
+// each of which is kSegmentCost units and then its chunks; `first` units lie before the current
+// entry.  With `parts` every segment is cut into that many, one to a CTA; with 0 the list is
+// cut into even shares, and a CTA may end one segment and begin the next.
 struct Place {
     int64_t begin, end, first;
     int share, parts, entry, chunks;
@@ -562,11 +578,12 @@ __device__ __forceinline__ int chunks_of(const Params& p, int entry) {
 // The CTA's place.  The lengths are in device memory, so every CTA finds its own.
 //
 // Segments of one length (a single sequence, or selected slots) are cut into equal parts, one to a
-// CTA, where that costs no more than a quarter over even shares: each further segment that a CTA
-// enters costs it about 5 us of latency (queries, page lookups, first copies, merge).  At 32 x 8
-// heads x 32768 tokens on 296 CTAs: 37 parts a head against shares that straddle heads.
-template <bool kSelected>
+// CTA, where those are not much longer than even shares, which straddle segments and make a CTA
+// merge two of them: 32 query and 8 KV heads x 32768 tokens take 17.9 us in 18 parts a head and
+// 20.7 us in even shares.
+template <bool kSelected, int kWarps>
 __device__ Place find_place(const Params& p, int segments) {
+    constexpr int kThreads = 32 * kWarps;
     __shared__ int64_t sums[kWarps];
     __shared__ int extremes[2][kWarps];
     __shared__ int64_t found_first;
@@ -611,36 +628,41 @@ __device__ Place find_place(const Params& p, int segments) {
     }
     const int ctas = gridDim.x, number = p.n * segments;
     const int floor_share = min(kWarps, static_cast<int>(quotient(all, number)));  // a chunk to each warp
-    place.share = max(floor_share, static_cast<int>(quotient(all + ctas - 1, ctas)));
+    const int64_t units = all + static_cast<int64_t>(number) * kSegmentCost;
+    place.share = max(floor_share + kSegmentCost, static_cast<int>(quotient(units + ctas - 1, ctas)));
     place.parts = 0;
     if (least == most && number <= ctas) {
         const int parts = ctas / number;
         const int share = max(floor_share, (most + parts - 1) / parts);
-        if (share - place.share <= place.share / 4) {
-            place.share = share;
+        const int even = static_cast<int>(quotient(all + ctas - 1, ctas));
+        if (share <= even + even / 4 + kSegmentCost / 2) {
+            place.share = share + kSegmentCost;
             place.parts = (most + share - 1) / share;
             const int segment = blockIdx.x / place.parts, part = blockIdx.x - segment * place.parts;
             place.chunks = most;
             place.entry = segment / segments;
-            place.first = static_cast<int64_t>(place.entry) * segments * most;
-            place.begin = static_cast<int64_t>(segment) * most + part * share;
-            place.end = segment < number ? min(place.begin + share, static_cast<int64_t>(segment + 1) * most) : 0;
+            place.first = static_cast<int64_t>(place.entry) * segments * (most + kSegmentCost);
+            const int64_t from = static_cast<int64_t>(segment) * (most + kSegmentCost) + kSegmentCost;
+            place.begin = from + part * share;
+            place.end = segment < number ? min(place.begin + share, from + most) : 0;
             return place;
         }
     }
     place.begin = static_cast<int64_t>(blockIdx.x) * place.share;
-    place.end = min(place.begin + place.share, all);
-    if (place.begin >= all) return place;
+    place.end = min(place.begin + place.share, units);
+    if (place.begin >= units) return place;
     if (kSelected) {
         place.chunks = most;
-        place.entry = static_cast<int>(quotient(place.begin, place.chunks) / segments);
-        place.first = static_cast<int64_t>(place.entry) * place.chunks * segments;
+        const int cost = most + kSegmentCost;
+        place.entry = static_cast<int>(quotient(place.begin, cost) / segments);
+        place.first = static_cast<int64_t>(place.entry) * cost * segments;
         return place;
     }
     int64_t before = 0;
     for (int base = 0; base < p.n; base += kThreads) {
         const int i = base + threadIdx.x;
-        const int chunks = base == 0 ? mine : i < p.n ? chunks_of<kSelected>(p, i) : 0;
+        int chunks = base == 0 ? mine : i < p.n ? chunks_of<kSelected>(p, i) : 0;
+        if (chunks) chunks += kSegmentCost;
         int64_t upto = chunks;
 #pragma unroll
         for (int step = 1; step < 32; step *= 2) {
@@ -655,7 +677,7 @@ __device__ Place find_place(const Params& p, int segments) {
         if (chunks && place.begin >= from && place.begin < upto * segments) {
             found_first = from;
             found_entry = i;
-            found_chunks = chunks;
+            found_chunks = chunks - kSegmentCost;
         }
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) before += sums[w];
@@ -678,11 +700,13 @@ __device__ __forceinline__ void copy8(uint8_t* to, const uint8_t* from, bool the
                  : "memory");
 }
 
-template <int NG, int NT, int NC>
+template <int NG, int NT, int NC, bool kSelected>
 struct Sizes {
+    static constexpr int kWarps = kSelected || NC == 1 ? 12 : 8;
+    static constexpr int kTogether = NT == 1 && !kSelected ? 2 : 1;  // tiles of one pass
     static constexpr int kTile = kKv4PairOffset + kKv4TileTokens * 8 * NG;
     static constexpr int kStageBytes = 2 * kTile;
-    static constexpr int kStages = NT == 1 ? KV4_S : NT == 2 ? 3 : 2;  // chunks of a warp in flight: what fits
+    static constexpr int kStages = 2;  // chunks of a warp in flight
     static constexpr int kRing = kWarps * kStages * kStageBytes;
     static constexpr int kMerge = kWarps * Columns<NT, NC>::kRows * kMergeStride * 4;
 };
@@ -692,9 +716,11 @@ __device__ __forceinline__ Segment segment_at(const Params& p, const Place& plac
                                               int rows) {
     Segment s;
     const int64_t offset = at - place.first;
-    s.number = static_cast<int>(quotient(offset, place.chunks));
-    s.chunk0 = static_cast<int>(offset - static_cast<int64_t>(s.number) * place.chunks);
-    s.chunk1 = static_cast<int>(min(static_cast<int64_t>(place.chunks), s.chunk0 + (place.end - at)));
+    const int cost = place.chunks + kSegmentCost;
+    s.number = static_cast<int>(quotient(offset, cost));
+    const int64_t from = place.first + static_cast<int64_t>(s.number) * cost + kSegmentCost;
+    s.chunk0 = static_cast<int>(max(at, from) - from);
+    s.chunk1 = static_cast<int>(min(static_cast<int64_t>(place.chunks), place.end - from));  // none: <= chunk0
     s.whole = s.chunk0 == 0 && s.chunk1 == place.chunks;
     s.entry = place.entry;
     const int head = s.number / p.tiles;
@@ -716,6 +742,7 @@ struct Share {
     int first, todo;
 };
 
+template <int kWarps>
 __device__ __forceinline__ Share share_of(const Segment& s, bool none) {
     const int warp = threadIdx.x >> 5, stop = min(s.chunk1, (s.seen + kChunk - 1) / kChunk);
     Share share;
@@ -726,7 +753,7 @@ __device__ __forceinline__ Share share_of(const Segment& s, bool none) {
 
 // Copies a warp's chunks of consecutive tokens: one bulk copy each (two where pages hold one
 // tile), issued by one lane, from addresses that the lanes look up 32 chunks at a time.
-template <int kTile>
+template <int kTile, int kWarps>
 struct TokenCopies {
     uint64_t now0, now1, next0, next1;  // of this lane's chunk of the 32, by tile; 0 where there is no page
     uint32_t gone0, gone1;              // chunks without a page, of the 32 in use
@@ -782,11 +809,13 @@ struct TokenCopies {
 
 // Copies a warp's chunks of selected slots: lane l resolves slot l (indices are read two chunks
 // ahead of their copies, pages one), the copies of a row go over neighbouring lanes.
-template <int NG, int kTile>
+template <int NG, int kTile, int kWarps>
 struct SlotCopies {
     int64_t index0, index1;
     int64_t row_at;
-    int page0, seq, length, kv_head;
+    const uint8_t* layer;
+    uint32_t page_units, head_units;  // 16-byte units
+    int page0, seq, length, page_mask;
     Share share;
 
     __device__ __forceinline__ int64_t index_of(const Params& p, int j) const {
@@ -803,7 +832,10 @@ struct SlotCopies {
         share = chunks;
         seq = s.seq;
         length = s.length;
-        kv_head = s.kv_head;
+        layer = p.view.pages + p.layer * p.view.layer_bytes;
+        page_units = static_cast<uint32_t>(p.view.page_bytes / 16);
+        head_units = static_cast<uint32_t>(s.kv_head * p.view.head_bytes / 16);
+        page_mask = p.view.page_size() - 1;
         row_at = (static_cast<int64_t>(s.entry) * p.q_heads + s.head0) * p.selected;
         index0 = index_of(p, 0);
         index1 = index_of(p, 1);
@@ -813,35 +845,39 @@ struct SlotCopies {
     __device__ __forceinline__ uint32_t issue(const Params& p, int j, uint8_t* to) {
         const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
         const bool there = page0 >= 0;
-        const int position = static_cast<int>(index0), at = there ? position & 15 : 0;
-        const uint64_t tile = reinterpret_cast<uint64_t>(there ? p.view.tile_at(p.layer, page0, kv_head, position)
-                                                               : p.view.pages);
-        const uint64_t key_row = tile + at * kKv4RowBytes, pair_row = tile + kKv4PairOffset + at * 8 * NG;
+        const int position = static_cast<int>(index0), at = position & 15;
+        // Rows by their distance from the layer's first page, in 16 bytes.
+        const uint32_t tile = there ? static_cast<uint32_t>(page0) * page_units + head_units +
+                                          ((position & page_mask) >> 4) * (kTile / 16)
+                                    : 0u;
+        const uint32_t key_row = there ? tile + at * (kKv4RowBytes / 16) : 0u;
         const uint32_t live = __ballot_sync(0xFFFFFFFFu, there);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {  // 8 tokens, 4 lanes each
             const int token = 8 * i + g;
-            const uint64_t from = __shfl_sync(0xFFFFFFFFu, key_row, token) + 16 * t;
+            const uint8_t* from = layer + static_cast<uint64_t>(__shfl_sync(0xFFFFFFFFu, key_row, token) + t) * 16;
             uint8_t* line = to + (token >> 4) * kTile + (token & 15) * kKv4RowBytes + 16 * t;
             const bool has = live >> token & 1u;
-            copy16(line, reinterpret_cast<const uint8_t*>(from), has);
-            copy16(line + kKv4ValueOffset, reinterpret_cast<const uint8_t*>(from) + kKv4ValueOffset, has);
+            copy16(line, from, has);
+            copy16(line + kKv4ValueOffset, from + kKv4ValueOffset, has);
         }
         uint8_t* pairs = to + kKv4PairOffset;
         if constexpr (NG == 4) {
+            const uint32_t pair_row = there ? tile + kKv4PairOffset / 16 + at * 2 : 0u;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int token = 16 * i + (lane >> 1);
-                const uint64_t from = __shfl_sync(0xFFFFFFFFu, pair_row, token) + 16 * (lane & 1);
-                copy16(pairs + i * kTile + (lane >> 1) * 32 + 16 * (lane & 1), reinterpret_cast<const uint8_t*>(from),
+                const uint32_t from = __shfl_sync(0xFFFFFFFFu, pair_row, token) + (lane & 1);
+                copy16(pairs + i * kTile + (lane >> 1) * 32 + 16 * (lane & 1), layer + static_cast<uint64_t>(from) * 16,
                        live >> token & 1u);
             }
         } else {
             uint8_t* line = pairs + (lane >> 4) * kTile + (lane & 15) * 8 * NG;
+            const uint8_t* from = layer + static_cast<uint64_t>(tile) * 16 + (there ? kKv4PairOffset + at * 8 * NG : 0);
             if constexpr (NG == 2)
-                copy16(line, reinterpret_cast<const uint8_t*>(pair_row), there);
+                copy16(line, from, there);
             else
-                copy8(line, reinterpret_cast<const uint8_t*>(pair_row), there);
+                copy8(line, from, there);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         index0 = index1;
@@ -869,8 +905,10 @@ struct Join {
 };
 
 template <int NG, int NT, int NC, bool kSelected>
-__global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ Params p) {
-    using Size = Sizes<NG, NT, NC>;
+__global__ void __launch_bounds__(32 * Sizes<NG, NT, NC, kSelected>::kWarps, 1)
+    attention_kernel(const __grid_constant__ Params p) {
+    using Size = Sizes<NG, NT, NC, kSelected>;
+    constexpr int kWarps = Size::kWarps, kThreads = 32 * kWarps, kTogether = Size::kTogether;
     constexpr int kTile = Size::kTile, kStageBytes = Size::kStageBytes, kStages = Size::kStages;
     constexpr int kRows = Columns<NT, NC>::kRows;
     constexpr int kPartFloats = kRows * (kDim + 2);
@@ -893,19 +931,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     const int group = p.q_heads / p.view.kv_heads;
     const int rows = kSelected ? 1 : p.q_len * group;
     const int segments = heads * p.tiles;
-    Place place = find_place<kSelected>(p, segments);
+    Place place = find_place<kSelected, kWarps>(p, segments);
     if (place.begin >= place.end) return;
     int next_slot = 0;  // the stage to wait for, and its phase
     uint32_t phase = 0;
     bool failed = false;
     uint32_t live[kStages];
-    using Copies = std::conditional_t<kSelected, SlotCopies<NG, kTile>, TokenCopies<kTile>>;
+    using Copies = std::conditional_t<kSelected, SlotCopies<NG, kTile, kWarps>, TokenCopies<kTile, kWarps>>;
     Copies copies;
     uint4 raw[(NT * 128 + kThreads - 1) / kThreads];
+    Segment segment;
 
     // The first copies of a segment's part, and its queries.
     auto begin = [&](const Segment& s) {
-        copies.start(p, s, share_of(s, failed));
+        copies.start(p, s, share_of<kWarps>(s, failed));
         if constexpr (kSelected) {
 #pragma unroll
             for (int j = 0; j < kStages - 1; ++j) live[j] = copies.issue(p, j, ring + j * kStageBytes);
@@ -916,13 +955,26 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 slot = slot + 1 == kStages ? 0 : slot + 1;
             }
         }
-        load_queries<NT, NC>(p, s, group, rows, raw);
+        load_queries<NT, NC, kThreads>(p, s, group, rows, raw);
     };
 
-    int64_t at = place.begin;
-    Segment segment = segment_at<kSelected, kRows>(p, place, at, segments, group, rows);
+    // Moves to the segment at `place.begin`; false when nothing of it is left for this CTA.
+    auto enter = [&]() {
+        if (place.begin >= place.end) return false;
+        const int64_t next = place.first + static_cast<int64_t>(place.chunks + kSegmentCost) * segments;
+        if (place.begin >= next) {
+            place.first = next;
+            ++place.entry;
+            place.chunks = chunks_of<kSelected>(p, place.entry);
+        }
+        segment = segment_at<kSelected, kRows>(p, place, place.begin, segments, group, rows);
+        place.begin = place.first + static_cast<int64_t>(segment.number + 1) * (place.chunks + kSegmentCost);
+        return segment.chunk0 < segment.chunk1;
+    };
+    if (!enter()) return;
     begin(segment);
-    stage_queries<NG, NT>(p, staged, raw);
+    bool is_first = true;
+    stage_queries<NG, NT, kThreads>(p, staged, raw);
     __syncthreads();
     while (true) {
         State<NG, NT, NC> state;
@@ -946,7 +998,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 #pragma unroll
                 for (int i = 0; i + 2 < kStages; ++i) live[i] = live[i + 1];
                 live[kStages - 2] = issued;
-                chunk_pass<NG, NT, NC, true>(state, ring_at + (j % kStages) * kStageBytes, lanes, mask);
+                chunk_pass<NG, NT, NC, kTogether, true>(state, ring_at + (j % kStages) * kStageBytes, lanes, mask);
                 __syncwarp();
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -964,14 +1016,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 const bool has0 = !(copies.gone0 >> (j & 31) & 1u), has1 = !(copies.gone1 >> (j & 31) & 1u);
                 const uint32_t data = ring_at + next_slot * kStageBytes;
                 if (position + kChunk <= segment.seen_by_all && has0 && has1) {
-                    chunk_pass<NG, NT, NC, false>(state, data, lanes, mask);
+                    chunk_pass<NG, NT, NC, kTogether, false>(state, data, lanes, mask);
                 } else {
                     const int left = segment.length - position;  // > 0
                     mask.tokens = left >= 32 ? 0xFFFFFFFFu : (1u << left) - 1u;
                     if (!has0) mask.tokens &= 0xFFFF0000u;
                     if (!has1) mask.tokens &= 0x0000FFFFu;
                     mask.base = position;
-                    chunk_pass<NG, NT, NC, true>(state, data, lanes, mask);
+                    chunk_pass<NG, NT, NC, kTogether, true>(state, data, lanes, mask);
                 }
                 __syncwarp();
                 if (j + kStages < copies.share.todo)
@@ -987,19 +1039,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         const Segment done = segment;
         const int64_t done_first = place.first;
         const int done_chunks = place.chunks;
-        const bool is_first = at == place.begin;
-        at += done.chunk1 - done.chunk0;
-        const bool more = at < place.end;
-        if (more) {
-            const int64_t next = place.first + static_cast<int64_t>(place.chunks) * segments;
-            if (at >= next) {
-                place.first = next;
-                ++place.entry;
-                place.chunks = chunks_of<kSelected>(p, place.entry);
-            }
-            segment = segment_at<kSelected, kRows>(p, place, at, segments, group, rows);
-            begin(segment);
-        }
+        const bool more = enter();
+        if (more) begin(segment);
 
         // The warps' states, row by row.
         const int live_rows = min(rows - done.first_row, kRows);
@@ -1031,6 +1072,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         __syncthreads();
         // A CTA has at most a first and a last part of a segment.
         float* part = p.partials + (blockIdx.x * 2 + (is_first ? 0 : 1)) * static_cast<int64_t>(kPartFloats);
+        is_first = false;
         auto write_row = [&](int r, const Join& row_of) {
             const int row = done.first_row + r;
             uint16_t* to = p.out + ((static_cast<int64_t>(done.entry) * p.q_len + (kSelected ? 0 : row / group)) * p.q_heads +
@@ -1056,18 +1098,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 if (lane == 0) *reinterpret_cast<float2*>(part + kRows * kDim + 2 * r) = make_float2(row.top, row.sum);
             }
         }
-        if (more) stage_queries<NG, NT>(p, staged, raw);
+        if (more) stage_queries<NG, NT, kThreads>(p, staged, raw);
         if (!done.whole) {
             // The CTA that completes the segment joins its parts, in their order.
-            const int64_t from = done_first + static_cast<int64_t>(done.number) * done_chunks;
+            const int64_t from = done_first + static_cast<int64_t>(done.number) * (done_chunks + kSegmentCost);
             int owner0, owner1;
             bool second = false;  // whether the first owner's part is that CTA's last
             if (place.parts) {
                 owner0 = blockIdx.x / place.parts * place.parts;
                 owner1 = owner0 + place.parts - 1;
             } else {
-                owner0 = static_cast<int>(quotient(from, place.share));
-                owner1 = static_cast<int>(quotient(from + done_chunks - 1, place.share));
+                owner0 = static_cast<int>(quotient(from + kSegmentCost, place.share));
+                owner1 = static_cast<int>(quotient(from + kSegmentCost + done_chunks - 1, place.share));
                 second = static_cast<int64_t>(owner0) * place.share < from;
             }
             __syncthreads();  // every thread's part is written: the atomic below releases them all
@@ -1142,13 +1184,13 @@ int check_queries(const char* what, const Kv4View& view, int64_t layer, int64_t 
 
 template <int NG, int NT, int NC, bool kSelected>
 int launch(const char* what, const Params& p, int64_t most_chunks, cudaStream_t stream) {
-    using Size = Sizes<NG, NT, NC>;
+    using Size = Sizes<NG, NT, NC, kSelected>;
     constexpr int kSmem = Size::kRing + Size::kMerge;
     static_assert(kSmem + sizeof(Queries<NT>) < 225 * 1024, "one CTA fits an SM");
     auto kernel = attention_kernel<NG, NT, NC, kSelected>;
     if (int status = allow_dynamic_smem(kernel, kSmem)) return status;
     const unsigned grid = static_cast<unsigned>(most_chunks < kMostCtas ? most_chunks : kMostCtas);
-    const cudaError_t err = launch_pdl(kernel, dim3(grid), dim3(kThreads), kSmem, stream, 1, p);
+    const cudaError_t err = launch_pdl(kernel, dim3(grid), dim3(32 * Size::kWarps), kSmem, stream, 1, p);
     if (err != cudaSuccess) return fail(POPKV_ERR_CUDA, "%s: %s", what, cudaGetErrorString(err));
     return check_launch(what);
 }
@@ -1247,6 +1289,8 @@ extern "C" int popkv_kv4_attention_selected(const popkv_kv4_cache* cache, int64_
     if (int status = check_queries(what, p.view, layer, n, q_heads, 1, dtype, queries, q_seq_stride, q_head_stride, 0))
         return status;
     if (selected < 0 || selected > (1 << 30)) return fail(POPKV_ERR_INVALID, "%s: selected out of range", what);
+    if (p.view.layer_bytes / 16 > 0xFFFFFFFFll)
+        return fail(POPKV_ERR_UNSUPPORTED, "%s: at most 64 GiB of pages in a layer", what);
     if (n == 0) return POPKV_OK;
     if (!seqs || !queries || !out || (selected && !indices)) return fail(POPKV_ERR_INVALID, "%s: null pointer", what);
     p.layer = static_cast<int>(layer);
