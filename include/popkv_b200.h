@@ -771,13 +771,15 @@ POPKV_API int popkv_kv4_copy_pages(const popkv_kv4_cache* cache, const int32_t* 
  * everywhere), p when none was refused.  With noise ~ Exp(1), uniforms ~ U[0, 1) the tokens
  * are distributed as the target's.  A drafted id out of range is refused.
  * out_tokens int64 [n, drafts + 1]: the accepted drafts, the next token, then -1;
- * accepted int32 [n].  The reference decodes one token per call and has no counterpart.
+ * accepted int32 [n].  workspace: 12 n bytes, 8-byte aligned, zero before the first call; every
+ * call leaves it zero.  Calls that overlap in time need a workspace each.
+ * The reference decodes one token per call and has no counterpart.
  */
 POPKV_API int popkv_verify_drafts(const void* target, int64_t t_seq_stride, int64_t t_place_stride,
                                   const void* draft, int64_t d_seq_stride, int64_t d_place_stride, int dtype,
                                   int64_t n, int64_t drafts, int64_t vocab, const int64_t* tokens,
                                   const int32_t* counts, const float* uniforms, const float* noise,
-                                  int64_t* out_tokens, int32_t* accepted, void* stream);
+                                  void* workspace, int64_t* out_tokens, int32_t* accepted, void* stream);
 
 #ifdef __cplusplus
 }

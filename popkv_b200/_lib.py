@@ -83,7 +83,7 @@ _SIGNATURES = {
     "popkv_kv4_truncate": ([_P, _P, _L, _P, _P], _I),
     "popkv_kv4_compact": ([_P, _P, _P], _I),
     "popkv_kv4_copy_pages": ([_P, _P, _P, _L, _P], _I),
-    "popkv_verify_drafts": ([_P, _L, _L, _P, _L, _L, _I, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P], _I),
+    "popkv_verify_drafts": ([_P, _L, _L, _P, _L, _L, _I, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P], _I),
     "popkv_norm_lm_head_argmax": ([_P, _L, _L, _L, _P, _P, _P, ctypes.c_float, _P, _P, _P, _P, _P, _P], _I),
 }
 

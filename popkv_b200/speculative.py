@@ -13,9 +13,36 @@ import torch
 from . import _lib
 
 
+_workspaces: dict[tuple[int, int], torch.Tensor] = {}  # of each (device, stream): all zero between calls
+
+
+def verify_workspace(n: int, device) -> torch.Tensor:
+    """Scratch for ``verify_drafts`` calls of up to ``n`` sequences, zeroed.
+
+    Without one, calls keep one per stream; inside a graph capture, where that cannot be, each call
+    would allocate and clear its own.  Calls that overlap in time need one each.
+    """
+    return torch.zeros(12 * n, dtype=torch.uint8, device=device)
+
+
+def _workspace(given, n: int, device, stream: int) -> torch.Tensor:
+    if given is not None:
+        if given.dtype != torch.uint8 or not given.is_contiguous() or given.device != device or given.numel() < 12 * n:
+            raise ValueError(f"workspace must be a tensor of verify_workspace({n}, ...)")
+        return given
+    held = _workspaces.get((device.index, stream))
+    if held is not None and held.numel() >= 12 * n:
+        return held
+    made = verify_workspace(n, device)
+    if not torch.cuda.is_current_stream_capturing():
+        _workspaces[device.index, stream] = made
+    return made
+
+
 def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, uniforms: torch.Tensor,
                   noise: torch.Tensor, *, draft_probs: torch.Tensor | None = None,
-                  counts: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+                  counts: torch.Tensor | None = None,
+                  workspace: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Accept drafted tokens against the target's probabilities, from given random numbers.
 
     Args:
@@ -28,6 +55,7 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, unifor
             drafts that were not drawn at random (greedy or looked up).
         counts: int32 [n], drafts of each sequence (default all); row j = counts[i] of target_probs
             follows the last one.
+        workspace: a tensor of ``verify_workspace``, for calls inside a graph capture.
 
     Draft j is accepted while ``uniforms * q(draft) < p(draft)``.  The following token wins the race
     ``argmax weight / noise`` over weight > 0, weight = max(p - q, 0) at the first refusal (p where
@@ -38,40 +66,57 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, unifor
     """
     if target_probs.ndim != 3 or draft_tokens.ndim != 2:
         raise ValueError("target_probs must be [n, drafts + 1, vocab] and draft_tokens [n, drafts]")
-    n, drafts = (int(x) for x in draft_tokens.shape)
-    vocab = int(target_probs.shape[2])
-    if tuple(target_probs.shape[:2]) != (n, drafts + 1) or vocab < 1:
+    n, drafts = draft_tokens.shape
+    shape = target_probs.shape
+    vocab = shape[2]
+    if shape[0] != n or shape[1] != drafts + 1 or vocab < 1:
         raise ValueError("target_probs must be [n, drafts + 1, vocab]")
-    if tuple(uniforms.shape) != (n, drafts) or tuple(noise.shape) != (n, vocab):
+    if uniforms.shape != (n, drafts) or noise.shape != (n, vocab):
         raise ValueError("uniforms must be [n, drafts] and noise [n, vocab]")
-    if draft_probs is not None and tuple(draft_probs.shape) != (n, drafts, vocab):
-        raise ValueError("draft_probs must be [n, drafts, vocab]")
-    if counts is not None and tuple(counts.shape) != (n,):
-        raise ValueError("counts must be [n]")
-    device = target_probs.device
-    given = [draft_tokens, uniforms, noise] + [t for t in (draft_probs, counts) if t is not None]
+    dtype, device = target_probs.dtype, target_probs.device
+    given = [draft_tokens, uniforms, noise]
+    if draft_probs is not None:
+        if draft_probs.shape != (n, drafts, vocab):
+            raise ValueError("draft_probs must be [n, drafts, vocab]")
+        given.append(draft_probs)
+    if counts is not None:
+        if counts.shape != (n,):
+            raise ValueError("counts must be [n]")
+        given.append(counts)
     if device.type != "cuda" or any(t.device != device for t in given):
         raise RuntimeError("verification tensors must share a CUDA device")
-    if target_probs.dtype not in _lib.DTYPE_CODES or (draft_probs is not None
-                                                      and draft_probs.dtype != target_probs.dtype):
+    code = _lib.DTYPE_CODES.get(dtype)
+    if code is None or (draft_probs is not None and draft_probs.dtype != dtype):
         raise RuntimeError("probabilities must share an fp32/fp16/bf16 dtype")
     if draft_tokens.dtype != torch.int64 or uniforms.dtype != torch.float32 or noise.dtype != torch.float32:
         raise RuntimeError("draft_tokens must be int64, uniforms and noise fp32")
     if counts is not None and counts.dtype != torch.int32:
         raise RuntimeError("counts must be int32")
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return _verify(target_probs, draft_tokens, uniforms, noise, draft_probs, counts, workspace, code)
+    return _verify(target_probs, draft_tokens, uniforms, noise, draft_probs, counts, workspace, code)
+
+
+def _verify(target_probs, draft_tokens, uniforms, noise, draft_probs, counts, workspace, code):
+    n, places, vocab = target_probs.shape
+    device = target_probs.device
     target_probs = target_probs if target_probs.stride(2) == 1 else target_probs.contiguous()
-    if draft_probs is not None and draft_probs.stride(2) != 1:
-        draft_probs = draft_probs.contiguous()
+    draft, d_seq, d_place = None, 0, 0
+    if draft_probs is not None:
+        draft_probs = draft_probs if draft_probs.stride(2) == 1 else draft_probs.contiguous()
+        draft, (d_seq, d_place, _) = draft_probs.data_ptr(), draft_probs.stride()
     draft_tokens, uniforms, noise = draft_tokens.contiguous(), uniforms.contiguous(), noise.contiguous()
     counts = None if counts is None else counts.contiguous()
-    tokens = torch.empty((n, drafts + 1), dtype=torch.int64, device=device)
+    tokens = torch.empty((n, places), dtype=torch.int64, device=device)
     accepted = torch.empty(n, dtype=torch.int32, device=device)
-    args = (target_probs.data_ptr(), target_probs.stride(0), target_probs.stride(1),
-            None if draft_probs is None else draft_probs.data_ptr(),
-            0 if draft_probs is None else draft_probs.stride(0), 0 if draft_probs is None else draft_probs.stride(1),
-            _lib.DTYPE_CODES[target_probs.dtype], n, drafts, vocab, draft_tokens.data_ptr(),
-            None if counts is None else counts.data_ptr(), uniforms.data_ptr(), noise.data_ptr(), tokens.data_ptr(),
-            accepted.data_ptr())
-    with torch.cuda.device(device):
-        _lib.check(_lib.lib().popkv_verify_drafts(*args, torch.cuda.current_stream(device).cuda_stream))
+    stream = torch.cuda.current_stream(device).cuda_stream
+    scratch = _workspace(workspace, n, device, stream)
+    t_seq, t_place, _ = target_probs.stride()
+    status = _lib.lib().popkv_verify_drafts(
+        target_probs.data_ptr(), t_seq, t_place, draft, d_seq, d_place, code, n, places - 1, vocab,
+        draft_tokens.data_ptr(), None if counts is None else counts.data_ptr(), uniforms.data_ptr(),
+        noise.data_ptr(), scratch.data_ptr(), tokens.data_ptr(), accepted.data_ptr(), stream)
+    if status:
+        _lib.check(status)
     return tokens, accepted

@@ -65,10 +65,21 @@ def test_entries_check_their_arguments(lib):
     refused(lib, lib.popkv_kv4_extend(c, p, 1, None, 1, None, None), "null pointer")
     refused(lib, lib.popkv_kv4_fork(c, p, None, 1, p, None), "null pointer")
     refused(lib, lib.popkv_kv4_copy_pages(c, p, p, -1, None), "count out of range")
-    refused(lib, lib.popkv_verify_drafts(p, 1, 1, p, 1, 1, 9, 1, 1, 10, p, None, p, p, p, p, None), "fp32/fp16/bf16")
-    refused(lib, lib.popkv_verify_drafts(p, 1, 1, p, 1, 1, 0, 1, 1, 0, p, None, p, p, p, p, None), "sizes out of range")
-    refused(lib, lib.popkv_verify_drafts(p, 1, 1, p, 1, 1, 0, 1, 2000, 10, p, None, p, p, p, p, None), "sizes out of")
-    refused(lib, lib.popkv_verify_drafts(p, 1, 1, p, 1, 1, 0, 1, 1, 10, None, None, p, p, p, p, None), "null pointer")
+    refused(lib, lib.popkv_verify_drafts(p, 1, 1, p, 1, 1, 9, 1, 1, 10, p, None, p, p, p, p, p, None), "fp32/fp16/bf16")
+    refused(lib, lib.popkv_verify_drafts(p, 1, 1, p, 1, 1, 0, 1, 1, 0, p, None, p, p, p, p, p, None), "sizes out of range")
+    refused(lib, lib.popkv_verify_drafts(p, 1, 1, p, 1, 1, 0, 1, 2000, 10, p, None, p, p, p, p, p, None), "sizes out of")
+    refused(lib, lib.popkv_verify_drafts(p, 1, 1, p, 1, 1, 0, 1, 1, 10, None, None, p, p, p, p, p, None), "null pointer")
+    refused(lib, lib.popkv_verify_drafts(p, 1, 1, p, 1, 1, 0, 1, 1, 10, p, None, p, p, None, p, p, None), "workspace")
+    refused(lib, lib.popkv_kv4_attention(c, 0, p, 1, None, p, 2, 3, 1, 8, 8, 8, 1.0, p, 1 << 30, p, None), "multiple of")
+    refused(lib, lib.popkv_kv4_attention(c, 0, p, 1, None, p, 0, 4, 1, 8, 8, 8, 1.0, p, 1 << 30, p, None), "fp16 or bf16")
+    refused(lib, lib.popkv_kv4_attention(c, 0, p, 1, None, p, 2, 4, 1, 8, 8, 4, 1.0, p, 1 << 30, p, None), "aligned")
+    refused(lib, lib.popkv_kv4_attention(c, 0, p, 1, None, p, 2, 4, 1, 8, 8, 8, 1.0, p, 100, p, None), "workspace")
+    refused(lib, lib.popkv_kv4_attention(c, 2, p, 1, None, p, 2, 4, 1, 8, 8, 8, 1.0, p, 100, p, None), "layer out of")
+    refused(lib, lib.popkv_kv4_attention_selected(c, 0, p, 1, p, 2, 4, 8, 8, None, 5, None, 1.0, p, 1 << 30, p, None),
+            "null pointer")
+    refused(lib, lib.popkv_kv4_attention_selected(c, 0, p, 1, p, 2, 4, 8, 8, p, -1, None, 1.0, p, 1 << 30, p, None),
+            "selected out of range")
+    assert lib.popkv_kv4_attention_workspace(1, 2, 3, 1) == -1 and lib.popkv_kv4_attention_workspace(1, 2, 4, 1) > 0
     # Nothing to do is no error, and needs no GPU.
     assert lib.popkv_kv4_extend(c, None, 0, None, 1, None, None) == 0
     assert lib.popkv_kv4_write(c, 0, None, 0, None, None, None, 2, 1, 1, 1, 1, 1, 1, 1, None) == 0
