@@ -54,6 +54,8 @@ __device__ int block_scan(int value, int* total) {
 __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Kv4View view, const int32_t* __restrict__ seqs, int n,
                                                               const int32_t* __restrict__ counts, int count,
                                                               int32_t* __restrict__ workspace) {
+    pdl_wait();
+    pdl_launch_dependents();
     int32_t* found = workspace;
     int32_t* first = found + view.num_pages;
     int32_t* source = first + n;
@@ -144,50 +146,80 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Kv4View view, cons
     }
 }
 
-// fork, first half: the parents' rows as they are, and a reference more for each page.
-__global__ void __launch_bounds__(kRowThreads) fork_read_kernel(Kv4View view, const int32_t* __restrict__ parents,
-                                                                const int32_t* __restrict__ children, int n,
-                                                                int32_t* __restrict__ workspace) {
-    const int i = blockIdx.x;
+// fork, first half, entry i: the parent's row as it is, and a reference more for each page.
+__device__ void fork_read(const Kv4View& view, const int32_t* parents, const int32_t* children, int n, int i, int thread,
+                          int threads, int32_t* workspace) {
     const int parent = parents[i];
     const bool fine = view.has_sequence(parent) && first_of(view, children, i);
-    if (threadIdx.x == 0) {
+    if (thread == 0) {
         workspace[i] = fine ? view.length_of(parent) : -1;
         if (!fine && children[i] != -1) atomicOr(view.status, kKv4StatusSequence);
     }
     if (!fine) return;
     int32_t* row = workspace + n + static_cast<int64_t>(i) * view.max_pages;
     const int pages = view.pages_of(view.length_of(parent));
-    for (int j = threadIdx.x; j < pages; j += kRowThreads) {
+    for (int j = thread; j < pages; j += threads) {
         const int page = view.table[static_cast<int64_t>(parent) * view.max_pages + j];
         row[j] = page;
         if (page >= 0 && page < view.num_pages) atomicAdd(view.refs + page, 1);
     }
 }
 
-// fork, second half: each child gives its pages back and takes the rows read.
-__global__ void __launch_bounds__(kRowThreads) fork_write_kernel(Kv4View view, const int32_t* __restrict__ children,
-                                                                 int n, const int32_t* __restrict__ workspace) {
-    const int i = blockIdx.x;
+// fork, second half: the child gives its pages back and takes the row read.  Its length is
+// written by the caller, after every thread has read the old one.
+__device__ void fork_write(const Kv4View& view, const int32_t* children, int n, int i, int thread, int threads,
+                           const int32_t* workspace) {
     const int length = workspace[i];
     if (length < 0) return;
     const int child = children[i];
     const int before = view.pages_of(view.length_of(child)), after = view.pages_of(length);
     const int32_t* row = workspace + n + static_cast<int64_t>(i) * view.max_pages;
     int32_t* to = view.table + static_cast<int64_t>(child) * view.max_pages;
-    for (int j = threadIdx.x; j < max(before, after); j += kRowThreads) {
+    for (int j = thread; j < max(before, after); j += threads) {
         if (j < before) {
             const int page = to[j];
             if (page >= 0 && page < view.num_pages) atomicSub(view.refs + page, 1);
         }
         to[j] = j < after ? row[j] : -1;
     }
+}
+
+// Both halves in one CTA, a warp per entry.
+__global__ void __launch_bounds__(kPlanThreads) fork_kernel(Kv4View view, const int32_t* __restrict__ parents,
+                                                            const int32_t* __restrict__ children, int n,
+                                                            int32_t* __restrict__ workspace) {
+    pdl_wait();
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int i = warp; i < n; i += kPlanThreads / 32) fork_read(view, parents, children, n, i, lane, 32, workspace);
     __syncthreads();
-    if (threadIdx.x == 0) view.lengths[child] = length;
+    for (int i = warp; i < n; i += kPlanThreads / 32) fork_write(view, children, n, i, lane, 32, workspace);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kPlanThreads)
+        if (workspace[i] >= 0) view.lengths[children[i]] = workspace[i];
+}
+
+__global__ void __launch_bounds__(kRowThreads) fork_read_kernel(Kv4View view, const int32_t* __restrict__ parents,
+                                                                const int32_t* __restrict__ children, int n,
+                                                                int32_t* __restrict__ workspace) {
+    pdl_wait();
+    pdl_launch_dependents();
+    fork_read(view, parents, children, n, blockIdx.x, threadIdx.x, kRowThreads, workspace);
+}
+
+__global__ void __launch_bounds__(kRowThreads) fork_write_kernel(Kv4View view, const int32_t* __restrict__ children,
+                                                                 int n, const int32_t* __restrict__ workspace) {
+    pdl_wait();
+    pdl_launch_dependents();
+    fork_write(view, children, n, blockIdx.x, threadIdx.x, kRowThreads, workspace);
+    __syncthreads();
+    if (threadIdx.x == 0 && workspace[blockIdx.x] >= 0) view.lengths[children[blockIdx.x]] = workspace[blockIdx.x];
 }
 
 __global__ void __launch_bounds__(kRowThreads) truncate_kernel(Kv4View view, const int32_t* __restrict__ seqs,
                                                                const int32_t* __restrict__ lengths) {
+    pdl_wait();
+    pdl_launch_dependents();
     const int i = blockIdx.x;
     if (!first_of(view, seqs, i)) {
         if (threadIdx.x == 0 && seqs[i] != -1) atomicOr(view.status, kKv4StatusSequence);
@@ -207,6 +239,8 @@ __global__ void __launch_bounds__(kRowThreads) truncate_kernel(Kv4View view, con
 
 // One CTA.  workspace: source [num_pages] | target [num_pages] | place [num_pages].
 __global__ void __launch_bounds__(kPlanThreads) compact_kernel(Kv4View view, int32_t* __restrict__ workspace) {
+    pdl_wait();
+    pdl_launch_dependents();
     int32_t* source = workspace;
     int32_t* target = source + view.num_pages;
     int32_t* place = target + view.num_pages;
@@ -243,6 +277,8 @@ __global__ void __launch_bounds__(kPlanThreads) compact_kernel(Kv4View view, int
 }
 
 __global__ void __launch_bounds__(kRowThreads) place_kernel(Kv4View view, const int32_t* __restrict__ workspace) {
+    pdl_wait();
+    pdl_launch_dependents();
     const int s = blockIdx.x;
     const int live = view.status[1];
     const int32_t* place = workspace + 2 * static_cast<int64_t>(view.num_pages);
@@ -254,21 +290,38 @@ __global__ void __launch_bounds__(kRowThreads) place_kernel(Kv4View view, const 
     }
 }
 
-// Page i of layer blockIdx.z, one part of it per blockIdx.x.
+// A persistent grid over (entry, layer, part of the page); a thread has kUnits 16-byte loads in
+// flight.  Bound by HBM: a copy of 0.5 GB runs at what the device's plain copy reaches.
+constexpr int kUnits = 8;
+
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(Kv4View view, const int32_t* __restrict__ sources,
                                                             const int32_t* __restrict__ targets, int64_t count,
                                                             const int32_t* __restrict__ count_dev) {
+    pdl_wait();
+    pdl_launch_dependents();
     if (count_dev) count = min(count, static_cast<int64_t>(*count_dev));
-    const int64_t units = view.page_bytes / 16;
-    for (int64_t i = blockIdx.y; i < count; i += gridDim.y) {
-        const int from = sources[i], to = targets[i];
+    const int units = static_cast<int>(view.page_bytes / 16);
+    constexpr int kPart = kCopyThreads * kUnits;
+    const int parts = (units + kPart - 1) / kPart;
+    const int64_t items = count * view.layers * parts;
+    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+        const int64_t of_page = item / parts;
+        const int part = static_cast<int>(item - of_page * parts);
+        const int64_t entry = of_page / view.layers;
+        const int layer_number = static_cast<int>(of_page - entry * view.layers);
+        const int from = sources[entry], to = targets[entry];
         if (from < 0 || from >= view.num_pages || to < 0 || to >= view.num_pages) continue;
-        const uint8_t* layer = view.pages + blockIdx.z * view.layer_bytes;
+        uint8_t* layer = view.pages + layer_number * view.layer_bytes;
         const auto* src = reinterpret_cast<const uint4*>(layer + from * view.page_bytes);
-        auto* dst = reinterpret_cast<uint4*>(const_cast<uint8_t*>(layer) + to * view.page_bytes);
-        for (int64_t u = blockIdx.x * static_cast<int64_t>(kCopyThreads) + threadIdx.x; u < units;
-             u += static_cast<int64_t>(gridDim.x) * kCopyThreads)
-            dst[u] = src[u];
+        auto* dst = reinterpret_cast<uint4*>(layer + to * view.page_bytes);
+        uint4 v[kUnits];
+        const int first = part * kPart + threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i)
+            if (first + i * kCopyThreads < units) v[i] = __ldcs(src + first + i * kCopyThreads);
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i)
+            if (first + i * kCopyThreads < units) __stcs(dst + first + i * kCopyThreads, v[i]);
     }
 }
 
@@ -277,10 +330,12 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(Kv4View view, const 
 int kv4_copy_launch(const char* what, const Kv4View& view, const int32_t* sources, const int32_t* targets,
                     int64_t count, const int32_t* count_dev, cudaStream_t stream) {
     if (count == 0) return POPKV_OK;
-    const int64_t units = view.page_bytes / 16;
-    const unsigned x = static_cast<unsigned>(units > 16 * kCopyThreads ? 16 : (units + kCopyThreads - 1) / kCopyThreads);
-    const unsigned y = static_cast<unsigned>(count > 4096 ? 4096 : count);
-    copy_kernel<<<dim3(x, y, view.layers), kCopyThreads, 0, stream>>>(view, sources, targets, count, count_dev);
+    constexpr int64_t kGrid = 148 * 6;
+    const int64_t units = view.page_bytes / 16, part = kCopyThreads * kUnits;
+    const int64_t items = count * view.layers * ((units + part - 1) / part);
+    const cudaError_t err = launch_pdl(copy_kernel, dim3(static_cast<unsigned>(items < kGrid ? items : kGrid)),
+                                       dim3(kCopyThreads), 0, stream, 1, view, sources, targets, count, count_dev);
+    if (err != cudaSuccess) return fail(POPKV_ERR_CUDA, "%s: %s", what, cudaGetErrorString(err));
     return check_launch(what);
 }
 
@@ -300,6 +355,15 @@ extern "C" int popkv_kv4_copy_pages(const popkv_kv4_cache* cache, const int32_t*
 
 namespace popkv {
 namespace {
+template <typename... Parameters, typename... Arguments>
+int launch_plan(const char* what, void (*kernel)(Parameters...), unsigned blocks, int threads, void* stream,
+                Arguments... arguments) {
+    const cudaError_t err =
+        launch_pdl(kernel, dim3(blocks), dim3(threads), 0, static_cast<cudaStream_t>(stream), 1, arguments...);
+    if (err != cudaSuccess) return fail(POPKV_ERR_CUDA, "%s: %s", what, cudaGetErrorString(err));
+    return check_launch(what);
+}
+
 int check_entries(const char* what, int64_t n) {
     if (n < 0 || n > 4096) return fail(POPKV_ERR_INVALID, "%s: between 0 and 4096 sequences in one call", what);
     return POPKV_OK;
@@ -317,9 +381,9 @@ extern "C" int popkv_kv4_extend(const popkv_kv4_cache* cache, const int32_t* seq
     if (n == 0) return POPKV_OK;
     if (!seqs || !workspace) return fail(POPKV_ERR_INVALID, "popkv_kv4_extend: null pointer");
     const auto s = static_cast<cudaStream_t>(stream);
-    extend_kernel<<<1, kPlanThreads, 0, s>>>(view, seqs, static_cast<int>(n), counts, static_cast<int>(count),
-                                             workspace);
-    if (int status = check_launch("popkv_kv4_extend")) return status;
+    if (int status = launch_plan("popkv_kv4_extend", extend_kernel, 1, kPlanThreads, stream, view, seqs,
+                                 static_cast<int>(n), counts, static_cast<int>(count), workspace))
+        return status;
     const int32_t* source = workspace + view.num_pages + n;
     return kv4_copy_launch("popkv_kv4_extend", view, source, source + n, n, nullptr, s);
 }
@@ -332,11 +396,16 @@ extern "C" int popkv_kv4_fork(const popkv_kv4_cache* cache, const int32_t* paren
     if (int status = check_entries("popkv_kv4_fork", n)) return status;
     if (n == 0) return POPKV_OK;
     if (!parents || !children || !workspace) return fail(POPKV_ERR_INVALID, "popkv_kv4_fork: null pointer");
-    const auto s = static_cast<cudaStream_t>(stream);
     const int count = static_cast<int>(n);
-    fork_read_kernel<<<count, kRowThreads, 0, s>>>(view, parents, children, count, workspace);
-    fork_write_kernel<<<count, kRowThreads, 0, s>>>(view, children, count, workspace);
-    return check_launch("popkv_kv4_fork");
+    const char* what = "popkv_kv4_fork";
+    // One CTA for both halves while the rows are few (one launch less), a CTA per row beyond.
+    if (n * view.max_pages <= 32768)
+        return launch_plan(what, fork_kernel, 1, kPlanThreads, stream, view, parents, children, count, workspace);
+    if (int status = launch_plan(what, fork_read_kernel, count, kRowThreads, stream, view, parents, children, count,
+                                 workspace))
+        return status;
+    return launch_plan(what, fork_write_kernel, count, kRowThreads, stream, view, children, count,
+                       static_cast<const int32_t*>(workspace));
 }
 
 extern "C" int popkv_kv4_truncate(const popkv_kv4_cache* cache, const int32_t* seqs, int64_t n,
@@ -347,9 +416,8 @@ extern "C" int popkv_kv4_truncate(const popkv_kv4_cache* cache, const int32_t* s
     if (int status = check_entries("popkv_kv4_truncate", n)) return status;
     if (n == 0) return POPKV_OK;
     if (!seqs) return fail(POPKV_ERR_INVALID, "popkv_kv4_truncate: null pointer");
-    truncate_kernel<<<static_cast<unsigned>(n), kRowThreads, 0, static_cast<cudaStream_t>(stream)>>>(view, seqs,
-                                                                                                      lengths);
-    return check_launch("popkv_kv4_truncate");
+    return launch_plan("popkv_kv4_truncate", truncate_kernel, static_cast<unsigned>(n), kRowThreads, stream, view, seqs,
+                       lengths);
 }
 
 extern "C" int popkv_kv4_compact(const popkv_kv4_cache* cache, int32_t* workspace, void* stream) {
@@ -357,10 +425,11 @@ extern "C" int popkv_kv4_compact(const popkv_kv4_cache* cache, int32_t* workspac
     Kv4View view;
     if (int status = kv4_view("popkv_kv4_compact", cache, &view)) return status;
     if (!workspace) return fail(POPKV_ERR_INVALID, "popkv_kv4_compact: null pointer");
-    const auto s = static_cast<cudaStream_t>(stream);
-    compact_kernel<<<1, kPlanThreads, 0, s>>>(view, workspace);
-    place_kernel<<<view.max_seqs, kRowThreads, 0, s>>>(view, workspace);
-    if (int status = check_launch("popkv_kv4_compact")) return status;
-    return kv4_copy_launch("popkv_kv4_compact", view, workspace, workspace + view.num_pages, view.num_pages,
-                           view.status + 2, s);
+    const char* what = "popkv_kv4_compact";
+    if (int status = launch_plan(what, compact_kernel, 1, kPlanThreads, stream, view, workspace)) return status;
+    if (int status = launch_plan(what, place_kernel, static_cast<unsigned>(view.max_seqs), kRowThreads, stream, view,
+                                 static_cast<const int32_t*>(workspace)))
+        return status;
+    return kv4_copy_launch(what, view, workspace, workspace + view.num_pages, view.num_pages, view.status + 2,
+                           static_cast<cudaStream_t>(stream));
 }

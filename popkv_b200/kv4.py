@@ -111,7 +111,7 @@ class Kv4Cache:
         self.lengths = tables[self.num_pages:self.num_pages + self.max_seqs]
         self.table = tables[self.num_pages + self.max_seqs:].view(self.max_seqs, -1)
         self.max_pages = int(self.table.shape[1])
-        self.device = pages.device
+        self.device = pages.device  # a CUDA device has its index here
         self.status = torch.zeros(4, dtype=torch.int32, device=pages.device)
         self._descriptor = _Descriptor(
             pages.data_ptr(), self.refs.data_ptr(), self.lengths.data_ptr(), self.table.data_ptr(),
@@ -119,17 +119,18 @@ class Kv4Cache:
             self.dim_group_size, self.max_seqs, self.max_pages)
         self._address = ctypes.addressof(self._descriptor)
         self._workspaces = {}  # of each stream: the attention's scratch and the sizes it holds
+        self._scratches = {}   # of each stream: the page operations' scratch
 
     # -- arguments -----------------------------------------------------------------
     def _call(self, entry, *args) -> None:
-        device = self.device
-        if device.type != "cuda":
+        index = self.device.index
+        if index is None:
             raise RuntimeError("the 4-bit cache must be on a CUDA device")
-        if torch.cuda.current_device() == device.index:
-            status = entry(self._address, *args, torch.cuda.current_stream(device).cuda_stream)
+        if torch.cuda.current_device() == index:
+            status = entry(self._address, *args, _lib.raw_stream(index))
         else:
-            with torch.cuda.device(device):
-                status = entry(self._address, *args, torch.cuda.current_stream(device).cuda_stream)
+            with torch.cuda.device(index):
+                status = entry(self._address, *args, _lib.raw_stream(index))
         if status:
             _lib.check(status)
 
@@ -147,15 +148,17 @@ class Kv4Cache:
             raise RuntimeError(f"{name} must be on the cache's device")
         return ids
 
-    def _sequences(self, seqs, name: str = "seqs", most: int = MAX_SEQUENCES_PER_CALL) -> torch.Tensor:
+    def _sequences(self, seqs, name: str = "seqs", most: int = MAX_SEQUENCES_PER_CALL) -> tuple[torch.Tensor, int]:
+        """The ids and their number."""
         seqs = self._ids(seqs, name)
-        if seqs.shape[0] > most:
+        n = seqs.shape[0]
+        if n > most:
             raise ValueError(f"at most {most} sequences in one call")
-        return seqs
+        return seqs, n
 
-    def _per_sequence(self, values, seqs: torch.Tensor, name: str) -> torch.Tensor:
+    def _per_sequence(self, values, n: int, name: str) -> torch.Tensor:
         values = self._ids(values, name)
-        if values.shape[0] != seqs.shape[0]:
+        if values.shape[0] != n:
             raise ValueError(f"{name} must have one value per listed sequence")
         return values
 
@@ -163,6 +166,17 @@ class Kv4Cache:
         if not 0 <= layer < self.layers:
             raise ValueError(f"layer must be in [0, {self.layers})")
         return layer
+
+    def _scratch(self, numbers: int) -> torch.Tensor:
+        """int32 scratch of a page operation, one buffer per stream (its own inside a graph capture)."""
+        index = self.device.index
+        if index is None or torch.cuda.is_current_stream_capturing():
+            return torch.empty(numbers, dtype=torch.int32, device=self.device)
+        key = _lib.raw_stream(index)
+        held = self._scratches.get(key)
+        if held is None or held.shape[0] < numbers:
+            held = self._scratches[key] = torch.empty(numbers, dtype=torch.int32, device=self.device)
+        return held
 
     # -- rows ----------------------------------------------------------------------
     def write(self, keys: torch.Tensor, values: torch.Tensor, *, seqs, layer: int = 0, counts=None) -> None:
@@ -175,20 +189,28 @@ class Kv4Cache:
         """
         if keys.ndim == 3 and values.ndim == 3:
             keys, values = keys.unsqueeze(1), values.unsqueeze(1)
-        seqs = self._sequences(seqs, most=1 << 30)
-        if (keys.ndim != 4 or keys.shape != values.shape or keys.shape[0] != seqs.shape[0]
-                or keys.shape[2] != self.kv_heads or keys.shape[3] != HEAD_DIM):
-            raise ValueError(f"keys and values must be [{seqs.shape[0]}, tokens, {self.kv_heads}, {HEAD_DIM}]")
-        if keys.dtype != values.dtype or keys.dtype not in _lib.DTYPE_CODES:
+        seqs, n = self._sequences(seqs, most=1 << 30)
+        shape = keys.shape
+        if (len(shape) != 4 or shape != values.shape or shape[0] != n or shape[2] != self.kv_heads
+                or shape[3] != HEAD_DIM):
+            raise ValueError(f"keys and values must be [{n}, tokens, {self.kv_heads}, {HEAD_DIM}]")
+        code = _lib.DTYPE_CODES.get(keys.dtype)
+        if code is None or keys.dtype != values.dtype:
             raise RuntimeError("keys and values must share an fp32/fp16/bf16 dtype")
         if keys.device != self.device or values.device != self.device:
             raise RuntimeError("keys and values must be on the cache's device")
-        keys, values = _rows(keys), _rows(values)
-        counts = None if counts is None else self._per_sequence(counts, seqs, "counts")
-        ks, vs = keys.stride(), values.stride()
-        self._call(_lib.lib().popkv_kv4_write, self._layer(layer), seqs.data_ptr(), seqs.shape[0],
-                   None if counts is None else counts.data_ptr(), keys.data_ptr(), values.data_ptr(),
-                   _lib.DTYPE_CODES[keys.dtype], keys.shape[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2])
+        k0, k1, k2, last = keys.stride()
+        if last != 1:
+            keys = keys.contiguous()
+            k0, k1, k2, _ = keys.stride()
+        v0, v1, v2, last = values.stride()
+        if last != 1:
+            values = values.contiguous()
+            v0, v1, v2, _ = values.stride()
+        counts = None if counts is None else self._per_sequence(counts, n, "counts")
+        self._call(_lib.lib().popkv_kv4_write, self._layer(layer), seqs.data_ptr(), n,
+                   None if counts is None else counts.data_ptr(), keys.data_ptr(), values.data_ptr(), code, shape[1],
+                   k0, k1, k2, v0, v1, v2)
 
     def read(self, seqs, *, start: int = 0, tokens: int, layer: int = 0,
              dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
@@ -196,60 +218,67 @@ class Kv4Cache:
 
         Rows past a sequence's end are zeros.
         """
-        if dtype not in _lib.DTYPE_CODES:
+        code = _lib.DTYPE_CODES.get(dtype)
+        if code is None:
             raise RuntimeError("dtype must be fp32/fp16/bf16")
         if start < 0 or tokens < 0:
             raise ValueError("start and tokens must not be negative")
-        seqs = self._sequences(seqs, most=1 << 30)
-        shape = (seqs.shape[0], tokens, self.kv_heads, HEAD_DIM)
-        keys = torch.empty(shape, dtype=dtype, device=self.device)
-        values = torch.empty(shape, dtype=dtype, device=self.device)
-        self._call(_lib.lib().popkv_kv4_read, self._layer(layer), seqs.data_ptr(), seqs.shape[0], start, tokens,
-                   keys.data_ptr(), values.data_ptr(), _lib.DTYPE_CODES[dtype])
+        seqs, n = self._sequences(seqs, most=1 << 30)
+        keys, values = torch.empty((2, n, tokens, self.kv_heads, HEAD_DIM), dtype=dtype, device=self.device).unbind(0)
+        self._call(_lib.lib().popkv_kv4_read, self._layer(layer), seqs.data_ptr(), n, start, tokens, keys.data_ptr(),
+                   values.data_ptr(), code)
         return keys, values
 
     # -- attention -----------------------------------------------------------------
     def workspace(self, n: int, q_heads: int, q_len: int = 1) -> torch.Tensor:
-        """Scratch for attention calls of up to these sizes, zeroed, for the ``workspace`` arguments.
+        """Scratch for attention calls of up to these sizes, for the ``workspace`` arguments.
 
-        Without one, calls keep one per stream; inside a graph capture, where that cannot be, each
-        call would allocate and clear its own.  Calls that overlap in time need one each.
+        Without one, calls keep one per stream; inside a graph capture each call would make and clear
+        its own.  Calls that overlap in time need one each.
         """
-        size = _lib.lib().popkv_kv4_attention_workspace(n, self.kv_heads, q_heads, q_len)
+        lib = _lib.lib()
+        size = lib.popkv_kv4_attention_workspace(n, self.kv_heads, q_heads, q_len)
         if size < 0:
             raise ValueError("query heads must be a multiple of the cache's KV heads")
-        return torch.zeros(size, dtype=torch.uint8, device=self.device)
+        made = torch.empty(size, dtype=torch.uint8, device=self.device)
+        made[lib.popkv_kv4_attention_workspace(0, self.kv_heads, q_heads, q_len):].zero_()  # the counters
+        return made
 
     def _workspace(self, given, n: int, q_heads: int, q_len: int) -> torch.Tensor:
         if given is not None:
             if given.dtype != torch.uint8 or not given.is_contiguous() or given.device != self.device:
                 raise ValueError("workspace must be a tensor of workspace()")
             return given
-        key = torch.cuda.current_stream(self.device).cuda_stream
+        index = self.device.index
+        if index is None or torch.cuda.is_current_stream_capturing():
+            return self.workspace(n, q_heads, q_len)
+        key = _lib.raw_stream(index)
         held = self._workspaces.get(key)
         if held is not None and held[1] >= n and held[2] >= q_heads and held[3] >= q_len:
             return held[0]
-        if torch.cuda.is_current_stream_capturing():
-            return self.workspace(n, q_heads, q_len)
         sizes = (n, q_heads, q_len) if held is None else (max(n, held[1]), max(q_heads, held[2]), max(q_len, held[3]))
         made = self.workspace(*sizes)
         self._workspaces[key] = (made, *sizes)
         return made
 
-    def _queries(self, queries: torch.Tensor, seqs: torch.Tensor) -> torch.Tensor:
-        if queries.shape[0] != seqs.shape[0] or queries.shape[-1] != HEAD_DIM:
-            raise ValueError(f"queries must be [{seqs.shape[0]}, ..., query heads, {HEAD_DIM}]")
-        if queries.shape[-2] < 1 or queries.shape[-2] % self.kv_heads:
+    def _queries(self, queries: torch.Tensor, shape, n: int) -> tuple[torch.Tensor, tuple, int]:
+        """Rows that start on 16 bytes, their strides and their type's code."""
+        if shape[0] != n or shape[-1] != HEAD_DIM:
+            raise ValueError(f"queries must be [{n}, ..., query heads, {HEAD_DIM}]")
+        if shape[-2] < 1 or shape[-2] % self.kv_heads:
             raise ValueError("query heads must be a multiple of the cache's KV heads")
-        if queries.dtype not in (torch.float16, torch.bfloat16):
+        dtype = queries.dtype
+        if dtype != torch.bfloat16 and dtype != torch.float16:
             raise RuntimeError("queries must be fp16 or bf16")
         if queries.device != self.device:
             raise RuntimeError("queries must be on the cache's device")
-        if queries.stride(-1) != 1 or queries.data_ptr() % 16 or any(s % 8 for s in queries.stride()[:-1]):
+        strides = queries.stride()
+        if strides[-1] != 1 or queries.data_ptr() % 16 or strides[0] % 8 or strides[1] % 8 or strides[-2] % 8:
             queries = queries.contiguous()
             if queries.data_ptr() % 16:
                 queries = queries.clone()
-        return queries
+            strides = queries.stride()
+        return queries, strides, _lib.DTYPE_CODES[dtype]
 
     def attention(self, queries: torch.Tensor, *, seqs, layer: int = 0, counts=None,
                   softmax_scale: float | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
@@ -260,20 +289,21 @@ class Kv4Cache:
         Returns the same shape and type; rows past ``counts[i]``, and rows that see no token, are
         zeros.  ``softmax_scale`` defaults to 1 / sqrt(128).
         """
-        if queries.ndim not in (3, 4):
+        shape = queries.shape
+        if len(shape) != 4 and len(shape) != 3:
             raise ValueError("queries must be [n, q_len, query heads, 128] or [n, query heads, 128]")
-        seqs = self._sequences(seqs, most=65535)
-        queries = self._queries(queries, seqs)
-        counts = None if counts is None else self._per_sequence(counts, seqs, "counts")
-        out = torch.empty(queries.shape, dtype=queries.dtype, device=self.device)
-        strides = queries.stride()
-        n, q_heads, q_len = seqs.shape[0], queries.shape[-2], queries.shape[1] if queries.ndim == 4 else 1
+        seqs, n = self._sequences(seqs, most=65535)
+        queries, strides, code = self._queries(queries, shape, n)
+        if counts is not None:
+            counts = self._per_sequence(counts, n, "counts")
+        out = torch.empty(shape, dtype=queries.dtype, device=self.device)
+        q_heads = shape[-2]
+        q_len, token_stride = (shape[1], strides[1]) if len(shape) == 4 else (1, 0)
         scratch = self._workspace(workspace, n, q_heads, q_len)
         self._call(_lib.lib().popkv_kv4_attention, self._layer(layer), seqs.data_ptr(), n,
-                   None if counts is None else counts.data_ptr(), queries.data_ptr(),
-                   _lib.DTYPE_CODES[queries.dtype], q_heads, q_len, strides[0],
-                   strides[1] if queries.ndim == 4 else 0, strides[-2], _scale(softmax_scale), scratch.data_ptr(),
-                   scratch.numel(), out.data_ptr())
+                   None if counts is None else counts.data_ptr(), queries.data_ptr(), code, q_heads, q_len,
+                   strides[0], token_stride, strides[-2], _scale(softmax_scale), scratch.data_ptr(),
+                   scratch.shape[0], out.data_ptr())
         return out
 
     def attention_selected(self, queries: torch.Tensor, indices: torch.Tensor, *, seqs, layer: int = 0,
@@ -285,30 +315,32 @@ class Kv4Cache:
         (``popkv_cuda.topk``'s); valid_mask: bool of the same shape.  A slot that is masked, negative
         or past the sequence's end contributes nothing.  Returns [n, q_heads, 128].
         """
-        if queries.ndim != 3:
+        shape, picked = queries.shape, indices.shape
+        if len(shape) != 3:
             raise ValueError("queries must be [n, query heads, 128]")
-        if indices.ndim != 3 or indices.shape[:2] != queries.shape[:2]:
+        if len(picked) != 3 or picked[:2] != shape[:2]:
             raise ValueError("indices must be [n, query heads, selected tokens]")
-        if valid_mask is not None and valid_mask.shape != indices.shape:
-            raise ValueError("valid mask must match indices")
         if indices.dtype != torch.int64:
             raise ValueError("indices must be int64")
-        seqs = self._sequences(seqs, most=65535)
-        queries = self._queries(queries, seqs)
-        if indices.device != self.device or (valid_mask is not None and valid_mask.device != self.device):
+        seqs, n = self._sequences(seqs, most=65535)
+        queries, strides, code = self._queries(queries, shape, n)
+        if indices.device != self.device:
             raise RuntimeError("indices and valid mask must be on the cache's device")
         indices = indices.contiguous()
         if valid_mask is not None:
-            if valid_mask.dtype not in (torch.bool, torch.uint8):
+            if valid_mask.shape != picked:
+                raise ValueError("valid mask must match indices")
+            if valid_mask.dtype != torch.bool and valid_mask.dtype != torch.uint8:
                 raise ValueError("valid mask must be bool or uint8")
+            if valid_mask.device != self.device:
+                raise RuntimeError("indices and valid mask must be on the cache's device")
             valid_mask = valid_mask.contiguous()
-        out = torch.empty(queries.shape, dtype=queries.dtype, device=self.device)
-        strides = queries.stride()
-        scratch = self._workspace(workspace, seqs.shape[0], queries.shape[1], 1)
-        self._call(_lib.lib().popkv_kv4_attention_selected, self._layer(layer), seqs.data_ptr(), seqs.shape[0],
-                   queries.data_ptr(), _lib.DTYPE_CODES[queries.dtype], queries.shape[1], strides[0], strides[1],
-                   indices.data_ptr(), indices.shape[2], None if valid_mask is None else valid_mask.data_ptr(),
-                   _scale(softmax_scale), scratch.data_ptr(), scratch.numel(), out.data_ptr())
+        out = torch.empty(shape, dtype=queries.dtype, device=self.device)
+        scratch = self._workspace(workspace, n, shape[1], 1)
+        self._call(_lib.lib().popkv_kv4_attention_selected, self._layer(layer), seqs.data_ptr(), n,
+                   queries.data_ptr(), code, shape[1], strides[0], strides[1], indices.data_ptr(), picked[2],
+                   None if valid_mask is None else valid_mask.data_ptr(), _scale(softmax_scale), scratch.data_ptr(),
+                   scratch.shape[0], out.data_ptr())
         return out
 
     # -- pages ---------------------------------------------------------------------
@@ -319,16 +351,15 @@ class Kv4Cache:
         sequence is copied first, in every layer.  All or nothing: without enough free pages
         nothing changes and ``check`` raises.
         """
-        seqs = self._sequences(seqs)
+        seqs, n = self._sequences(seqs)
         counts, count = None, 0
         if isinstance(tokens, int):
             count = tokens
             if count < 0:
                 raise ValueError("tokens must not be negative")
         else:
-            counts = self._per_sequence(tokens, seqs, "tokens")
-        n = seqs.shape[0]
-        workspace = torch.empty(self.num_pages + 3 * n, dtype=torch.int32, device=self.device)
+            counts = self._per_sequence(tokens, n, "tokens")
+        workspace = self._scratch(self.num_pages + 3 * n)
         self._call(_lib.lib().popkv_kv4_extend, seqs.data_ptr(), n, None if counts is None else counts.data_ptr(),
                    count, workspace.data_ptr())
 
@@ -338,23 +369,23 @@ class Kv4Cache:
         What a child held before is given back.  Every parent is read before any child changes,
         so one call can reorder beams (children distinct, parents repeated at will).
         """
-        parents, children = self._sequences(parents, "parents"), self._sequences(children, "children")
-        if parents.shape != children.shape:
+        parents, n = self._sequences(parents, "parents")
+        children, m = self._sequences(children, "children")
+        if m != n:
             raise ValueError("parents and children must have the same length")
-        n = parents.shape[0]
-        workspace = torch.empty(n * (1 + self.max_pages), dtype=torch.int32, device=self.device)
+        workspace = self._scratch(n * (1 + self.max_pages))
         self._call(_lib.lib().popkv_kv4_fork, parents.data_ptr(), children.data_ptr(), n, workspace.data_ptr())
 
     def truncate(self, seqs, lengths) -> None:
         """Shorten each listed sequence to ``lengths[i]`` tokens (longer: unchanged)."""
-        seqs = self._sequences(seqs)
-        lengths = self._per_sequence(lengths, seqs, "lengths")
-        self._call(_lib.lib().popkv_kv4_truncate, seqs.data_ptr(), seqs.shape[0], lengths.data_ptr())
+        seqs, n = self._sequences(seqs)
+        lengths = self._per_sequence(lengths, n, "lengths")
+        self._call(_lib.lib().popkv_kv4_truncate, seqs.data_ptr(), n, lengths.data_ptr())
 
     def free(self, seqs) -> None:
         """Give back every page of the listed sequences."""
-        seqs = self._sequences(seqs)
-        self._call(_lib.lib().popkv_kv4_truncate, seqs.data_ptr(), seqs.shape[0], None)
+        seqs, n = self._sequences(seqs)
+        self._call(_lib.lib().popkv_kv4_truncate, seqs.data_ptr(), n, None)
 
     def compact(self) -> None:
         """Move the live pages to the front of the pool (``status[1]`` then counts them).
@@ -362,7 +393,7 @@ class Kv4Cache:
         Live pages past the number of live pages move, in order, to the free pages below it, in
         order; the tables follow.  The tail of the pool is then free.
         """
-        workspace = torch.empty(3 * self.num_pages, dtype=torch.int32, device=self.device)
+        workspace = self._scratch(3 * self.num_pages)
         self._call(_lib.lib().popkv_kv4_compact, workspace.data_ptr())
 
     def copy_pages(self, sources, targets) -> None:
@@ -387,10 +418,6 @@ class Kv4Cache:
     def free_pages(self) -> int:
         """Free pages of the pool (synchronises)."""
         return int((self.refs == 0).sum().item())
-
-
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    return x if x.stride(-1) == 1 else x.contiguous()
 
 
 def _scale(softmax_scale: float | None) -> float:

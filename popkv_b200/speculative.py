@@ -19,8 +19,8 @@ _workspaces: dict[tuple[int, int], torch.Tensor] = {}  # of each (device, stream
 def verify_workspace(n: int, device) -> torch.Tensor:
     """Scratch for ``verify_drafts`` calls of up to ``n`` sequences, zeroed.
 
-    Without one, calls keep one per stream; inside a graph capture, where that cannot be, each call
-    would allocate and clear its own.  Calls that overlap in time need one each.
+    Without one, calls keep one per stream; inside a graph capture each call would make and clear its
+    own.  Calls that overlap in time need one each.
     """
     return torch.zeros(12 * n, dtype=torch.uint8, device=device)
 
@@ -30,13 +30,12 @@ def _workspace(given, n: int, device, stream: int) -> torch.Tensor:
         if given.dtype != torch.uint8 or not given.is_contiguous() or given.device != device or given.numel() < 12 * n:
             raise ValueError(f"workspace must be a tensor of verify_workspace({n}, ...)")
         return given
+    if torch.cuda.is_current_stream_capturing():
+        return verify_workspace(n, device)
     held = _workspaces.get((device.index, stream))
-    if held is not None and held.numel() >= 12 * n:
-        return held
-    made = verify_workspace(n, device)
-    if not torch.cuda.is_current_stream_capturing():
-        _workspaces[device.index, stream] = made
-    return made
+    if held is None or held.shape[0] < 12 * n:
+        held = _workspaces[device.index, stream] = verify_workspace(n, device)
+    return held
 
 
 def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, uniforms: torch.Tensor,
@@ -110,7 +109,7 @@ def _verify(target_probs, draft_tokens, uniforms, noise, draft_probs, counts, wo
     counts = None if counts is None else counts.contiguous()
     tokens = torch.empty((n, places), dtype=torch.int64, device=device)
     accepted = torch.empty(n, dtype=torch.int32, device=device)
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = _lib.raw_stream(device.index)
     scratch = _workspace(workspace, n, device, stream)
     t_seq, t_place, _ = target_probs.stride()
     status = _lib.lib().popkv_verify_drafts(
