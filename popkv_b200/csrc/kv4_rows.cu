@@ -35,6 +35,7 @@ int kv4_view(const char* what, const popkv_kv4_cache* cache, Kv4View* view) {
     view->head_bytes = p / kKv4TileTokens * view->tile_bytes();
     view->page_bytes = view->kv_heads * view->head_bytes;
     view->layer_bytes = view->num_pages * view->page_bytes;
+    if (view->page_bytes > 0x7FFFFFFF) return fail(POPKV_ERR_INVALID, "%s: a page is too large", what);
     return POPKV_OK;
 }
 
@@ -42,7 +43,7 @@ namespace {
 
 constexpr float kHalfMost = 65504.0f;
 constexpr int kRowsThreads = 256;
-constexpr int kMostBlocks = 148 * 8;
+constexpr int kMostBlocks = 148 * 4;  // resident at once
 
 // A warp handles the key and the value row of one (sequence, token, head) at a time: lane l
 // of each half holds dims 8l..8l+7, which are natural word l of the row's 4-bit numbers.
@@ -95,198 +96,265 @@ __device__ __forceinline__ uint32_t group_pair(float least, float most, float& l
     low = half_bits_to_float(low_bits);
     const uint16_t delta_bits = float_to_half_bits(fmaxf(__fdiv_rn(__fsub_rn(most, low), 15.0f), 0.0f));
     const float delta = half_bits_to_float(delta_bits);
-    scale = delta > 0.0f ? __fdiv_rn(1.0f, delta) : 0.0f;
+    scale = delta > 0.0f ? __frcp_rn(delta) : 0.0f;
     return low_bits | static_cast<uint32_t>(delta_bits) << 16;
 }
 
-// Value rows are the 8 x 8 transposition of their 64 natural bytes.  Lane s of the half warp
-// gets stored word s (rows 2g, 2g + 1 of it: bytes 4 (s & 1) + k of column s >> 1) from the
-// lanes' natural words; the same exchange the other way.
-__device__ __forceinline__ uint32_t stored_value_word(uint32_t natural, int lane) {
-    const int s = lane & 15, g = s >> 1, half = lane & 16;
-    uint32_t word = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int i = 4 * (s & 1) + k;  // natural byte 8 i + g
-        const uint32_t from = __shfl_sync(0xFFFFFFFFu, natural, half | (2 * i + (g >> 2)));
-        word |= (from >> (8 * (g & 3)) & 0xFFu) << (8 * k);
-    }
-    return word;
-}
+// Value rows are the 8 x 8 transposition of their 64 natural bytes.  Each word of either order
+// takes one byte, the same one, of four words of the other: byte `pick` of lanes first, first +
+// step, ... of the half warp.
+struct Exchange {
+    int first, step;
+    uint32_t pick;  // of two words at a time, as a byte permutation's selector
 
-__device__ __forceinline__ uint32_t natural_value_word(uint32_t stored, int lane) {
-    const int l = lane & 15, half = lane & 16;
-    uint32_t word = 0;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const int g = 4 * (l & 1) + k;  // natural byte 4 l + k is byte l >> 1 of column g
-        const uint32_t from = __shfl_sync(0xFFFFFFFFu, stored, half | (2 * g + (l >> 3)));
-        word |= (from >> (8 * (l >> 1 & 3)) & 0xFFu) << (8 * k);
+    // Lane s gets stored word s: natural bytes 8 i + s / 2, i = 4 (s % 2) + 0..3.
+    __device__ static Exchange to_stored(int lane) {
+        const int s = lane & 15, g = s >> 1;
+        return {(lane & 16) | (8 * (s & 1) + (g >> 2)), 2, (g & 3) * 0x11u + 0x40u};
     }
-    return word;
+    // Lane l gets natural word l: bytes l / 2 of the stored columns 4 (l % 2) + 0..3.
+    __device__ static Exchange to_natural(int lane) {
+        const int l = lane & 15;
+        return {(lane & 16) | (8 * (l & 1) + (l >> 3)), 2, (l >> 1 & 3) * 0x11u + 0x40u};
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t word) const {
+        const uint32_t a = __shfl_sync(0xFFFFFFFFu, word, first), b = __shfl_sync(0xFFFFFFFFu, word, first + step);
+        const uint32_t c = __shfl_sync(0xFFFFFFFFu, word, first + 2 * step);
+        const uint32_t d = __shfl_sync(0xFFFFFFFFu, word, first + 3 * step);
+        return __byte_perm(__byte_perm(a, b, pick), __byte_perm(c, d, pick), 0x5410u);
+    }
+};
+
+// The larger (smaller) of two, NaN if either is.
+__device__ __forceinline__ float larger_or_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float smaller_or_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
 // Key rows store natural word w at word (w % 4) * 4 + w / 4, its own inverse.
 __device__ __forceinline__ int key_slot(int word) { return (word & 3) * 4 + (word >> 2); }
 
+// a * b in 64 bits, one instruction.
+__device__ __forceinline__ uint64_t wide(int a, uint32_t b) {
+    return static_cast<uint64_t>(static_cast<uint32_t>(a)) * b;
+}
+
+// The warps of a block over heads and tokens: `heads` neighbouring warps (a power of two, at
+// most 8) take a token's heads, the others further tokens; blockIdx.y walks the entries.  No
+// division finds a row's place.
+struct Rows {
+    int head, head_step, token, token_step;
+};
+
+__device__ __forceinline__ Rows rows_of(int head_shift) {
+    const int warp = threadIdx.x >> 5;
+    const int tokens_per_block = (kRowsThreads / 32) >> head_shift;
+    Rows rows;
+    rows.head = warp & ((1 << head_shift) - 1);
+    rows.head_step = 1 << head_shift;
+    rows.token = blockIdx.x * tokens_per_block + (warp >> head_shift);
+    rows.token_step = gridDim.x * tokens_per_block;
+    return rows;
+}
+
 // Two rows of a warp at a time, so that one row's loads fly while the other is quantised.
-// What bounds it is issue: about 130 instructions a lane for 16 bytes read (two divisions
-// a group among them) at 44 + 10 MB for 8191 tokens of 8 heads in bf16.
 template <typename T, bool kVector>
-__global__ void __launch_bounds__(kRowsThreads) write_kernel(
-    Kv4View view, int layer, const int32_t* __restrict__ seqs, const int32_t* __restrict__ counts, int64_t rows,
-    int tokens, const T* __restrict__ keys, const T* __restrict__ values, int64_t k_seq, int64_t k_token,
+__global__ void __launch_bounds__(kRowsThreads, 4) write_kernel(
+    Kv4View view, int layer, int head_shift, const int32_t* __restrict__ seqs, const int32_t* __restrict__ counts,
+    int n, int tokens, const T* __restrict__ keys, const T* __restrict__ values, int64_t k_seq, int64_t k_token,
     int64_t k_head, int64_t v_seq, int64_t v_token, int64_t v_head) {
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31, l = lane & 15;
     const bool is_value = lane >= 16;
-    const int64_t warps = static_cast<int64_t>(gridDim.x) * (kRowsThreads / 32);
-    const int64_t warp = (blockIdx.x * static_cast<int64_t>(kRowsThreads) + threadIdx.x) >> 5;
+    const T* rows_at = (is_value ? values : keys) + 8 * l;
+    const int64_t seq_stride = is_value ? v_seq : k_seq, token_stride = is_value ? v_token : k_token,
+                  head_stride = is_value ? v_head : k_head;
+    const int lanes = 16 / view.groups;  // of a group
+    const Exchange exchange = Exchange::to_stored(lane);
+    const int line_offset = is_value ? kKv4ValueOffset + 4 * l : 4 * key_slot(l);
+    const int pair_offset = kKv4PairOffset + ((is_value ? view.groups : 0) + l / lanes) * 4;
+    const Rows rows = rows_of(head_shift);
+    uint8_t* base = view.pages + layer * view.layer_bytes;
+    const int page_mask = view.page_size() - 1, tile_bytes = view.tile_bytes();
+    const uint32_t page_bytes = static_cast<uint32_t>(view.page_bytes);
     constexpr int kTogether = 2;
-    for (int64_t first = warp; first < rows; first += warps * kTogether) {
-        uint8_t* tiles[kTogether];
-        int at[kTogether];
-        float x[kTogether][8];
+#pragma unroll 1
+    for (int entry = blockIdx.y; entry < n; entry += gridDim.y) {
+        const int seq = seqs[entry];
+        const int count = counts ? min(counts[entry], tokens) : tokens;
+        const int length = view.length_of(seq), offset = length - count;
+        if (length == 0) continue;  // an id out of range among them
+        const int32_t* pages_of_seq = view.table + static_cast<int64_t>(seq) * view.max_pages;
+        const T* rows_of_entry = rows_at + entry * seq_stride;
+#pragma unroll 1
+        for (int head = rows.head; head < view.kv_heads; head += rows.head_step) {
+            uint8_t* head_base = base + head * view.head_bytes;
+            const T* head_rows = rows_of_entry + head * head_stride;
+#pragma unroll 1
+            for (int first = rows.token; first < count; first += rows.token_step * kTogether) {
+                uint8_t* tiles[kTogether];
+                int at[kTogether];
+                float x[kTogether][8];
 #pragma unroll
-        for (int u = 0; u < kTogether; ++u) {
-            const int64_t row = first + u * warps;
-            tiles[u] = nullptr;
-            at[u] = 0;
+                for (int u = 0; u < kTogether; ++u) {
+                    const int token = first + u * rows.token_step, position = offset + token;
+                    tiles[u] = nullptr;
+                    at[u] = position & 15;
+                    if (token >= count || position < 0) continue;
+                    const int page = pages_of_seq[position >> view.page_shift];
+                    if (page < 0 || page >= view.num_pages) continue;
+                    tiles[u] = head_base + wide(page, page_bytes) + ((position & page_mask) >> 4) * tile_bytes;
+                    load_eight<T, kVector>(head_rows + token * token_stride, x[u]);
+                }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[u][i] = 0.0f;
-            if (row >= rows) continue;
-            const int64_t of_token = row / view.kv_heads;
-            const int head = static_cast<int>(row - of_token * view.kv_heads);
-            const int entry = static_cast<int>(of_token / tokens), token = static_cast<int>(of_token - static_cast<int64_t>(entry) * tokens);
-            const int seq = seqs[entry];
-            const int count = counts ? min(counts[entry], tokens) : tokens;
-            const int length = view.length_of(seq);
-            const int position = length - count + token;
-            if (token >= count || position < 0 || position >= length) continue;
-            const int page = view.page_at(seq, position);
-            if (page < 0) continue;
-            tiles[u] = view.tile_at(layer, page, head, position);
-            at[u] = position & 15;
-            load_eight<T, kVector>((is_value ? values + entry * v_seq + token * v_token + head * v_head
-                                             : keys + entry * k_seq + token * k_token + head * k_head) + 8 * l, x[u]);
-        }
+                for (int u = 0; u < kTogether; ++u) {
+                    if (!tiles[u]) continue;  // the whole warp
+                    float least = x[u][0], most = x[u][0];
 #pragma unroll
-        for (int u = 0; u < kTogether; ++u) {
-            if (!tiles[u]) continue;  // the whole warp
-            float least = x[u][0], most = x[u][0];
-            bool odd = false;
+                    for (int i = 1; i < 8; ++i) {
+                        least = smaller_or_nan(least, x[u][i]);
+                        most = larger_or_nan(most, x[u][i]);
+                    }
+                    if (__any_sync(0xFFFFFFFFu, !(least >= -kHalfMost && most <= kHalfMost))) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) odd |= !(fabsf(x[u][i]) <= kHalfMost);
-            if (__any_sync(0xFFFFFFFFu, odd)) {
+                        for (int i = 0; i < 8; ++i) {
+                            x[u][i] = storable(x[u][i]);
+                            least = i ? fminf(least, x[u][i]) : x[u][i];
+                            most = i ? fmaxf(most, x[u][i]) : x[u][i];
+                        }
+                    }
+                    for (int step = 1; step < lanes; step *= 2) {
+                        least = fminf(least, __shfl_xor_sync(0xFFFFFFFFu, least, step));
+                        most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, step));
+                    }
+                    float low, scale;
+                    const uint32_t pair = group_pair(least, most, low, scale);
+                    // rint of a number in 0..15: the low bits of 1.5 * 2^23 + it.  The eight are summed in
+                    // their places, and what the constants add up to (modulo 2^32) is taken off.
+                    uint32_t word = 0;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[u][i] = storable(x[u][i]);
-                least = most = x[u][0];
+                    for (int i = 0; i < 8; ++i) {
+                        const float number = fminf(fmaxf(__fmul_rn(__fsub_rn(x[u][i], low), scale), 0.0f), 15.0f);
+                        word += __float_as_uint(__fadd_rn(number, 12582912.0f)) << (4 * i);
+                    }
+                    word -= 0x4B400000u + 0xB4000000u + 0x40000000u;
+                    const uint32_t value_word = exchange(word);
+                    *reinterpret_cast<uint32_t*>(tiles[u] + at[u] * kKv4RowBytes + line_offset) =
+                        is_value ? value_word : word;
+                    if ((l & (lanes - 1)) == 0)
+                        *reinterpret_cast<uint32_t*>(tiles[u] + at[u] * view.pair_bytes() + pair_offset) = pair;
+                }
             }
-#pragma unroll
-            for (int i = 1; i < 8; ++i) {
-                least = fminf(least, x[u][i]);
-                most = fmaxf(most, x[u][i]);
-            }
-            const int lanes = 16 / view.groups;  // of a group
-            for (int step = 1; step < lanes; step *= 2) {
-                least = fminf(least, __shfl_xor_sync(0xFFFFFFFFu, least, step));
-                most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, step));
-            }
-            float low, scale;
-            const uint32_t pair = group_pair(least, most, low, scale);
-            // rint of a number in 0..15: the low bits of 1.5 * 2^23 + it.  The eight are summed in
-            // their places, and what the constants add up to (modulo 2^32) is taken off.
-            uint32_t word = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float n = fminf(fmaxf(__fmul_rn(__fsub_rn(x[u][i], low), scale), 0.0f), 15.0f);
-                word += __float_as_uint(__fadd_rn(n, 12582912.0f)) << (4 * i);
-            }
-            word -= 0x4B400000u + 0xB4000000u + 0x40000000u;
-            const uint32_t value_word = stored_value_word(word, lane);
-            uint8_t* line = tiles[u] + at[u] * kKv4RowBytes + (is_value ? kKv4ValueOffset : 0);
-            reinterpret_cast<uint32_t*>(line)[is_value ? l : key_slot(l)] = is_value ? value_word : word;
-            if (l % lanes == 0)
-                *reinterpret_cast<uint32_t*>(tiles[u] + kKv4PairOffset + at[u] * view.pair_bytes() +
-                                             ((is_value ? view.groups : 0) + l / lanes) * 4) = pair;
         }
     }
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kRowsThreads) read_kernel(Kv4View view, int layer,
-                                                            const int32_t* __restrict__ seqs, int64_t rows,
-                                                            int64_t start, int tokens, T* __restrict__ keys,
-                                                            T* __restrict__ values) {
+__global__ void __launch_bounds__(kRowsThreads, 4) read_kernel(Kv4View view, int layer, int head_shift,
+                                                            const int32_t* __restrict__ seqs, int n, int64_t start,
+                                                            int tokens, T* __restrict__ keys, T* __restrict__ values) {
     pdl_wait();
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31, l = lane & 15;
     const bool is_value = lane >= 16;
-    const int64_t warps = static_cast<int64_t>(gridDim.x) * (kRowsThreads / 32);
-    const int64_t warp = (blockIdx.x * static_cast<int64_t>(kRowsThreads) + threadIdx.x) >> 5;
-    T* out = is_value ? values : keys;
+    T* out = (is_value ? values : keys) + 8 * l;
+    const Exchange exchange = Exchange::to_natural(lane);
+    const int line_offset = is_value ? kKv4ValueOffset + 4 * l : 4 * key_slot(l);
+    const int pair_offset = kKv4PairOffset + ((is_value ? view.groups : 0) + l * view.groups / 16) * 4;
+    const Rows rows = rows_of(head_shift);
+    uint8_t* base = view.pages + layer * view.layer_bytes;
+    const int page_mask = view.page_size() - 1, tile_bytes = view.tile_bytes();
+    const uint32_t page_bytes = static_cast<uint32_t>(view.page_bytes);
     constexpr int kTogether = 4;  // a row is only 64 bytes to read: several in flight
-    for (int64_t first = warp; first < rows; first += warps * kTogether) {
-        uint32_t words[kTogether], pairs[kTogether];
+#pragma unroll 1
+    for (int entry = blockIdx.y; entry < n; entry += gridDim.y) {
+        const int seq = seqs[entry];
+        const int length = view.length_of(seq);
+        const int32_t* pages_of_seq = view.table + static_cast<int64_t>(length ? seq : 0) * view.max_pages;
+#pragma unroll 1
+        for (int head = rows.head; head < view.kv_heads; head += rows.head_step) {
+            const uint8_t* head_base = base + head * view.head_bytes;
+            T* head_out = out + (static_cast<int64_t>(entry) * tokens * view.kv_heads + head) * kKv4Dim;
+            const uint32_t token_size = static_cast<uint32_t>(view.kv_heads) * kKv4Dim;
+#pragma unroll 1
+            for (int first = rows.token; first < tokens; first += rows.token_step * kTogether) {
+                uint32_t words[kTogether], pairs[kTogether];
 #pragma unroll
-        for (int u = 0; u < kTogether; ++u) {
-            const int64_t row = first + u * warps;
-            words[u] = pairs[u] = 0;  // low = delta = 0: zeros
-            if (row >= rows) continue;
-            const int64_t of_token = row / view.kv_heads;
-            const int head = static_cast<int>(row - of_token * view.kv_heads);
-            const int entry = static_cast<int>(of_token / tokens);
-            const int64_t position = start + (of_token - static_cast<int64_t>(entry) * tokens);
-            const int seq = seqs[entry];
-            const int page = position < view.length_of(seq) ? view.page_at(seq, static_cast<int>(position)) : -1;
-            if (page < 0) continue;
-            const uint8_t* tile = view.tile_at(layer, page, head, static_cast<int>(position));
-            const int at = static_cast<int>(position) & 15;
-            const uint8_t* line = tile + at * kKv4RowBytes + (is_value ? kKv4ValueOffset : 0);
-            words[u] = reinterpret_cast<const uint32_t*>(line)[is_value ? l : key_slot(l)];
-            pairs[u] = *reinterpret_cast<const uint32_t*>(tile + kKv4PairOffset + at * view.pair_bytes() +
-                                                          ((is_value ? view.groups : 0) + l * view.groups / 16) * 4);
-        }
+                for (int u = 0; u < kTogether; ++u) {
+                    const int token = first + u * rows.token_step;
+                    words[u] = pairs[u] = 0;  // low = delta = 0: zeros
+                    if (token >= tokens || start + token >= length) continue;
+                    const int position = static_cast<int>(start) + token, at = position & 15;
+                    const int page = pages_of_seq[position >> view.page_shift];
+                    if (page < 0 || page >= view.num_pages) continue;
+                    const uint8_t* tile = head_base + wide(page, page_bytes) + ((position & page_mask) >> 4) * tile_bytes;
+                    words[u] = *reinterpret_cast<const uint32_t*>(tile + at * kKv4RowBytes + line_offset);
+                    pairs[u] = *reinterpret_cast<const uint32_t*>(tile + at * view.pair_bytes() + pair_offset);
+                }
 #pragma unroll
-        for (int u = 0; u < kTogether; ++u) {
-            const int64_t row = first + u * warps;
-            const uint32_t value_word = natural_value_word(words[u], lane);
-            if (row >= rows) continue;
-            const uint32_t word = is_value ? value_word : words[u];
-            const float low = half_bits_to_float(static_cast<uint16_t>(pairs[u]));
-            const float delta = half_bits_to_float(static_cast<uint16_t>(pairs[u] >> 16));
-            float x[8];
+                for (int u = 0; u < kTogether; ++u) {
+                    const int token = first + u * rows.token_step;
+                    if (token >= tokens) continue;  // the whole warp
+                    const uint32_t value_word = exchange(words[u]);
+                    const uint32_t word = is_value ? value_word : words[u];
+                    const float low = half_bits_to_float(static_cast<uint16_t>(pairs[u]));
+                    const float delta = half_bits_to_float(static_cast<uint16_t>(pairs[u] >> 16));
+                    float x[8];
+                    // n as the low byte of 2^23 + n.  n * delta has 15 bits, so one rounding as two.
+                    const uint32_t even = word & 0x0F0F0F0Fu, odd = word >> 4 & 0x0F0F0F0Fu;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                x[i] = __fadd_rn(low, __fmul_rn(small_int_to_float(static_cast<int>(word >> (4 * i) & 15u)), delta));
-            store_eight(out + row * kKv4Dim + 8 * l, x);
+                    for (int i = 0; i < 8; ++i) {
+                        const uint32_t bits = __byte_perm(i & 1 ? odd : even, 0x4B000000u, 0x7650u + (i >> 1));
+                        x[i] = __fmaf_rn(__fsub_rn(__uint_as_float(bits), 8388608.0f), delta, low);
+                    }
+                    store_eight(head_out + wide(token, token_size), x);
+                }
+            }
         }
     }
 }
 
-unsigned blocks_of(int64_t rows, int together) {
-    const int64_t warps = (rows + together - 1) / together, blocks = (warps + kRowsThreads / 32 - 1) / (kRowsThreads / 32);
-    return static_cast<unsigned>(blocks < kMostBlocks ? blocks : kMostBlocks);
+// Blocks for `tokens` tokens of n entries, `together` tokens a warp where there are plenty.
+dim3 row_grid(const Kv4View& view, int64_t n, int64_t tokens, int head_shift) {
+    const int64_t per_block = (kRowsThreads / 32) >> head_shift;
+    const int64_t blocks = (tokens + per_block - 1) / per_block;
+    const int64_t y = n < 65535 ? n : 65535, most = kMostBlocks / y > 0 ? kMostBlocks / y : 1;
+    return dim3(static_cast<unsigned>(blocks < most ? blocks : most), static_cast<unsigned>(y));
+}
+
+int head_shift_of(const Kv4View& view) {
+    int shift = 0;
+    while (shift < 3 && (1 << shift) < view.kv_heads) ++shift;
+    return shift;
 }
 
 template <typename T>
-cudaError_t launch_write(const Kv4View& view, int layer, const int32_t* seqs, const int32_t* counts, int64_t rows,
+cudaError_t launch_write(const Kv4View& view, int layer, const int32_t* seqs, int64_t n, const int32_t* counts,
                          int64_t tokens, const void* keys, const void* values, const int64_t* s, cudaStream_t stream) {
     // Rows in 16-byte loads where every row begins on one, else element by element.
     bool vector = aligned(keys, 16) && aligned(values, 16);
     for (int i = 0; i < 6; ++i) vector = vector && s[i] % (16 / static_cast<int64_t>(sizeof(T))) == 0;
-    // Few rows: a warp each, for the latency; many: two at a time.
-    return launch_pdl(vector ? write_kernel<T, true> : write_kernel<T, false>, dim3(blocks_of(rows, 1)),
-                      dim3(kRowsThreads), 0, stream, 1, view, layer, seqs, counts, rows, static_cast<int>(tokens),
-                      static_cast<const T*>(keys), static_cast<const T*>(values), s[0], s[1], s[2], s[3], s[4], s[5]);
+    const int shift = head_shift_of(view);
+    return launch_pdl(vector ? write_kernel<T, true> : write_kernel<T, false>, row_grid(view, n, tokens, shift),
+                      dim3(kRowsThreads), 0, stream, 1, view, layer, shift, seqs, counts, static_cast<int>(n),
+                      static_cast<int>(tokens), static_cast<const T*>(keys), static_cast<const T*>(values), s[0], s[1],
+                      s[2], s[3], s[4], s[5]);
 }
 
 template <typename T>
-cudaError_t launch_read(const Kv4View& view, int layer, const int32_t* seqs, int64_t rows, int64_t start,
-                        int64_t tokens, void* keys, void* values, cudaStream_t stream) {
-    return launch_pdl(read_kernel<T>, dim3(blocks_of(rows, 1)), dim3(kRowsThreads), 0, stream, 1, view, layer, seqs,
-                      rows, start, static_cast<int>(tokens), static_cast<T*>(keys), static_cast<T*>(values));
+cudaError_t launch_read(const Kv4View& view, int layer, const int32_t* seqs, int64_t n, int64_t start, int64_t tokens,
+                        void* keys, void* values, cudaStream_t stream) {
+    const int shift = head_shift_of(view);
+    return launch_pdl(read_kernel<T>, row_grid(view, n, tokens, shift), dim3(kRowsThreads), 0, stream, 1, view, layer,
+                      shift, seqs, static_cast<int>(n), start, static_cast<int>(tokens), static_cast<T*>(keys),
+                      static_cast<T*>(values));
 }
 
 constexpr int64_t kMostRows = int64_t{1} << 33;  // 2^31 - 1 blocks of 8 warps is far above
@@ -309,13 +377,12 @@ extern "C" int popkv_kv4_write(const popkv_kv4_cache* cache, int64_t layer, cons
     if (!seqs || !keys || !values) return fail(POPKV_ERR_INVALID, "popkv_kv4_write: null pointer");
     const int64_t strides[6] = {k_seq_stride, k_token_stride, k_head_stride,
                                 v_seq_stride, v_token_stride, v_head_stride};
-    const int64_t rows = n * tokens * view.kv_heads;
     const auto s = static_cast<cudaStream_t>(stream);
     const int at = static_cast<int>(layer);
     auto launch = dtype == POPKV_DTYPE_F32   ? launch_write<float>
                   : dtype == POPKV_DTYPE_F16 ? launch_write<__half>
                                              : launch_write<__nv_bfloat16>;
-    const cudaError_t err = launch(view, at, seqs, counts, rows, tokens, keys, values, strides, s);
+    const cudaError_t err = launch(view, at, seqs, n, counts, tokens, keys, values, strides, s);
     if (err != cudaSuccess) return fail(POPKV_ERR_CUDA, "popkv_kv4_write: %s", cudaGetErrorString(err));
     return check_launch("popkv_kv4_write");
 }
@@ -334,13 +401,12 @@ extern "C" int popkv_kv4_read(const popkv_kv4_cache* cache, int64_t layer, const
     if (!seqs || !keys || !values) return fail(POPKV_ERR_INVALID, "popkv_kv4_read: null pointer");
     if (!aligned(keys, 16) || !aligned(values, 16))
         return fail(POPKV_ERR_INVALID, "popkv_kv4_read: outputs must be 16-byte aligned");
-    const int64_t rows = n * tokens * view.kv_heads;
     const auto s = static_cast<cudaStream_t>(stream);
     const int at = static_cast<int>(layer);
     auto launch = dtype == POPKV_DTYPE_F32   ? launch_read<float>
                   : dtype == POPKV_DTYPE_F16 ? launch_read<__half>
                                              : launch_read<__nv_bfloat16>;
-    const cudaError_t err = launch(view, at, seqs, rows, start, tokens, keys, values, s);
+    const cudaError_t err = launch(view, at, seqs, n, start, tokens, keys, values, s);
     if (err != cudaSuccess) return fail(POPKV_ERR_CUDA, "popkv_kv4_read: %s", cudaGetErrorString(err));
     return check_launch("popkv_kv4_read");
 }
