@@ -1,0 +1,136 @@
+"""Sampling decode from the 4-bit cache: branches, drafts, retrieval and page moves end to end."""
+from __future__ import annotations
+
+from dataclasses import replace
+
+import pytest
+import torch
+
+from popkv_b200.decoder import LlamaConfig, LlamaWeights
+from popkv_b200.kv4_decode import Kv4Decoder, main
+from popkv_b200.popkv import RetrievalConfig
+
+pytestmark = pytest.mark.gpu
+
+CONFIG = LlamaConfig(hidden_size=256, num_attention_heads=4, num_key_value_heads=2, intermediate_size=512,
+                     vocab_size=503, num_hidden_layers=3)
+
+
+@pytest.fixture(scope="module")
+def weights(cuda_device):
+    return LlamaWeights.random(CONFIG, device=cuda_device, std=0.06, seed=3)
+
+
+def prompt(tokens, seed=0):
+    return torch.randint(0, CONFIG.vocab_size, (tokens,), generator=torch.Generator().manual_seed(seed))
+
+
+def near(a, b):
+    """Logits of the same tokens by another route: the routes differ by bf16 roundings (2^-8 of a value) in 3
+    layers and the head, each of which moves a logit by at most a few of its own; 12 of them of the spread."""
+    return float((a - b).abs().max()) <= 12 * 2.0 ** -8 * float(b.std() + b.abs().max())
+
+
+def test_several_tokens_in_one_pass_are_the_single_steps(weights, cuda_device):
+    one, many = (Kv4Decoder(weights, max_seqs=2, max_tokens=200, page_size=16) for _ in range(2))
+    slots = torch.tensor([1, 0], dtype=torch.int32, device=cuda_device)
+    for d in (one, many):
+        d.prefill(0, prompt(37))
+        d.prefill(1, prompt(70, 1))
+    tokens = torch.randint(0, 503, (2, 5), generator=torch.Generator().manual_seed(2)).to(cuda_device)
+    steps = torch.stack([one.forward(slots, tokens[:, i:i + 1])[:, 0] for i in range(5)], 1)
+    assert near(many.forward(slots, tokens), steps)
+    assert torch.equal(one.cache.tables, many.cache.tables) and one.cache.lengths.tolist() == [42, 75]
+
+
+def test_prefill_and_steps_agree(weights, cuda_device):
+    """The last prompt token through the cache: only the 4-bit rounding of keys and values differs."""
+    a, b = (Kv4Decoder(weights, max_seqs=1, max_tokens=200) for _ in range(2))
+    whole = a.prefill(0, prompt(90))
+    b.prefill(0, prompt(90)[:-1])
+    step = b.forward(torch.zeros(1, dtype=torch.int32, device=cuda_device), prompt(90)[-1:][None].to(cuda_device))
+    cosine = torch.nn.functional.cosine_similarity(whole, step[0, 0], dim=0)
+    assert float(cosine) > 0.97
+
+
+def test_branches_share_pages_and_go_their_own_ways(weights, cuda_device):
+    d = Kv4Decoder(weights, max_seqs=4, max_tokens=120, page_size=16)
+    d.prefill(0, prompt(40))
+    used = d.cache.num_pages - d.cache.free_pages()
+    d.fork(0, [1, 2, 3])
+    assert d.cache.num_pages - d.cache.free_pages() == used == 3
+    slots = torch.arange(4, dtype=torch.int32, device=cuda_device)
+    same = d.forward(slots, torch.full((4, 1), 7, device=cuda_device))
+    assert all(torch.equal(same[0], same[i]) for i in range(1, 4))
+    # All four wrote into their copies of the third page; the shared one is free again.
+    assert d.cache.num_pages - d.cache.free_pages() == 2 + 4
+    alone = Kv4Decoder(weights, max_seqs=1, max_tokens=120, page_size=16)
+    alone.prefill(0, prompt(40))
+    alone.forward(slots[:1], torch.full((1, 1), 7, device=cuda_device))
+    tokens = torch.tensor([[1], [2], [3], [4]], device=cuda_device)
+    assert near(d.forward(slots, tokens)[2], alone.forward(slots[:1], tokens[2:3])[0])
+    d.release([0, 1])
+    d.cache.check()
+    assert d.cache.status[1].item() == 2 + 2
+    assert near(d.forward(slots[2:3], tokens[:1]), alone.forward(slots[:1], tokens[:1]))
+
+
+def test_drafts_of_the_model_itself_are_kept(weights):
+    target, draft = (Kv4Decoder(weights, max_seqs=3, max_tokens=300, seed=s) for s in (0, 1))
+    for d in (target, draft):
+        d.prefill(0, prompt(50))
+        d.fork(0, [1, 2])
+    first, _ = target.sample(target.prefill(0, prompt(50)).expand(3, -1))
+    draft.prefill(0, prompt(50))
+    tokens, gain = target.generate([0, 1, 2], first, 40, draft=draft, drafts=3)
+    assert all(len(t) >= 40 for t in tokens) and all(0 <= x < 503 for t in tokens for x in t)
+    assert gain > 3.5  # of 4: the two differ by roundings alone
+    # Both caches hold what was kept, but for the last token of each slot.
+    held = target.cache.lengths.tolist()
+    assert held == draft.cache.lengths.tolist() == [50 + len(t) - 1 for t in tokens]
+
+
+def test_drafts_of_a_smaller_model(weights):
+    small = LlamaWeights(replace(CONFIG, num_hidden_layers=1), weights.embed, weights.layers[:1], weights.norm,
+                         weights.lm_head)
+    target, draft = Kv4Decoder(weights, max_seqs=2, max_tokens=200), Kv4Decoder(small, max_seqs=2, max_tokens=200)
+    logits = torch.stack([target.prefill(s, prompt(20 + s, s)) for s in range(2)])
+    for s in range(2):
+        draft.prefill(s, prompt(20 + s, s))
+    first, _ = target.sample(logits)
+    tokens, gain = target.generate([0, 1], first, 20, draft=draft, drafts=2)
+    assert 1.0 <= gain <= 3.0
+    assert target.cache.lengths.tolist() == [20 + s + len(t) - 1 for s, t in enumerate(tokens)]
+
+
+def test_retrieval_with_a_full_budget_is_the_dense_attention(weights, cuda_device):
+    dense = Kv4Decoder(weights, max_seqs=2, max_tokens=200)
+    sparse = Kv4Decoder(weights, max_seqs=2, max_tokens=200, retrieval=RetrievalConfig(budget=500, full_layers=(0,)))
+    few = Kv4Decoder(weights, max_seqs=2, max_tokens=200, retrieval=RetrievalConfig(budget=24, full_layers=(0,)))
+    for d in (dense, sparse, few):
+        d.prefill(0, prompt(80))
+        d.fork(0, [1])
+    slots = torch.arange(2, dtype=torch.int32, device=cuda_device)
+    for i in range(4):
+        token = torch.full((2, 1), 11 * i + 1, device=cuda_device)
+        want = dense.forward(slots, token)
+        assert near(sparse.forward(slots, token), want)
+        got = few.forward(slots, token)
+        assert torch.isfinite(got).all() and not torch.equal(got, want)
+    with pytest.raises(ValueError, match="drafted tokens need dense"):
+        sparse.generate([0], torch.zeros(1, dtype=torch.int64), 3, draft=dense)
+    tokens, gain = few.generate([0, 1], torch.tensor([1, 2]), 6)
+    assert gain == 1.0 and [len(t) for t in tokens] == [6, 6]
+
+
+def test_a_full_pool_is_reported(weights):
+    d = Kv4Decoder(weights, max_seqs=2, max_tokens=64, num_pages=3, page_size=16)
+    d.prefill(0, prompt(40))
+    with pytest.raises(RuntimeError, match="too few free pages"):
+        d.prefill(1, prompt(40))
+
+
+def test_the_command_runs(cuda_device, capsys):
+    main()
+    text = capsys.readouterr().out
+    assert "two branches kept" in text and "16 more tokens" in text
