@@ -65,6 +65,36 @@ __device__ __forceinline__ float log2_of(float x) {
     return y;
 }
 
+// acc[0..N) = f * x[0..N) + acc, and products and sums alike: two at a time where a lane holds two
+// columns side by side.
+template <int N>
+__device__ __forceinline__ void fma_into(float* acc, float f, const float* x) {
+    if constexpr (N == 2) {
+        const float2 r = __ffma2_rn(make_float2(f, f), make_float2(x[0], x[1]), make_float2(acc[0], acc[1]));
+        acc[0] = r.x, acc[1] = r.y;
+    } else {
+        acc[0] = __fmaf_rn(f, x[0], acc[0]);
+    }
+}
+template <int N>
+__device__ __forceinline__ void scale_by(float* x, const float* f) {
+    if constexpr (N == 2) {
+        const float2 r = __fmul2_rn(make_float2(x[0], x[1]), make_float2(f[0], f[1]));
+        x[0] = r.x, x[1] = r.y;
+    } else {
+        x[0] *= f[0];
+    }
+}
+template <int N>
+__device__ __forceinline__ void add_into(float* acc, const float* x) {
+    if constexpr (N == 2) {
+        const float2 r = __fadd2_rn(make_float2(acc[0], acc[1]), make_float2(x[0], x[1]));
+        acc[0] = r.x, acc[1] = r.y;
+    } else {
+        acc[0] += x[0];
+    }
+}
+
 __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -318,11 +348,9 @@ __device__ __forceinline__ void tile_logits(const State<NG, NT, NC>& s, uint32_t
 #pragma unroll
     for (int r = 0; r < NT; ++r) {
         mma_new(x[r], la, lb, la, lb, s.q_sum[r][0], s.q_sum[r][1]);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            x[r][c] *= 0x1p-18f;
-            x[r][2 + c] *= 0x1p-18f;
-        }
+        const float down[2] = {0x1p-18f, 0x1p-18f};
+        scale_by<NC>(x[r], down);
+        scale_by<NC>(x[r] + 2, down);
     }
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
@@ -343,11 +371,8 @@ __device__ __forceinline__ void tile_logits(const State<NG, NT, NC>& s, uint32_t
         const float fa = high_of(pa[k]), fb = high_of(pb[k]);
 #pragma unroll
         for (int r = 0; r < NT; ++r) {
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                x[r][c] = __fmaf_rn(fa, dots[r][c], x[r][c]);
-                x[r][2 + c] = __fmaf_rn(fb, dots[r][2 + c], x[r][2 + c]);
-            }
+            fma_into<NC>(x[r], fa, dots[r]);
+            fma_into<NC>(x[r] + 2, fb, dots[r] + 2);
         }
     }
 }
@@ -413,13 +438,15 @@ __device__ __forceinline__ void tiles_pass(State<NG, NT, NC>& s, uint32_t data, 
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int b = 0; b < NT; ++b)
+            for (int b = 0; b < NT; ++b) {
+                scale_by<NC>(x[h][b] + 2 * half, s.factor[b]);  // may be negative (a negative scale), so -inf comes after it
+                if (kMasked) {
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    float& v = x[h][b][2 * half + c];
-                    v *= s.factor[b][c];  // may be negative (a negative scale), so -inf comes after it
-                    if (kMasked && !(there[h][half] && token + 8 * half < mask.limit[b][c] - mask.base)) v = -INFINITY;
+                    for (int c = 0; c < NC; ++c)
+                        if (!(there[h][half] && token + 8 * half < mask.limit[b][c] - mask.base))
+                            x[h][b][2 * half + c] = -INFINITY;
                 }
+            }
     }
     auto largest = [&](int b, int c) {
         float most = fmaxf(x[0][b][c], x[0][b][2 + c]);
@@ -470,12 +497,15 @@ __device__ __forceinline__ void tiles_pass(State<NG, NT, NC>& s, uint32_t data, 
         for (int half = 0; half < 2; ++half) {
             float p[NT][NC];
 #pragma unroll
-            for (int b = 0; b < NT; ++b)
+            for (int b = 0; b < NT; ++b) {
+                float below[NC];
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    p[b][c] = exp2_of(x[h][b][2 * half + c] - s.top[b][c]);
-                    s.sum[b][c] += p[b][c];
-                }
+                for (int c = 0; c < NC; ++c) below[c] = -s.top[b][c];
+                add_into<NC>(below, x[h][b] + 2 * half);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) p[b][c] = exp2_of(below[c]);
+                add_into<NC>(s.sum[b], p[b]);
+            }
             float delta[NG];
 #pragma unroll
             for (int k = 0; k < NG; ++k) {
@@ -484,19 +514,18 @@ __device__ __forceinline__ void tiles_pass(State<NG, NT, NC>& s, uint32_t data, 
                 const float centre = __fmaf_rn(8.0f, pair.y, pair.x);
                 delta[k] = pair.y;
 #pragma unroll
-                for (int b = 0; b < NT; ++b)
-#pragma unroll
-                    for (int c = 0; c < NC; ++c)
-                        s.low_sum[b][k][c] = __fmaf_rn(p[b][c], centre, s.low_sum[b][k][c]);
+                for (int b = 0; b < NT; ++b) fma_into<NC>(s.low_sum[b][k], centre, p[b]);
             }
 #pragma unroll
             for (int k = 0; k < NG; k += kPer)
 #pragma unroll
-                for (int b = 0; b < NT; ++b)
-                    weights[b][k / kPer][half] =
-                        transposed(half2_of(p[b][0] * delta[k], NC == 2     ? p[b][NC - 1] * delta[k]
-                                                                : kPer == 2 ? p[b][0] * delta[k + kPer - 1]
-                                                                            : 0.0f));
+                for (int b = 0; b < NT; ++b) {
+                    // Two columns of a group, or with one column to a lane two groups.
+                    float w[2] = {p[b][0], NC == 2 ? p[b][NC - 1] : kPer == 2 ? p[b][0] : 0.0f};
+                    const float by[2] = {delta[k], NC == 2 ? delta[k] : delta[k + kPer - 1]};
+                    scale_by<2>(w, by);
+                    weights[b][k / kPer][half] = transposed(half2_of(w[0], w[1]));
+                }
         }
         // Value numbers of tokens j, j + 1 (and + 8) side by side, 16 dims at a time.  They enter
         // as n - 8: the sums stay near zero, so that neither the weights' rounding nor the tensor
