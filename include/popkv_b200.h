@@ -781,6 +781,17 @@ POPKV_API int popkv_verify_drafts(const void* target, int64_t t_seq_stride, int6
                                   const int32_t* counts, const float* uniforms, const float* noise,
                                   void* workspace, int64_t* out_tokens, int32_t* accepted, void* stream);
 
+/*
+ * The entry points above with their arguments, in order, as an array of 64-bit words
+ * (pointers and integers as they are, a float in a word's low 32 bits), for callers whose
+ * foreign-function interface costs per argument.
+ */
+POPKV_API int popkv_kv4_write_words(const int64_t* words);
+POPKV_API int popkv_kv4_read_words(const int64_t* words);
+POPKV_API int popkv_kv4_attention_words(const int64_t* words);
+POPKV_API int popkv_kv4_attention_selected_words(const int64_t* words);
+POPKV_API int popkv_verify_drafts_words(const int64_t* words);
+
 #ifdef __cplusplus
 }
 #endif

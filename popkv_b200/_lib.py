@@ -20,6 +20,7 @@ F32, F16, BF16 = 0, 1, 2
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
+_S = ctypes.c_char_p  # packed argument words
 
 _SIGNATURES = {
     "popkv_abi_version": ([], _I),
@@ -84,6 +85,11 @@ _SIGNATURES = {
     "popkv_kv4_compact": ([_P, _P, _P], _I),
     "popkv_kv4_copy_pages": ([_P, _P, _P, _L, _P], _I),
     "popkv_verify_drafts": ([_P, _L, _L, _P, _L, _L, _I, _L, _L, _L, _P, _P, _P, _P, _P, _P, _P, _P], _I),
+    "popkv_kv4_write_words": ([_S], _I),
+    "popkv_kv4_read_words": ([_S], _I),
+    "popkv_kv4_attention_words": ([_S], _I),
+    "popkv_kv4_attention_selected_words": ([_S], _I),
+    "popkv_verify_drafts_words": ([_S], _I),
     "popkv_norm_lm_head_argmax": ([_P, _L, _L, _L, _P, _P, _P, ctypes.c_float, _P, _P, _P, _P, _P, _P], _I),
 }
 

@@ -22,7 +22,7 @@ LIB_DIR = PACKAGE / "lib"
 LIB_PATH = LIB_DIR / "libpopkv_b200.so"
 SOURCES = ("abi.cu", "pack.cu", "score.cu", "score_mma.cu", "topk.cu", "attention.cu", "attention_static.cu",
            "peer.cu", "retrieve.cu", "decoder.cu", "gemv.cu", "kv4_rows.cu", "kv4_pages.cu", "kv4_attention.cu",
-           "verify.cu")
+           "kv4_words.cu", "verify.cu")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

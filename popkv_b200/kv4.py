@@ -30,6 +30,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import torch
 
@@ -39,6 +40,12 @@ HEAD_DIM = 128
 DIM_GROUP_SIZES = (32, 64, 128)
 PAGE_SIZES = (16, 32, 64, 128, 256)
 MAX_SEQUENCES_PER_CALL = 4096
+
+
+# Argument words of the calls that a decode step makes for each layer (see popkv_kv4_*_words).
+_WRITE = struct.Struct("16q").pack
+_READ = struct.Struct("10q").pack
+_ATTENTION = struct.Struct("12qf4x4q").pack
 
 
 class _Descriptor(ctypes.Structure):
@@ -134,11 +141,23 @@ class Kv4Cache:
         if status:
             _lib.check(status)
 
+    def _call_words(self, entry, pack, *args) -> None:
+        index = self.device.index
+        if index is None:
+            raise RuntimeError("the 4-bit cache must be on a CUDA device")
+        if torch.cuda.current_device() == index:
+            status = entry(pack(self._address, *args, _lib.raw_stream(index)))
+        else:
+            with torch.cuda.device(index):
+                status = entry(pack(self._address, *args, _lib.raw_stream(index)))
+        if status:
+            _lib.check(status)
+
     def _ids(self, ids, name: str) -> torch.Tensor:
         """int32 [n] on the cache's device, from a tensor or a sequence of ints."""
         if not isinstance(ids, torch.Tensor):
             ids = torch.tensor(ids, dtype=torch.int32, device=self.device)
-        if ids.dtype != torch.int32 or not ids.is_contiguous():
+        if ids.dtype is not torch.int32 or not ids.is_contiguous():
             if ids.dtype not in (torch.int32, torch.int64):
                 raise ValueError(f"{name} must be int32 or int64")
             ids = ids.to(torch.int32).contiguous()
@@ -208,9 +227,9 @@ class Kv4Cache:
             values = values.contiguous()
             v0, v1, v2, _ = values.stride()
         counts = None if counts is None else self._per_sequence(counts, n, "counts")
-        self._call(_lib.lib().popkv_kv4_write, self._layer(layer), seqs.data_ptr(), n,
-                   None if counts is None else counts.data_ptr(), keys.data_ptr(), values.data_ptr(), code, shape[1],
-                   k0, k1, k2, v0, v1, v2)
+        self._call_words(_lib.lib().popkv_kv4_write_words, _WRITE, self._layer(layer), seqs.data_ptr(), n,
+                         0 if counts is None else counts.data_ptr(), keys.data_ptr(), values.data_ptr(), code,
+                         shape[1], k0, k1, k2, v0, v1, v2)
 
     def read(self, seqs, *, start: int = 0, tokens: int, layer: int = 0,
              dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
@@ -225,8 +244,8 @@ class Kv4Cache:
             raise ValueError("start and tokens must not be negative")
         seqs, n = self._sequences(seqs, most=1 << 30)
         keys, values = torch.empty((2, n, tokens, self.kv_heads, HEAD_DIM), dtype=dtype, device=self.device).unbind(0)
-        self._call(_lib.lib().popkv_kv4_read, self._layer(layer), seqs.data_ptr(), n, start, tokens, keys.data_ptr(),
-                   values.data_ptr(), code)
+        self._call_words(_lib.lib().popkv_kv4_read_words, _READ, self._layer(layer), seqs.data_ptr(), n, start, tokens,
+                         keys.data_ptr(), values.data_ptr(), code)
         return keys, values
 
     # -- attention -----------------------------------------------------------------
@@ -296,14 +315,15 @@ class Kv4Cache:
         queries, strides, code = self._queries(queries, shape, n)
         if counts is not None:
             counts = self._per_sequence(counts, n, "counts")
-        out = torch.empty(shape, dtype=queries.dtype, device=self.device)
+        out = (torch.empty_like(queries) if queries.is_contiguous()
+               else torch.empty(shape, dtype=queries.dtype, device=self.device))
         q_heads = shape[-2]
         q_len, token_stride = (shape[1], strides[1]) if len(shape) == 4 else (1, 0)
         scratch = self._workspace(workspace, n, q_heads, q_len)
-        self._call(_lib.lib().popkv_kv4_attention, self._layer(layer), seqs.data_ptr(), n,
-                   None if counts is None else counts.data_ptr(), queries.data_ptr(), code, q_heads, q_len,
-                   strides[0], token_stride, strides[-2], _scale(softmax_scale), scratch.data_ptr(),
-                   scratch.shape[0], out.data_ptr())
+        self._call_words(_lib.lib().popkv_kv4_attention_words, _ATTENTION, self._layer(layer), seqs.data_ptr(), n,
+                         0 if counts is None else counts.data_ptr(), queries.data_ptr(), code, q_heads, q_len,
+                         strides[0], token_stride, strides[-2], _scale(softmax_scale), scratch.data_ptr(),
+                         scratch.shape[0], out.data_ptr())
         return out
 
     def attention_selected(self, queries: torch.Tensor, indices: torch.Tensor, *, seqs, layer: int = 0,
@@ -335,12 +355,13 @@ class Kv4Cache:
             if valid_mask.device != self.device:
                 raise RuntimeError("indices and valid mask must be on the cache's device")
             valid_mask = valid_mask.contiguous()
-        out = torch.empty(shape, dtype=queries.dtype, device=self.device)
+        out = (torch.empty_like(queries) if queries.is_contiguous()
+               else torch.empty(shape, dtype=queries.dtype, device=self.device))
         scratch = self._workspace(workspace, n, shape[1], 1)
-        self._call(_lib.lib().popkv_kv4_attention_selected, self._layer(layer), seqs.data_ptr(), n,
-                   queries.data_ptr(), code, shape[1], strides[0], strides[1], indices.data_ptr(), picked[2],
-                   None if valid_mask is None else valid_mask.data_ptr(), _scale(softmax_scale), scratch.data_ptr(),
-                   scratch.shape[0], out.data_ptr())
+        self._call_words(_lib.lib().popkv_kv4_attention_selected_words, _ATTENTION, self._layer(layer),
+                         seqs.data_ptr(), n, queries.data_ptr(), code, shape[1], strides[0], strides[1],
+                         indices.data_ptr(), picked[2], 0 if valid_mask is None else valid_mask.data_ptr(),
+                         _scale(softmax_scale), scratch.data_ptr(), scratch.shape[0], out.data_ptr())
         return out
 
     # -- pages ---------------------------------------------------------------------

@@ -8,9 +8,13 @@ The reference decodes one token per call (popkv.py:988-1115) and has no counterp
 """
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from . import _lib
+
+_WORDS = struct.Struct("18q").pack  # see popkv_verify_drafts_words
 
 
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}  # of each (device, stream): all zero between calls
@@ -73,19 +77,21 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, unifor
     if uniforms.shape != (n, drafts) or noise.shape != (n, vocab):
         raise ValueError("uniforms must be [n, drafts] and noise [n, vocab]")
     dtype, device = target_probs.dtype, target_probs.device
-    given = [draft_tokens, uniforms, noise]
+    together = device.type == "cuda" and draft_tokens.device == uniforms.device == noise.device == device
+    code = _lib.DTYPE_CODES.get(dtype)
+    typed = code is not None
     if draft_probs is not None:
         if draft_probs.shape != (n, drafts, vocab):
             raise ValueError("draft_probs must be [n, drafts, vocab]")
-        given.append(draft_probs)
+        together = together and draft_probs.device == device
+        typed = typed and draft_probs.dtype == dtype
     if counts is not None:
         if counts.shape != (n,):
             raise ValueError("counts must be [n]")
-        given.append(counts)
-    if device.type != "cuda" or any(t.device != device for t in given):
+        together = together and counts.device == device
+    if not together:
         raise RuntimeError("verification tensors must share a CUDA device")
-    code = _lib.DTYPE_CODES.get(dtype)
-    if code is None or (draft_probs is not None and draft_probs.dtype != dtype):
+    if not typed:
         raise RuntimeError("probabilities must share an fp32/fp16/bf16 dtype")
     if draft_tokens.dtype != torch.int64 or uniforms.dtype != torch.float32 or noise.dtype != torch.float32:
         raise RuntimeError("draft_tokens must be int64, uniforms and noise fp32")
@@ -101,7 +107,7 @@ def _verify(target_probs, draft_tokens, uniforms, noise, draft_probs, counts, wo
     n, places, vocab = target_probs.shape
     device = target_probs.device
     target_probs = target_probs if target_probs.stride(2) == 1 else target_probs.contiguous()
-    draft, d_seq, d_place = None, 0, 0
+    draft, d_seq, d_place = 0, 0, 0
     if draft_probs is not None:
         draft_probs = draft_probs if draft_probs.stride(2) == 1 else draft_probs.contiguous()
         draft, (d_seq, d_place, _) = draft_probs.data_ptr(), draft_probs.stride()
@@ -112,10 +118,10 @@ def _verify(target_probs, draft_tokens, uniforms, noise, draft_probs, counts, wo
     stream = _lib.raw_stream(device.index)
     scratch = _workspace(workspace, n, device, stream)
     t_seq, t_place, _ = target_probs.stride()
-    status = _lib.lib().popkv_verify_drafts(
+    status = _lib.lib().popkv_verify_drafts_words(_WORDS(
         target_probs.data_ptr(), t_seq, t_place, draft, d_seq, d_place, code, n, places - 1, vocab,
-        draft_tokens.data_ptr(), None if counts is None else counts.data_ptr(), uniforms.data_ptr(),
-        noise.data_ptr(), scratch.data_ptr(), tokens.data_ptr(), accepted.data_ptr(), stream)
+        draft_tokens.data_ptr(), 0 if counts is None else counts.data_ptr(), uniforms.data_ptr(),
+        noise.data_ptr(), scratch.data_ptr(), tokens.data_ptr(), accepted.data_ptr(), stream))
     if status:
         _lib.check(status)
     return tokens, accepted
