@@ -144,7 +144,6 @@ __device__ __forceinline__ void mma_new(float* c, uint32_t a0, uint32_t a1, uint
 }
 
 constexpr uint32_t kEven = 0x000F000Fu, kOdd = 0x00F000F0u;  // n and 16 n of two numbers, as fp16 denormals
-constexpr uint32_t kMinusEven = 0x80088008u, kMinusOdd = 0x80808080u;  // -8 and -16 * 8 likewise
 constexpr uint32_t kEightEven = 0x00080008u, kEightOdd = 0x00800080u;  // 8 and 16 * 8
 
 // Columns of the products: NT blocks of 8, of which a lane (g = lane / 4, t = lane % 4) holds
@@ -277,7 +276,6 @@ __device__ __forceinline__ int token_at(int j) { return j ^ (j >> 1 & 1); }
 // each tile): its two tokens' keys, pairs and group-t pair, and its tokens' values.
 struct Lane {
     uint32_t keys, pairs, low, values, queries;
-    uint32_t minus[4];  // the operand of -8: a register each, which the products want side by side
 };
 
 template <int NG>
@@ -289,10 +287,7 @@ __device__ __forceinline__ Lane lane_places(const void* queries) {
     at.low = at.pairs + 4 * (t & (NG - 1));
     at.values = kKv4ValueOffset + token_at(2 * t) * kKv4RowBytes + 8 * g;
     at.queries = smem_addr(queries) + 16 * lane;
-    at.minus[0] = at.minus[2] = kMinusEven;
-    at.minus[1] = at.minus[3] = kMinusOdd;
     asm volatile("" : "+r"(at.keys), "+r"(at.pairs), "+r"(at.low), "+r"(at.values));
-    asm volatile("" : "+r"(at.minus[0]), "+r"(at.minus[1]), "+r"(at.minus[2]), "+r"(at.minus[3]));
     return at;
 }
 
@@ -530,9 +525,8 @@ __device__ __forceinline__ void tiles_pass(State<NG, NT, NC>& s, uint32_t data, 
         // Value numbers of tokens j, j + 1 (and + 8) side by side, 16 dims at a time.  They enter
         // as n - 8: the sums stay near zero, so that neither the weights' rounding nor the tensor
         // cores' truncated additions are multiplied by the numbers' offset (over 131072 tokens:
-        // error 3.5 times smaller).  With one block of rows the 8 is a product of its own (8 more
-        // products a tile), with several it is taken off the operand that they share (32 more
-        // subtractions).
+        // error 3.5 times smaller).  The 32 subtractions a tile cost less than taking the 8 off in
+        // 8 products of its own (131072 tokens: 41.0 against 43.1 us).
         const uint32_t values = tile + at.values, others = values ^ kKv4RowBytes;  // token_at(2t + 1) = token_at(2t) ^ 1
         const uint2 v0 = shared_load<uint2>(values), v1 = shared_load<uint2>(others);
         const uint2 v2 = shared_load<uint2>(values + 8 * kKv4RowBytes), v3 = shared_load<uint2>(others + 8 * kKv4RowBytes);
@@ -544,20 +538,14 @@ __device__ __forceinline__ void tiles_pass(State<NG, NT, NC>& s, uint32_t data, 
             const uint32_t a8 = upper_numbers(a), c8 = upper_numbers(c);
             uint32_t n[2][4] = {{a & kEven, a & kOdd, c & kEven, c & kOdd},
                                 {a8 & kEven, a8 & kOdd, c8 & kEven, c8 & kOdd}};
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int v = 0; v < 4; ++v) n[u][v] = minus2(n[u][v], v & 1 ? kEightOdd : kEightEven);
             const int k = i * NG / 4 / kPer;
-            if constexpr (NT > 1) {
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int v = 0; v < 4; ++v) n[u][v] = minus2(n[u][v], v & 1 ? kEightOdd : kEightEven);
-            }
 #pragma unroll
             for (int b = 0; b < NT; ++b) {
                 const uint32_t w0 = weights[b][k][0], w1 = weights[b][k][1];
-                if constexpr (NT == 1) {
-                    mma(s.out[b][2 * i], at.minus[0], at.minus[1], at.minus[2], at.minus[3], w0, w1);
-                    mma(s.out[b][2 * i + 1], at.minus[0], at.minus[1], at.minus[2], at.minus[3], w0, w1);
-                }
                 mma(s.out[b][2 * i], n[0][0], n[0][1], n[0][2], n[0][3], w0, w1);
                 mma(s.out[b][2 * i + 1], n[1][0], n[1][1], n[1][2], n[1][3], w0, w1);
             }
