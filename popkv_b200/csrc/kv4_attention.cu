@@ -567,9 +567,10 @@ __device__ __forceinline__ uint16_t rounded(float v, int bf16) {
     return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
 
-// A segment costs a CTA about as much as this many chunks besides its own (queries, page
-// lookups, first copies, merge: 5 us against 0.3 us a chunk).
-constexpr int kSegmentCost = 16;
+// A segment costs a CTA about as much as this many chunks besides its own: queries, page
+// lookups, first copies and merge take 5 us, a chunk about 0.2 us.  33 sequences of 0 to 8192
+// tokens take 46.3 us with shares that count it so, 58.6 us with 8.
+constexpr int kSegmentCost = 24;
 
 // The work of one CTA: [begin, end) of the flat list of all (entry, head, row tile) segments,
 // each of which is kSegmentCost units and then its chunks; `first` units lie before the current

@@ -12,6 +12,7 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kCopyThreads = 256;
 constexpr int kRowThreads = 128;
+constexpr int kMostEntries = 4096;  // sequences of one call
 
 // Whether entry i names a sequence in range that no earlier entry names.
 __device__ bool first_of(const Kv4View& view, const int32_t* seqs, int i) {
@@ -50,18 +51,27 @@ __device__ int block_scan(int value, int* total) {
     return before + inclusive - value;
 }
 
-// One CTA.  workspace: found [num_pages] | first [n] | source [n] | target [n].
+// One CTA: its time is a chain of dependent loads (ids, lengths, last pages, their counts; the
+// free pages' counts are read ahead), so what an entry needs stays in shared memory up to
+// kPlanThreads entries.  workspace: found [num_pages] | first [n] | source [n] | target [n].
 __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Kv4View view, const int32_t* __restrict__ seqs, int n,
                                                               const int32_t* __restrict__ counts, int count,
                                                               int32_t* __restrict__ workspace) {
+    __shared__ int32_t ids[kMostEntries];
+    __shared__ int32_t near[3][kPlanThreads];
+    __shared__ int short_of_columns;
     pdl_wait();
     pdl_launch_dependents();
     int32_t* found = workspace;
-    int32_t* first = found + view.num_pages;
-    int32_t* source = first + n;
+    const bool few = n <= kPlanThreads;
+    int32_t* first = few ? near[0] : found + view.num_pages;
+    int32_t* needs = few ? near[1] : found + view.num_pages + 2 * n;
+    int32_t* copies = few ? near[2] : found + view.num_pages + n;
+    int32_t* source = found + view.num_pages + n;
     int32_t* target = source + n;
     const int size = view.page_size();
-    __shared__ int short_of_columns;
+    int refs_ahead = threadIdx.x < view.num_pages ? view.refs[threadIdx.x] : 1;
+    for (int i = threadIdx.x; i < n; i += kPlanThreads) ids[i] = seqs[i];
     if (threadIdx.x == 0) short_of_columns = 0;
     __syncthreads();
 
@@ -72,8 +82,8 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Kv4View view, cons
         const int i = base + threadIdx.x;
         int need = 0, copied = -1;
         if (i < n) {
-            if (first_of(view, seqs, i)) {
-                const int s = seqs[i], held = view.length_of(s);
+            if (first_of(view, ids, i)) {
+                const int s = ids[i], held = view.length_of(s);
                 const int more = max(0, counts ? counts[i] : count);
                 // 64 bits: a count near the int limit must not wrap past the check.
                 const int64_t columns = (static_cast<int64_t>(held) + more + size - 1) >> view.page_shift;
@@ -91,15 +101,15 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Kv4View view, cons
                 }
             } else {
                 need = -1;
-                if (seqs[i] != -1) atomicOr(view.status, kKv4StatusSequence);
+                if (ids[i] != -1) atomicOr(view.status, kKv4StatusSequence);
             }
         }
         int total;
         const int before = block_scan(max(need, 0), &total);
         if (i < n) {
             first[i] = needed + before;
-            source[i] = copied;
-            target[i] = need;  // until the pages are known; -1: not an entry to extend
+            copies[i] = copied;
+            needs[i] = need;  // -1: not an entry to extend
         }
         needed = min(needed + total, view.num_pages + 1);
     }
@@ -107,8 +117,9 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Kv4View view, cons
     // The lowest free pages, in order.
     int free_pages = 0;
     for (int base = 0; base < view.num_pages && free_pages < needed; base += kPlanThreads) {
-        const int p = base + threadIdx.x;
-        const bool is_free = p < view.num_pages && view.refs[p] == 0;
+        const int p = base + threadIdx.x, next = p + kPlanThreads;
+        const bool is_free = refs_ahead == 0;
+        refs_ahead = next < view.num_pages ? view.refs[next] : 1;
         int total;
         const int at = free_pages + block_scan(is_free, &total);
         if (is_free && at < needed) found[at] = p;
@@ -124,9 +135,13 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Kv4View view, cons
     // Hand them out, a warp per entry.
     for (int i = threadIdx.x >> 5; i < n; i += kPlanThreads / 32) {
         const int lane = threadIdx.x & 31;
-        const int need = target[i], at = first[i], copied = source[i];
-        const int s = seqs[i];
+        const int need = needs[i], at = first[i], copied = copies[i];
+        const int s = ids[i];
         __syncwarp();
+        if (lane == 0) {
+            source[i] = need < 0 ? -1 : copied;
+            if (copied >= 0) target[i] = found[at];
+        }
         if (need < 0) continue;
         const int held = view.length_of(s), more = max(0, counts ? counts[i] : count);
         int column = view.pages_of(held) - (copied >= 0);
@@ -135,12 +150,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Kv4View view, cons
             view.table[static_cast<int64_t>(s) * view.max_pages + column + j] = page;
             view.refs[page] = 1;
         }
-        if (lane == 0) {
-            if (copied >= 0) {
-                atomicSub(view.refs + copied, 1);
-                target[i] = found[at];
-            }
-        }
+        if (lane == 0 && copied >= 0) atomicSub(view.refs + copied, 1);
         __syncwarp();
         if (lane == 0) view.lengths[s] = held + more;
     }
@@ -365,7 +375,8 @@ int launch_plan(const char* what, void (*kernel)(Parameters...), unsigned blocks
 }
 
 int check_entries(const char* what, int64_t n) {
-    if (n < 0 || n > 4096) return fail(POPKV_ERR_INVALID, "%s: between 0 and 4096 sequences in one call", what);
+    if (n < 0 || n > kMostEntries)
+        return fail(POPKV_ERR_INVALID, "%s: between 0 and 4096 sequences in one call", what);
     return POPKV_OK;
 }
 }  // namespace
