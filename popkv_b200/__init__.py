@@ -14,6 +14,14 @@ Drop-in for the reference's retrieval path:
 * ``popkv_b200.sharding``       -- KV-head sharding across GPUs with one
                                     all-gather of head outputs per layer
 
+Beside it, for serving:
+
+* ``popkv_b200.kv4``            -- Kv4Cache: a KV cache held in 4 bits, in pages, its
+                                    attention and page operations
+* ``popkv_b200.speculative``    -- verify_drafts: drafted tokens against the target's
+                                    probabilities
+* ``popkv_b200.kv4_decode``     -- Kv4Decoder: sampling decode from the 4-bit cache
+
 All compute runs in ``lib/libpopkv_b200.so`` (hand-written CUDA for sm_100a
 behind the C ABI in ``include/popkv_b200.h``).
 """
