@@ -15,6 +15,13 @@
 // of the logits' product and the 16-deep axis of the outputs' product, query rows
 // are the 8 columns of both.  One pass over the cache serves every query row of a KV
 // head, and a warp needs no exchange with others until its tokens are through.
+//
+// What bounds it, measured with 32 query and 8 KV heads, groups of 32 dims: one query token over
+// 131072 tokens (168 MB) takes 41.1 us, of which about 12 us are fixed (finding the CTA's
+// share, first lookups and copies, merge, join); the loop itself runs at 84 to 91% of the
+// copy rate, with the ALU pipe, which takes the numbers apart, next at 46%.  Five query tokens
+// (20 rows) are bound by fixed-latency dependencies at 8 warps of 255 registers: 76 us.  Selected
+// slots are bound by 128-byte memory lines: 347 bytes move per slot of 160.
 #include <cmath>
 #include <type_traits>
 
@@ -597,7 +604,7 @@ __device__ __forceinline__ int chunks_of(const Params& p, int entry) {
 //
 // Segments of one length (a single sequence, or selected slots) are cut into equal parts, one to a
 // CTA, where those are not much longer than even shares, which straddle segments and make a CTA
-// merge two of them: 32 query and 8 KV heads x 32768 tokens take 17.9 us in 18 parts a head and
+// merge two of them: 32 query and 8 KV heads x 32768 tokens take 17.4 us in 18 parts a head and
 // 20.7 us in even shares.
 template <bool kSelected, int kWarps>
 __device__ Place find_place(const Params& p, int segments) {
@@ -721,11 +728,13 @@ __device__ __forceinline__ void copy8(uint8_t* to, const uint8_t* from, bool the
 
 template <int NG, int NT, int NC, bool kSelected>
 struct Sizes {
+    // 12 warps of 168 registers where a lane holds one row (131072 tokens: 41.0 against 43.5 us with 8),
+    // 8 of up to 255 where it holds more (16 rows with 12: spills, 71.3 against 69.4 us; 24 rows: 140 against 97).
     static constexpr int kWarps = kSelected || NC == 1 ? 12 : 8;
     static constexpr int kTogether = NT == 1 && !kSelected ? 2 : 1;  // tiles of one pass
     static constexpr int kTile = kKv4PairOffset + kKv4TileTokens * 8 * NG;
     static constexpr int kStageBytes = 2 * kTile;
-    static constexpr int kStages = 2;  // chunks of a warp in flight
+    static constexpr int kStages = 2;  // chunks of a warp in flight; 3 or 4 change nothing
     static constexpr int kRing = kWarps * kStages * kStageBytes;
     static constexpr int kMerge = kWarps * Columns<NT, NC>::kRows * kMergeStride * 4;
 };

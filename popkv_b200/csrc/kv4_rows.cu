@@ -1,5 +1,10 @@
 // Rows of the 4-bit cache: quantise new keys and values into their pages, and
 // read cached rows back as fp16/bf16/fp32.
+//
+// Of a group's values x: low = fp16(min), delta = fp16((max - low) / 15), n = rint((x - low) *
+// (1 / delta)) within 0..15; a number stands for low + n * delta.  Both kernels are bound by
+// issue (224 and 129 warp instructions a token and head, at 66 and 64% issue): 8191 tokens of
+// 8 heads in bf16 take 32.7 us written and read back, against 13.4 us for the bytes.
 #include "kv4.cuh"
 
 namespace popkv {
