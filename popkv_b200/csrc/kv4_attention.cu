@@ -731,7 +731,9 @@ struct Sizes {
     // 12 warps of 168 registers where a lane holds one row (131072 tokens: 41.0 against 43.5 us with 8),
     // 8 of up to 255 where it holds more (16 rows with 12: spills, 71.3 against 69.4 us; 24 rows: 140 against 97).
     static constexpr int kWarps = kSelected || NC == 1 ? 12 : 8;
-    static constexpr int kTogether = NT == 1 && !kSelected ? 2 : 1;  // tiles of one pass
+    // Tiles of one pass: two give the products more that does not wait (131072 tokens, 16 rows: 62.5 against
+    // 68.4 us with one; 8 x 4096 selected: 76.2 against 77.6).  With 24 rows two spill (73.7 against 74.9 us).
+    static constexpr int kTogether = NT <= 2 ? 2 : 1;
     static constexpr int kTile = kKv4PairOffset + kKv4TileTokens * 8 * NG;
     static constexpr int kStageBytes = 2 * kTile;
     static constexpr int kStages = 2;  // chunks of a warp in flight; 3 or 4 change nothing
