@@ -574,11 +574,6 @@ __device__ __forceinline__ uint16_t rounded(float v, int bf16) {
     return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
 
-// A segment costs a CTA about as much as this many chunks besides its own: queries, page
-// lookups, first copies and merge take 5 us, a chunk about 0.2 us.  33 sequences of 0 to 8192
-// tokens take 46.3 us with shares that count it so, 58.6 us with 8.
-constexpr int kSegmentCost = 24;
-
 // The work of one CTA: [begin, end) of the flat list of all (entry, head, row tile) segments,
 // each of which is kSegmentCost units and then its chunks; `first` units lie before the current
 // entry.  With `parts` every segment is cut into that many, one to a CTA; with 0 the list is
@@ -606,7 +601,7 @@ __device__ __forceinline__ int chunks_of(const Params& p, int entry) {
 // CTA, where those are not much longer than even shares, which straddle segments and make a CTA
 // merge two of them: 32 query and 8 KV heads x 32768 tokens take 17.4 us in 18 parts a head and
 // 20.7 us in even shares.
-template <bool kSelected, int kWarps>
+template <bool kSelected, int kWarps, int kSegmentCost>
 __device__ Place find_place(const Params& p, int segments) {
     constexpr int kThreads = 32 * kWarps;
     __shared__ int64_t sums[kWarps];
@@ -726,11 +721,21 @@ __device__ __forceinline__ void copy8(uint8_t* to, const uint8_t* from, bool the
                  : "memory");
 }
 
-template <int NG, int NT, int NC, bool kSelected>
+// kWhole: one CTA to an SM, otherwise several small ones.  Few long segments need the large one, whose
+// parts are fewer and longer (131072 tokens 41.1 against 46.9 us, 20 rows of 8000 21.5 against 33.5 us);
+// with many, small CTAs hide each other's 5 us a segment (33 ragged sequences 41.9 against 46.3 us,
+// 256 of 10 to 600 tokens 48.7 against 76.3 us, 8 x 4096 selected 70.4 against 76.0 us).
+template <int NG, int NT, int NC, bool kSelected, bool kWhole>
 struct Sizes {
     // 12 warps of 168 registers where a lane holds one row (131072 tokens: 41.0 against 43.5 us with 8),
     // 8 of up to 255 where it holds more (16 rows with 12: spills, 71.3 against 69.4 us; 24 rows: 140 against 97).
-    static constexpr int kWarps = kSelected || NC == 1 ? 12 : 8;
+    static constexpr int kCtas = kWhole ? 1 : NC == 1 ? 3 : 2;  // on an SM
+    static constexpr int kWarps = (NC == 1 ? 12 : 8) / kCtas;
+    // A segment costs a CTA about as much as this many chunks besides its own: queries, page lookups,
+    // first copies and merge.  33 ragged sequences by one CTA to an SM: 46.3 us with 24, 58.6 us with 8;
+    // by three: 43.4, 41.9 and 44.0 us with 6, 12 and 24.  64 of 100 to 2000 tokens and 20 rows: 73.3, 76.1
+    // and 79.7 us with 16, 24 and 32.  Selected, 16 x 512: 28.2, 26.6 and 28.2 us with 6, 8 and 10.
+    static constexpr int kSegmentCost = kWhole ? 24 : kSelected ? 8 : NC == 1 ? 12 : 16;
     // Tiles of one pass: two give the products more that does not wait (131072 tokens, 16 rows: 62.5 against
     // 68.4 us with one; 8 x 4096 selected: 76.2 against 77.6).  With 24 rows two spill (73.7 against 74.9 us).
     static constexpr int kTogether = NT <= 2 ? 2 : 1;
@@ -741,7 +746,7 @@ struct Sizes {
     static constexpr int kMerge = kWarps * Columns<NT, NC>::kRows * kMergeStride * 4;
 };
 
-template <bool kSelected, int kRows>
+template <bool kSelected, int kRows, int kSegmentCost>
 __device__ __forceinline__ Segment segment_at(const Params& p, const Place& place, int64_t at, int segments, int group,
                                               int rows) {
     Segment s;
@@ -934,11 +939,12 @@ struct Join {
     }
 };
 
-template <int NG, int NT, int NC, bool kSelected>
-__global__ void __launch_bounds__(32 * Sizes<NG, NT, NC, kSelected>::kWarps, 1)
+template <int NG, int NT, int NC, bool kSelected, bool kWhole>
+__global__ void __launch_bounds__(32 * Sizes<NG, NT, NC, kSelected, kWhole>::kWarps, Sizes<NG, NT, NC, kSelected, kWhole>::kCtas)
     attention_kernel(const __grid_constant__ Params p) {
-    using Size = Sizes<NG, NT, NC, kSelected>;
+    using Size = Sizes<NG, NT, NC, kSelected, kWhole>;
     constexpr int kWarps = Size::kWarps, kThreads = 32 * kWarps, kTogether = Size::kTogether;
+    constexpr int kSegmentCost = Size::kSegmentCost;
     constexpr int kTile = Size::kTile, kStageBytes = Size::kStageBytes, kStages = Size::kStages;
     constexpr int kRows = Columns<NT, NC>::kRows;
     constexpr int kPartFloats = kRows * (kDim + 2);
@@ -961,7 +967,7 @@ __global__ void __launch_bounds__(32 * Sizes<NG, NT, NC, kSelected>::kWarps, 1)
     const int group = p.q_heads / p.view.kv_heads;
     const int rows = kSelected ? 1 : p.q_len * group;
     const int segments = heads * p.tiles;
-    Place place = find_place<kSelected, kWarps>(p, segments);
+    Place place = find_place<kSelected, kWarps, kSegmentCost>(p, segments);
     if (place.begin >= place.end) return;
     int next_slot = 0;  // the stage to wait for, and its phase
     uint32_t phase = 0;
@@ -997,7 +1003,7 @@ __global__ void __launch_bounds__(32 * Sizes<NG, NT, NC, kSelected>::kWarps, 1)
             ++place.entry;
             place.chunks = chunks_of<kSelected>(p, place.entry);
         }
-        segment = segment_at<kSelected, kRows>(p, place, place.begin, segments, group, rows);
+        segment = segment_at<kSelected, kRows, kSegmentCost>(p, place, place.begin, segments, group, rows);
         place.begin = place.first + static_cast<int64_t>(segment.number + 1) * (place.chunks + kSegmentCost);
         return segment.chunk0 < segment.chunk1;
     };
@@ -1153,7 +1159,8 @@ __global__ void __launch_bounds__(32 * Sizes<NG, NT, NC, kSelected>::kWarps, 1)
             __syncthreads();
             if (is_last) {
                 // Few rows: several warps to a row, each with every few parts.
-                const int per_row = live_rows == 1 ? 8 : live_rows == 2 ? 4 : live_rows <= 4 ? 2 : 1;
+                constexpr int kMost = kWarps >= 8 ? 8 : 4;
+                const int per_row = max(1, live_rows == 1 ? kMost : live_rows == 2 ? kMost / 2 : live_rows <= 4 ? kMost / 4 : 1);
                 const int sub = warp & (per_row - 1);
                 for (int r = warp / per_row; r < live_rows; r += kWarps / per_row) {
                     Join row;
@@ -1193,9 +1200,9 @@ __global__ void __launch_bounds__(32 * Sizes<NG, NT, NC, kSelected>::kWarps, 1)
     if (failed && lane == 0) atomicOr(p.view.status, kKv4StatusWait);
 }
 
-constexpr int kMostCtas = 148;  // one to an SM
+constexpr int kSms = 148;
 constexpr int kMostRows = 24;
-constexpr int64_t kPartsBytes = int64_t{kMostCtas} * 2 * kMostRows * (kDim + 2) * 4;
+constexpr int64_t kPartsBytes = int64_t{2 * kSms} * 2 * kMostRows * (kDim + 2) * 4;
 
 int check_queries(const char* what, const Kv4View& view, int64_t layer, int64_t n, int64_t q_heads, int64_t q_len,
                   int dtype, const void* queries, int64_t s0, int64_t s1, int64_t s2) {
@@ -1212,24 +1219,25 @@ int check_queries(const char* what, const Kv4View& view, int64_t layer, int64_t 
     return POPKV_OK;
 }
 
-template <int NG, int NT, int NC, bool kSelected>
+template <int NG, int NT, int NC, bool kSelected, bool kWhole>
 int launch(const char* what, const Params& p, int64_t most_chunks, cudaStream_t stream) {
-    using Size = Sizes<NG, NT, NC, kSelected>;
-    constexpr int kSmem = Size::kRing + Size::kMerge;
-    static_assert(kSmem + sizeof(Queries<NT>) < 225 * 1024, "one CTA fits an SM");
-    auto kernel = attention_kernel<NG, NT, NC, kSelected>;
+    using Size = Sizes<NG, NT, NC, kSelected, kWhole>;
+    constexpr int kSmem = Size::kRing + Size::kMerge, kCtas = kSms * Size::kCtas;
+    static_assert(Size::kCtas * (kSmem + sizeof(Queries<NT>) + 2048) < 227 * 1024, "the CTAs fit an SM");
+    static_assert(kCtas * 2ll * Columns<NT, NC>::kRows * (kDim + 2) * 4 <= kPartsBytes, "their parts fit the workspace");
+    auto kernel = attention_kernel<NG, NT, NC, kSelected, kWhole>;
     if (int status = allow_dynamic_smem(kernel, kSmem)) return status;
-    const unsigned grid = static_cast<unsigned>(most_chunks < kMostCtas ? most_chunks : kMostCtas);
+    const unsigned grid = static_cast<unsigned>(most_chunks < kCtas ? most_chunks : kCtas);
     const cudaError_t err = launch_pdl(kernel, dim3(grid), dim3(32 * Size::kWarps), kSmem, stream, 1, p);
     if (err != cudaSuccess) return fail(POPKV_ERR_CUDA, "%s: %s", what, cudaGetErrorString(err));
     return check_launch(what);
 }
 
-template <int NT, int NC, bool kSelected>
+template <int NT, int NC, bool kSelected, bool kWhole>
 int launch_groups(const char* what, const Params& p, int64_t most_chunks, cudaStream_t stream) {
-    if (p.view.groups == 4) return launch<4, NT, NC, kSelected>(what, p, most_chunks, stream);
-    if (p.view.groups == 2) return launch<2, NT, NC, kSelected>(what, p, most_chunks, stream);
-    return launch<1, NT, NC, kSelected>(what, p, most_chunks, stream);
+    if (p.view.groups == 4) return launch<4, NT, NC, kSelected, kWhole>(what, p, most_chunks, stream);
+    if (p.view.groups == 2) return launch<2, NT, NC, kSelected, kWhole>(what, p, most_chunks, stream);
+    return launch<1, NT, NC, kSelected, kWhole>(what, p, most_chunks, stream);
 }
 
 constexpr float kLog2E = 1.4426950408889634f;
@@ -1301,10 +1309,19 @@ extern "C" int popkv_kv4_attention(const popkv_kv4_cache* cache, int64_t layer, 
     const int64_t chunks = (static_cast<int64_t>(p.view.max_pages) * p.view.page_size() + kChunk - 1) / kChunk;
     const int64_t most = n * p.view.kv_heads * p.tiles * chunks;
     const auto s = static_cast<cudaStream_t>(stream);
-    if (rows <= 4) return launch_groups<1, 1, false>(what, p, most, s);
-    return blocks == 1   ? launch_groups<1, 2, false>(what, p, most, s)
-           : blocks == 2 ? launch_groups<2, 2, false>(what, p, most, s)
-                         : launch_groups<3, 2, false>(what, p, most, s);
+    // From 64 segments on (128 with more than 8 rows) several small CTAs to an SM.  8 sequences of 8 KV heads and 100
+    // to 6000 tokens, 4 rows: 15.9 us so and 17.8 with one; of 100 to 8000, 20 rows: 37.6 and 36.8; 16 of up to 3000,
+    // 20 rows: 35.6 and 37.3.  4 sequences, 4 rows: 16.8 and 15.7 us.
+    if (n * p.view.kv_heads * p.tiles < (blocks == 1 ? 64 : 128)) {
+        if (rows <= 4) return launch_groups<1, 1, false, true>(what, p, most, s);
+        if (blocks == 1) return launch_groups<1, 2, false, true>(what, p, most, s);
+        if (blocks == 2) return launch_groups<2, 2, false, true>(what, p, most, s);
+        return launch_groups<3, 2, false, true>(what, p, most, s);
+    }
+    if (rows <= 4) return launch_groups<1, 1, false, false>(what, p, most, s);
+    if (blocks == 1) return launch_groups<1, 2, false, false>(what, p, most, s);
+    if (blocks == 2) return launch_groups<2, 2, false, false>(what, p, most, s);
+    return launch_groups<3, 2, false, false>(what, p, most, s);
 }
 
 extern "C" int popkv_kv4_attention_selected(const popkv_kv4_cache* cache, int64_t layer, const int32_t* seqs,
@@ -1340,5 +1357,5 @@ extern "C" int popkv_kv4_attention_selected(const popkv_kv4_cache* cache, int64_
     p.tiles = 1;
     if (int status = bind_workspace(what, p, n, workspace, workspace_bytes)) return status;
     const int64_t chunks = (selected + kChunk - 1) / kChunk;
-    return launch_groups<1, 1, true>(what, p, n * q_heads * (chunks > 0 ? chunks : 1), static_cast<cudaStream_t>(stream));
+    return launch_groups<1, 1, true, false>(what, p, n * q_heads * (chunks > 0 ? chunks : 1), static_cast<cudaStream_t>(stream));
 }

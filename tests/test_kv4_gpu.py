@@ -188,6 +188,34 @@ def test_attention_long_and_split(cuda_device):
     close(got, want, most)
 
 
+@pytest.mark.parametrize("dtype,group,page,heads,per,q_len", [
+    (torch.float16, 32, 16, 2, 4, 1),
+    (torch.bfloat16, 64, 64, 2, 3, 1),
+    (torch.float16, 128, 16, 4, 1, 1),
+    (torch.float16, 32, 32, 2, 7, 1),
+    (torch.float16, 128, 64, 2, 4, 4),
+    (torch.float16, 64, 16, 2, 2, 5),
+    (torch.bfloat16, 32, 64, 2, 4, 5),
+    (torch.float16, 64, 32, 2, 5, 4),
+    (torch.float16, 32, 16, 1, 8, 5),
+])
+def test_attention_of_many_uneven_sequences(cuda_device, dtype, group, page, heads, per, q_len):
+    """More (sequence, head) pairs than CTAs of an SM take in a wave, some of them cut into parts."""
+    lengths = [(53 * i) % 140 if i % 23 else 900 * (i % 4) + 33 for i in range(150)]
+    cache = make(cuda_device, lengths, kv_heads=heads, page=page, group=group)
+    host = R.HostCache.like(cache)
+    queries = random_queries((150, q_len, heads * per, 128), dtype, cuda_device, group + q_len)
+    got = cache.attention(queries, seqs=list(range(150)))
+    some = [0, 1, 23, 46, 69, 70, 92, 115, 138, 149]
+    want, most = expect(cache, host, queries[some],
+                        lambda at: (some[at[0]], range(max(0, lengths[some[at[0]]] - q_len + at[1] + 1))))
+    close(got[some], want, most)
+    # A sequence's result is the same to rounding in a batch of its own, where the work is cut in another way.
+    alone = [cache.attention(queries[i:i + 1], seqs=[i]) for i in range(150)]
+    close(got, torch.cat(alone).double().cpu().numpy(), 2 * most)
+    assert torch.equal(got, cache.attention(queries, seqs=list(range(150))))
+
+
 def test_attention_counts_padding_and_strides(cuda_device):
     lengths = [40, 18, 2]
     cache = make(cuda_device, lengths, kv_heads=2, page=16)
