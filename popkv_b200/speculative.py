@@ -113,8 +113,7 @@ def _verify(target_probs, draft_tokens, uniforms, noise, draft_probs, counts, wo
         draft, (d_seq, d_place, _) = draft_probs.data_ptr(), draft_probs.stride()
     draft_tokens, uniforms, noise = draft_tokens.contiguous(), uniforms.contiguous(), noise.contiguous()
     counts = None if counts is None else counts.contiguous()
-    tokens = torch.empty((n, places), dtype=torch.int64, device=device)
-    accepted = torch.empty(n, dtype=torch.int32, device=device)
+    tokens, accepted = draft_tokens.new_empty((n, places)), draft_tokens.new_empty(n, dtype=torch.int32)
     stream = _lib.raw_stream(device.index)
     scratch = _workspace(workspace, n, device, stream)
     t_seq, t_place, _ = target_probs.stride()
