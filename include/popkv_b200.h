@@ -684,7 +684,7 @@ typedef struct popkv_kv4_cache {
  * values.  low is the group's least value and delta a fifteenth of its range, both
  * rounded to fp16; n = rint((x - low) * (1 / delta)) in fp32, within 0..15.  NaN is
  * stored as 0 and magnitudes past 65504 as 65504.  The pages must belong to the
- * sequence alone (popkv_kv4_extend sees to it).
+ * sequence alone (popkv_kv4_extend sees to it), and no sequence be listed twice.
  */
 POPKV_API int popkv_kv4_write(const popkv_kv4_cache* cache, int64_t layer, const int32_t* seqs, int64_t n,
                               const int32_t* counts, const void* keys, const void* values, int dtype,

@@ -20,8 +20,9 @@
 // 131072 tokens (168 MB) takes 41.1 us, of which about 12 us are fixed (finding the CTA's
 // share, first lookups and copies, merge, join); the loop itself runs at 84 to 91% of the
 // copy rate, with the ALU pipe, which takes the numbers apart, next at 46%.  Five query tokens
-// (20 rows) are bound by fixed-latency dependencies at 8 warps of 255 registers: 76 us.  Selected
-// slots are bound by 128-byte memory lines: 347 bytes move per slot of 160.
+// (20 rows) are bound by fixed-latency dependencies at 8 warps of 255 registers: 76 us.  Many
+// sequences are bound by what each costs besides its chunks (256 of 10 to 600 tokens, 104 MB: 48.7 us),
+// selected slots by three random accesses each, 45 to 50 a nanosecond (8 x 4096 of 131072 tokens: 69.3 us).
 #include <cmath>
 #include <type_traits>
 
@@ -712,7 +713,7 @@ __device__ Place find_place(const Params& p, int segments) {
 
 // 16-byte (or 8-byte) copy into shared memory, zeros where `there` is false.
 __device__ __forceinline__ void copy16(uint8_t* to, const uint8_t* from, bool there) {
-    // 64 bytes at a time from memory: the rows are that long (8 x 4096 slots of 131072 tokens 79.6 -> 77.4 us).
+    // 64 bytes at a time from memory: the rows are that long (8 x 4096 slots of 131072 tokens 70.3 us, by lines of 128 73.6).
     asm volatile("cp.async.cg.shared.global.L2::64B [%0], [%1], 16, %2;" ::"r"(smem_addr(to)), "l"(from), "r"(there ? 16 : 0)
                  : "memory");
 }

@@ -204,7 +204,7 @@ class Kv4Cache:
         keys, values: fp32/fp16/bf16 [n, tokens, kv_heads, 128], or [n, kv_heads, 128] for one
         token; any strides with contiguous dims (slices of a fused projection).  They are the
         last ``tokens`` (or ``counts[i]`` <= tokens, the first of the row's) of sequence
-        ``seqs[i]``, for which ``extend`` has made room.
+        ``seqs[i]`` (each listed once), for which ``extend`` has made room.
         """
         if keys.ndim == 3 and values.ndim == 3:
             keys, values = keys.unsqueeze(1), values.unsqueeze(1)
