@@ -681,7 +681,7 @@ typedef struct popkv_kv4_cache {
  * Quantise keys and values of the LAST counts[i] (NULL: `tokens`) tokens of each
  * listed sequence into its pages of `layer`.  keys[i, t, h, d] is read at keys +
  * i*k_seq_stride + t*k_token_stride + h*k_head_stride + d (elements); likewise the
- * values.  low is the group's least value and delta a fifteenth of its range, both
+ * values.  low is the group's least value and delta its range times 1/15 (fp32), both
  * rounded to fp16; n = rint((x - low) * (1 / delta)) in fp32, within 0..15.  NaN is
  * stored as 0 and magnitudes past 65504 as 65504.  The pages must belong to the
  * sequence alone (popkv_kv4_extend sees to it), and no sequence be listed twice.

@@ -14,7 +14,7 @@ def quantise(x: np.ndarray, group: int):
     x = np.where(np.isnan(x), np.float32(0), x.astype(np.float32))
     x = np.clip(x, np.float32(-65504), np.float32(65504)).reshape(*x.shape[:-1], D // group, group)
     low = x.min(-1).astype(np.float16)
-    span = (x.max(-1) - low.astype(np.float32)) / np.float32(15)
+    span = (x.max(-1) - low.astype(np.float32)) * (np.float32(1) / np.float32(15))
     delta = np.maximum(span, np.float32(0)).astype(np.float16)
     d32 = delta.astype(np.float32)
     scale = np.divide(np.float32(1), d32, out=np.zeros_like(d32), where=d32 > 0)

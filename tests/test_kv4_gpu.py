@@ -132,6 +132,24 @@ def test_write_odd_values(cuda_device):
     assert torch.isfinite(keys).all() and torch.isfinite(values).all()
 
 
+def test_write_rounds_the_range_as_documented(cuda_device):
+    """Ranges whose product with 1/15 and quotient by 15 round to different fp16 deltas."""
+    r = np.random.default_rng(0).uniform(1.0, 30.0, 1 << 21).astype(np.float32)
+    r = r[(r * (np.float32(1) / np.float32(15))).astype(np.float16) != (r / np.float32(15)).astype(np.float16)][:64]
+    assert len(r) >= 32
+    x = torch.rand(1, len(r), 1, 128, generator=torch.Generator().manual_seed(1)) * torch.from_numpy(r)[:, None, None]
+    x[..., 0] = 0.0
+    x[..., 127] = torch.from_numpy(r)[:, None]
+    cache = Kv4Cache(8, kv_heads=1, max_seqs=1, max_tokens=128, dim_group_size=128, page_size=16, device=cuda_device)
+    cache.extend([0], len(r))
+    cache.write(x.to(cuda_device), -x.to(cuda_device), seqs=[0])
+    keys, values = cache.read([0], tokens=len(r), dtype=torch.float32)
+    for got, given in ((keys, x), (values, -x)):
+        n, low, delta = R.quantise(given.numpy(), 128)
+        want = low.astype(np.float32) + n.astype(np.float32) * delta.astype(np.float32)
+        assert np.array_equal(got.cpu().numpy(), want)
+
+
 def test_write_counts_padding_and_unaligned_views(cuda_device):
     cache = make(cuda_device, [20, 33, 7])
     host = R.HostCache.like(cache)
