@@ -183,6 +183,17 @@ struct Queries {
     float factor[NT][8];
 };
 
+// Query token and place in its group of a row.  Up to 4 rows are mostly one token's: no division then
+// (77 tokens 6.8 -> 6.4 us, 64 sequences 32.3 -> 31.6 us); with more rows the test costs as much as it saves.
+template <bool kFew>
+__device__ __forceinline__ int token_of(const Params& p, int row, int group) {
+    return kFew && p.q_len == 1 ? 0 : row / group;
+}
+template <bool kFew>
+__device__ __forceinline__ int member_of(const Params& p, int row, int group) {
+    return kFew && p.q_len == 1 ? row : row % group;
+}
+
 // The part of one CTA's work inside one segment: chunks [chunk0, chunk1) of a row tile of a KV
 // head (or of a query head's selected slots).
 struct Segment {
@@ -202,8 +213,9 @@ __device__ __forceinline__ void load_queries(const Params& p, const Segment& seg
         const int row = segment.first_row + (NC == 2 ? column : column >> 1);
         raw[k] = make_uint4(0u, 0u, 0u, 0u);
         if (item < NT * 128 && row < rows && (NC == 2 || (column & 1) == 0))
-            raw[k] = *reinterpret_cast<const uint4*>(p.queries + segment.entry * p.q_seq + (row / group) * p.q_token +
-                                                     (segment.head0 + row % group) * p.q_head + 8 * word);
+            raw[k] = *reinterpret_cast<const uint4*>(p.queries + segment.entry * p.q_seq +
+                                                     token_of<NC == 1>(p, row, group) * p.q_token +
+                                                     (segment.head0 + member_of<NC == 1>(p, row, group)) * p.q_head + 8 * word);
     }
 }
 
@@ -713,7 +725,8 @@ __device__ Place find_place(const Params& p, int segments) {
 
 // 16-byte (or 8-byte) copy into shared memory, zeros where `there` is false.
 __device__ __forceinline__ void copy16(uint8_t* to, const uint8_t* from, bool there) {
-    // 64 bytes at a time from memory: the rows are that long (8 x 4096 slots of 131072 tokens 70.3 us, by lines of 128 73.6).
+    // 64 bytes at a time from memory: the rows are that long (8 x 4096 slots of 131072 tokens 70.3 us, by lines
+    // of 128 73.6).
     asm volatile("cp.async.cg.shared.global.L2::64B [%0], [%1], 16, %2;" ::"r"(smem_addr(to)), "l"(from), "r"(there ? 16 : 0)
                  : "memory");
 }
@@ -759,7 +772,8 @@ __device__ __forceinline__ Segment segment_at(const Params& p, const Place& plac
     s.chunk1 = static_cast<int>(min(static_cast<int64_t>(place.chunks), place.end - from));  // none: <= chunk0
     s.whole = s.chunk0 == 0 && s.chunk1 == place.chunks;
     s.entry = place.entry;
-    const int head = s.number / p.tiles;
+    constexpr bool kFew = kRows == 4;
+    const int head = kFew && p.tiles == 1 ? s.number : s.number / p.tiles;
     s.first_row = (s.number - head * p.tiles) * kRows;
     s.seq = p.seqs[s.entry];
     s.length = p.view.length_of(s.seq);
@@ -768,8 +782,8 @@ __device__ __forceinline__ Segment segment_at(const Params& p, const Place& plac
     s.head0 = kSelected ? head : head * group;
     s.last_row = min(s.first_row + kRows, min(rows, s.count * group)) - 1;
     s.seen = kSelected ? p.selected
-             : s.last_row < s.first_row ? 0 : max(0, s.length - s.count + s.last_row / group + 1);
-    s.seen_by_all = kSelected ? 0 : max(0, s.length - s.count + s.first_row / group + 1);
+             : s.last_row < s.first_row ? 0 : max(0, s.length - s.count + token_of<kFew>(p, s.last_row, group) + 1);
+    s.seen_by_all = kSelected ? 0 : max(0, s.length - s.count + token_of<kFew>(p, s.first_row, group) + 1);
     return s;
 }
 
@@ -941,7 +955,8 @@ struct Join {
 };
 
 template <int NG, int NT, int NC, bool kSelected, bool kWhole>
-__global__ void __launch_bounds__(32 * Sizes<NG, NT, NC, kSelected, kWhole>::kWarps, Sizes<NG, NT, NC, kSelected, kWhole>::kCtas)
+__global__ void __launch_bounds__(32 * Sizes<NG, NT, NC, kSelected, kWhole>::kWarps,
+                                  Sizes<NG, NT, NC, kSelected, kWhole>::kCtas)
     attention_kernel(const __grid_constant__ Params p) {
     using Size = Sizes<NG, NT, NC, kSelected, kWhole>;
     constexpr int kWarps = Size::kWarps, kThreads = 32 * kWarps, kTogether = Size::kTogether;
@@ -1022,8 +1037,9 @@ __global__ void __launch_bounds__(32 * Sizes<NG, NT, NC, kSelected, kWhole>::kWa
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const int row = segment.first_row + Columns<NT, NC>::row_of(b, t, c);
-                mask.limit[b][c] =
-                    kSelected || row > segment.last_row ? 0x7FFFFFFF : segment.length - segment.count + row / group + 1;
+                mask.limit[b][c] = kSelected || row > segment.last_row
+                                       ? 0x7FFFFFFF
+                                       : segment.length - segment.count + token_of<NC == 1>(p, row, group) + 1;
             }
         if constexpr (kSelected) {
             mask.base = 0;
@@ -1112,8 +1128,9 @@ __global__ void __launch_bounds__(32 * Sizes<NG, NT, NC, kSelected, kWhole>::kWa
         is_first = false;
         auto write_row = [&](int r, const Join& row_of) {
             const int row = done.first_row + r;
-            uint16_t* to = p.out + ((static_cast<int64_t>(done.entry) * p.q_len + (kSelected ? 0 : row / group)) * p.q_heads +
-                                    done.head0 + (kSelected ? 0 : row % group)) * kDim;
+            const int token = kSelected ? 0 : token_of<NC == 1>(p, row, group);
+            const int head = done.head0 + (kSelected ? 0 : member_of<NC == 1>(p, row, group));
+            uint16_t* to = p.out + ((static_cast<int64_t>(done.entry) * p.q_len + token) * p.q_heads + head) * kDim;
             const bool none = row_of.sum == 0.0f || row > done.last_row;
             const float by = none ? 0.0f : 1.0f / row_of.sum;
             uint2 bits;
@@ -1161,7 +1178,8 @@ __global__ void __launch_bounds__(32 * Sizes<NG, NT, NC, kSelected, kWhole>::kWa
             if (is_last) {
                 // Few rows: several warps to a row, each with every few parts.
                 constexpr int kMost = kWarps >= 8 ? 8 : 4;
-                const int per_row = max(1, live_rows == 1 ? kMost : live_rows == 2 ? kMost / 2 : live_rows <= 4 ? kMost / 4 : 1);
+                const int per_row =
+                    max(1, live_rows == 1 ? kMost : live_rows == 2 ? kMost / 2 : live_rows <= 4 ? kMost / 4 : 1);
                 const int sub = warp & (per_row - 1);
                 for (int r = warp / per_row; r < live_rows; r += kWarps / per_row) {
                     Join row;
@@ -1358,5 +1376,6 @@ extern "C" int popkv_kv4_attention_selected(const popkv_kv4_cache* cache, int64_
     p.tiles = 1;
     if (int status = bind_workspace(what, p, n, workspace, workspace_bytes)) return status;
     const int64_t chunks = (selected + kChunk - 1) / kChunk;
-    return launch_groups<1, 1, true, false>(what, p, n * q_heads * (chunks > 0 ? chunks : 1), static_cast<cudaStream_t>(stream));
+    return launch_groups<1, 1, true, false>(what, p, n * q_heads * (chunks > 0 ? chunks : 1),
+                                            static_cast<cudaStream_t>(stream));
 }
