@@ -132,15 +132,15 @@ struct Exchange {
     }
 };
 
-// The larger (smaller) of two, NaN if either is.
-__device__ __forceinline__ float larger_or_nan(float a, float b) {
+// The largest (smallest) of three, NaN if one is.
+__device__ __forceinline__ float largest_or_nan(float a, float b, float c) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-__device__ __forceinline__ float smaller_or_nan(float a, float b) {
+__device__ __forceinline__ float smallest_or_nan(float a, float b, float c) {
     float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 
@@ -223,11 +223,11 @@ __global__ void __launch_bounds__(kRowsThreads, 4) write_kernel(
 #pragma unroll
                 for (int u = 0; u < kTogether; ++u) {
                     if (!tiles[u]) continue;  // the whole warp
-                    float least = x[u][0], most = x[u][0];
+                    float least = x[u][7], most = x[u][7];
 #pragma unroll
-                    for (int i = 1; i < 8; ++i) {
-                        least = smaller_or_nan(least, x[u][i]);
-                        most = larger_or_nan(most, x[u][i]);
+                    for (int i = 0; i < 7; i += 2) {
+                        least = smallest_or_nan(least, x[u][i], x[u][min(i + 1, 6)]);
+                        most = largest_or_nan(most, x[u][i], x[u][min(i + 1, 6)]);
                     }
                     if (__any_sync(0xFFFFFFFFu, !(least >= -kHalfMost && most <= kHalfMost))) {
 #pragma unroll
@@ -237,21 +237,26 @@ __global__ void __launch_bounds__(kRowsThreads, 4) write_kernel(
                             most = i ? fmaxf(most, x[u][i]) : x[u][i];
                         }
                     }
-                    for (int step = 1; step < lanes; step *= 2) {
+#pragma unroll
+                    for (int step = 1; step < 16; step *= 2) {
+                        if (step >= 4 && step >= lanes) break;  // a group has 4, 8 or 16 lanes
                         least = fminf(least, __shfl_xor_sync(0xFFFFFFFFu, least, step));
                         most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, step));
                     }
                     float low, scale;
                     const uint32_t pair = group_pair(least, most, low, scale);
-                    // rint of a number in 0..15: the low bits of 1.5 * 2^23 + it.  The eight are summed in
-                    // their places, and what the constants add up to (modulo 2^32) is taken off.
+                    // rint of a number, as the low 16 bits of 1.5 * 2^23 + it; past 15 it is at most 23 (a delta that
+                    // is a denormal), below 0 it may be anything.  Two at a time, i and i + 4 of the word.
                     uint32_t word = 0;
+                    const float2 lows = make_float2(-low, -low), scales = make_float2(scale, scale);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float number = fminf(fmaxf(__fmul_rn(__fsub_rn(x[u][i], low), scale), 0.0f), 15.0f);
-                        word += __float_as_uint(__fadd_rn(number, 12582912.0f)) << (4 * i);
+                    for (int i = 3; i >= 0; --i) {
+                        float2 number = __fmul2_rn(__fadd2_rn(make_float2(x[u][i], x[u][i + 4]), lows), scales);
+                        number = __fadd2_rn(make_float2(fmaxf(number.x, 0.0f), fmaxf(number.y, 0.0f)),
+                                            make_float2(12582912.0f, 12582912.0f));
+                        const uint32_t both = __byte_perm(__float_as_uint(number.x), __float_as_uint(number.y), 0x5410u);
+                        word = (word << 4) + __vminu2(both, 0x000F000Fu);
                     }
-                    word -= 0x4B400000u + 0xB4000000u + 0x40000000u;
                     const uint32_t value_word = exchange(word);
                     *reinterpret_cast<uint32_t*>(tiles[u] + at[u] * kKv4RowBytes + line_offset) =
                         is_value ? value_word : word;
@@ -317,9 +322,14 @@ __global__ void __launch_bounds__(kRowsThreads, 4) read_kernel(Kv4View view, int
                     // n as the low byte of 2^23 + n.  n * delta has 15 bits, so one rounding as two.
                     const uint32_t even = word & 0x0F0F0F0Fu, odd = word >> 4 & 0x0F0F0F0Fu;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const uint32_t bits = __byte_perm(i & 1 ? odd : even, 0x4B000000u, 0x7650u + (i >> 1));
-                        x[i] = __fmaf_rn(__fsub_rn(__uint_as_float(bits), 8388608.0f), delta, low);
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t two[2] = {__byte_perm(even, 0x4B000000u, 0x7650u + i),
+                                                 __byte_perm(odd, 0x4B000000u, 0x7650u + i)};
+                        const float2 n = __fadd2_rn(make_float2(__uint_as_float(two[0]), __uint_as_float(two[1])),
+                                                    make_float2(-8388608.0f, -8388608.0f));
+                        const float2 value = __ffma2_rn(n, make_float2(delta, delta), make_float2(low, low));
+                        x[2 * i] = value.x;
+                        x[2 * i + 1] = value.y;
                     }
                     store_eight(head_out + wide(token, token_size), x);
                 }
