@@ -3,8 +3,8 @@
 //
 // Of a group's values x: low = fp16(min), delta = fp16((max - low) * (1 / 15)), n = rint((x - low) *
 // (1 / delta)) within 0..15; a number stands for low + n * delta.  Both kernels are bound by
-// issue (216 and 129 warp instructions a token and head, at 65 and 64% issue): 8191 tokens of
-// 8 heads in bf16 take 32.2 us written and read back, against 13.4 us for the bytes.
+// issue and the loads' latency (187 and 110 warp instructions a token and head, at 61 and 58% issue): 8191 tokens of
+// 8 heads in bf16 take 30.2 us written and read back, against 13.4 us for the bytes.
 #include "kv4.cuh"
 
 namespace popkv {
@@ -170,7 +170,8 @@ __device__ __forceinline__ Rows rows_of(int head_shift) {
     return rows;
 }
 
-// Two rows of a warp at a time, so that one row's loads fly while the other is quantised.
+// Two rows of a warp at a time, so that one row's loads fly while the other is quantised (three or four, kept
+// as they are in memory, spill: 33.8 and 39.2 against 30.5 us; one, with 6 CTAs to an SM: 31.7).
 template <typename T, bool kVector>
 __global__ void __launch_bounds__(kRowsThreads, 4) write_kernel(
     Kv4View view, int layer, int head_shift, const int32_t* __restrict__ seqs, const int32_t* __restrict__ counts,
