@@ -160,15 +160,21 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const __grid_
     }
     best = block_best(best);
     __shared__ int is_last;
+    __shared__ unsigned long long winner;
     if (threadIdx.x == 0) {
         if (best) atomicMax(p.best + b, best);
         int before;
         asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.arrived + b) : "memory");
         is_last = before == static_cast<int>(gridDim.x) - 1;
+        if (is_last) {  // one thread reads the winner and clears the workspace, so that no warp reads it cleared
+            winner = __ldcg(p.best + b);
+            p.best[b] = 0;
+            p.arrived[b] = 0;
+        }
     }
     __syncthreads();
     if (!is_last) return;
-    best = __ldcg(p.best + b);
+    best = winner;
     if (refused && best == 0) {
         // p nowhere above q (rounding alone can do that): the target's row decides.
         for (int64_t v = threadIdx.x; v < p.vocab; v += kVerifyThreads) {
@@ -180,11 +186,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const __grid_
     const int64_t next = best ? static_cast<int64_t>(0xFFFFFFFFu - static_cast<uint32_t>(best)) : 0;
     for (int i = threadIdx.x; i <= p.drafts; i += kVerifyThreads)
         p.out[b * (p.drafts + 1) + i] = i < accepted ? tokens[i] : i == accepted ? next : -1;
-    if (threadIdx.x == 0) {
-        p.accepted[b] = accepted;
-        p.best[b] = 0;
-        p.arrived[b] = 0;
-    }
+    if (threadIdx.x == 0) p.accepted[b] = accepted;
 }
 
 template <typename T>

@@ -154,3 +154,30 @@ def test_refusals(cuda_device):
         verify_drafts(target, tokens, uniforms, noise, counts=torch.zeros(2, dtype=torch.int64, device=cuda_device))
     with pytest.raises(RuntimeError, match="CUDA device"):
         verify_drafts(target, tokens.cpu(), uniforms, noise)
+
+
+def many_drafts(n, drafts, vocab, device, seed):
+    """Inputs whose first refusal falls on a chosen place of each sequence, or on none."""
+    target, tokens, uniforms, noise, draft = inputs(n, drafts, vocab, torch.float32, device, seed)
+    places = [i * 7919 % (drafts + 1) if i % 3 else drafts - i // 3 % 4 for i in range(n)]
+    uniforms = torch.zeros_like(uniforms)
+    for i, place in enumerate(places):
+        if place < drafts:  # the draft's id of the largest q / p, which is above 1, and the largest u
+            tokens[i, place] = (draft[i, place] / target[i, place]).argmax()
+            uniforms[i, place] = 1 - 2.0 ** -24
+    return places, (target, tokens, uniforms, noise, draft)
+
+
+@pytest.mark.parametrize("drafts,n,vocab", [(31, 40, 700), (32, 40, 700), (32, 40, 9001), (33, 200, 515), (40, 500, 67), (100, 64, 516),
+                                            (1024, 5, 20)])
+@pytest.mark.parametrize("proposal", (True, False))
+def test_refusals_at_any_place_of_many_drafts(cuda_device, drafts, n, vocab, proposal):
+    """More drafts than a warp has lanes: every place may be refused, and every warp writes tokens."""
+    places, (target, tokens, uniforms, noise, draft) = many_drafts(n, drafts, vocab, cuda_device, drafts)
+    draft = draft if proposal else None
+    got, accepted = check(target, tokens, uniforms, noise, draft)
+    if proposal:
+        assert accepted.tolist() == places
+    for _ in range(30):
+        again = verify_drafts(target, tokens, uniforms, noise, draft_probs=draft)
+        assert torch.equal(again[0], got) and torch.equal(again[1], accepted)
