@@ -1058,8 +1058,9 @@ __global__ void __launch_bounds__(32 * Sizes<NG, NT, NC, kSelected, kWhole>::kWa
             __syncwarp();
         } else {
             for (int j = 0; j < copies.share.todo; ++j) {
-                if (!mbar_wait(&full[warp][next_slot], phase)) {
-                    // A copy did not arrive in time: no further copies, and a last chance for those in flight.
+                if (!__all_sync(0xFFFFFFFFu, mbar_wait(&full[warp][next_slot], phase))) {
+                    // A copy did not arrive in time for every lane (the warp decides as one: shuffles and products
+                    // follow): no further copies, and a last chance for those in flight.
                     failed = true;
                     for (int k = 0; k < kStages; ++k) mbar_wait(&full[warp][k], k > next_slot ? phase : phase ^ 1u);
                     break;

@@ -2,6 +2,8 @@
 from __future__ import annotations
 
 import ctypes
+import re
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -143,3 +145,11 @@ def test_verification_model_keeps_the_target_distribution():
         counts[out[0]] += 1
     want = p.astype(np.float64) * n
     assert (np.abs(counts - want) <= 5 * np.sqrt(want) + 1e-9).all()
+
+
+def test_waits_that_steer_a_warp_are_voted_on():
+    """A bounded wait ends lane by lane; a warp that goes on with shuffles and matrix products has to agree first."""
+    for name in ("kv4_attention.cu", "gemv.cu"):
+        text = (Path(kv4.__file__).parent / "csrc" / name).read_text()
+        assert "mbar_wait(" in text
+        assert not re.findall(r"(?:if|while)\s*\(\s*!?\s*mbar_wait\(|=\s*mbar_wait\(", text), name
