@@ -29,28 +29,29 @@ __device__ bool first_of(const Kv4View& view, const int32_t* seqs, int i) {
 }
 
 // Exclusive prefix sum over the block (kPlanThreads threads); *total for everybody.
-__device__ int block_scan(int value, int* total) {
-    __shared__ int sums[kPlanThreads / 32];
+template <typename T>
+__device__ T block_scan(T value, T* total) {
+    __shared__ T sums[kPlanThreads / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int inclusive = value;
+    T inclusive = value;
 #pragma unroll
     for (int step = 1; step < 32; step *= 2) {
-        const int other = __shfl_up_sync(0xFFFFFFFFu, inclusive, step);
+        const T other = __shfl_up_sync(0xFFFFFFFFu, inclusive, step);
         if (lane >= step) inclusive += other;
     }
     if (lane == 31) sums[warp] = inclusive;
     __syncthreads();
     if (warp == 0) {
-        int s = sums[lane];
+        T s = sums[lane];
 #pragma unroll
         for (int step = 1; step < 32; step *= 2) {
-            const int other = __shfl_up_sync(0xFFFFFFFFu, s, step);
+            const T other = __shfl_up_sync(0xFFFFFFFFu, s, step);
             if (lane >= step) s += other;
         }
         sums[lane] = s;
     }
     __syncthreads();
-    const int before = warp ? sums[warp - 1] : 0;
+    const T before = warp ? sums[warp - 1] : 0;
     *total = sums[kPlanThreads / 32 - 1];
     __syncthreads();
     return before + inclusive - value;
@@ -109,14 +110,16 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Kv4View view, cons
                 if (ids[i] != -1) atomicOr(view.status, kKv4StatusSequence);
             }
         }
-        int total;
-        const int before = block_scan(max(need, 0), &total);
+        // 64 bits: 1024 entries may need 2^26 pages each.  Past the pool's end the first pages do not matter.
+        const int64_t most = view.num_pages + 1ll;
+        int64_t total;
+        const int64_t before = block_scan(static_cast<int64_t>(max(need, 0)), &total);
         if (i < n) {
-            first[i] = needed + before;
+            first[i] = static_cast<int>(min(needed + before, most));
             copies[i] = copied;
             needs[i] = need;  // -1: not an entry to extend
         }
-        needed = min(needed + total, view.num_pages + 1);
+        needed = static_cast<int>(min(needed + total, most));
     }
 
     // The lowest free pages, in order.
@@ -126,7 +129,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Kv4View view, cons
         const bool is_free = refs_ahead == 0;
         refs_ahead = next < view.num_pages ? view.refs[next] : 1;
         int total;
-        const int at = free_pages + block_scan(is_free, &total);
+        const int at = free_pages + block_scan<int>(is_free, &total);
         if (is_free && at < needed) found[at] = p;
         free_pages += total;
     }
@@ -263,7 +266,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_kernel(Kv4View view, int
     for (int base = 0; base < view.num_pages; base += kPlanThreads) {
         const int p = base + threadIdx.x;
         int total;
-        block_scan(p < view.num_pages && view.refs[p] > 0, &total);
+        block_scan<int>(p < view.num_pages && view.refs[p] > 0, &total);
         live += total;
     }
     int moved = 0, holes = 0;
@@ -272,9 +275,9 @@ __global__ void __launch_bounds__(kPlanThreads) compact_kernel(Kv4View view, int
         const bool used = p < view.num_pages && view.refs[p] > 0;
         const bool moves = used && p >= live, hole = p < live && !used;
         int total;
-        const int at = moved + block_scan(moves, &total);
+        const int at = moved + block_scan<int>(moves, &total);
         moved += total;
-        const int into = holes + block_scan(hole, &total);
+        const int into = holes + block_scan<int>(hole, &total);
         holes += total;
         if (moves) source[at] = p;
         if (hole) target[into] = p;

@@ -614,6 +614,21 @@ def test_empty_calls(cuda_device):
     host.same(cache)
 
 
+def test_extend_adds_pages_up_in_64_bits(cuda_device):
+    """32 sequences that ask for 2^30 tokens each: 2^31 pages, which 32 bits would take for none."""
+    cache = Kv4Cache(64, kv_heads=1, max_seqs=32, max_tokens=1 << 30, page_size=16, dim_group_size=128,
+                     device=cuda_device)
+    seqs = torch.arange(32, dtype=torch.int32, device=cuda_device)
+    cache.extend(seqs, 1 << 30)
+    with pytest.raises(RuntimeError, match="too few free pages"):
+        cache.check()
+    assert cache.free_pages() == 64 and not cache.lengths.any()
+    assert int(cache.table.min()) == -1 == int(cache.table.max())
+    cache.extend(seqs, 17)
+    cache.check()
+    assert cache.free_pages() == 0 and cache.table[:, :2].flatten().tolist() == list(range(64))
+
+
 # -- refusals -----------------------------------------------------------------------
 def test_refusals(cuda_device):
     cache = make(cuda_device, [5, 6])
