@@ -673,7 +673,8 @@ typedef struct popkv_kv4_cache {
     int64_t max_pages;
 } popkv_kv4_cache;
 
-#define POPKV_KV4_FULL 1     /* an extend found too few free pages or table columns, and did nothing */
+#define POPKV_KV4_FULL 1     /* an extend found too few free pages or table columns, and did nothing; until the
+                                caller clears the bit, extends and writes do nothing */
 #define POPKV_KV4_SEQUENCE 2 /* a sequence id was out of range or repeated; its entry was skipped */
 #define POPKV_KV4_WAIT 4     /* an attention's bounded wait for its copies gave up: its output is incomplete */
 
@@ -685,6 +686,8 @@ typedef struct popkv_kv4_cache {
  * rounded to fp16; n = rint((x - low) * (1 / delta)) in fp32, within 0..15.  NaN is
  * stored as 0 and magnitudes past 65504 as 65504.  The pages must belong to the
  * sequence alone (popkv_kv4_extend sees to it), and no sequence be listed twice.
+ * While POPKV_KV4_FULL is set nothing is written: the tokens have no room, and the last
+ * ones held are others, maybe in pages that other sequences share.
  */
 POPKV_API int popkv_kv4_write(const popkv_kv4_cache* cache, int64_t layer, const int32_t* seqs, int64_t n,
                               const int32_t* counts, const void* keys, const void* values, int dtype,
@@ -738,8 +741,10 @@ POPKV_API int popkv_kv4_attention_selected(const popkv_kv4_cache* cache, int64_t
  *
  * popkv_kv4_extend: room for counts[i] (NULL: `count`) more tokens of each listed
  *   sequence; lengths grow.  A last page that is partly filled and shared is copied
- *   first, in every layer.  All or nothing: with too few free pages or table columns it
- *   sets POPKV_KV4_FULL and changes nothing else.  workspace: num_pages + 3 n.
+ *   first, in every layer.  All or nothing: with too few free pages or table columns, or
+ *   POPKV_KV4_FULL set already, it sets POPKV_KV4_FULL and changes nothing else.  Every listed
+ *   holder of a shared page copies it, so that even where all of them are listed the pool needs
+ *   a page for each.  workspace: num_pages + 3 n.
  * popkv_kv4_fork: children take their parents' tokens, sharing the pages, and give back
  *   their own; every parent is read before any child changes, so one call can reorder
  *   beams.  workspace: n * (1 + max_pages).

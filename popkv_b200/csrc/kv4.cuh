@@ -23,7 +23,8 @@ constexpr int kKv4RowBytes = 64;                                  // 128 dims of
 constexpr int kKv4ValueOffset = kKv4TileTokens * kKv4RowBytes;    // within a tile
 constexpr int kKv4PairOffset = 2 * kKv4ValueOffset;
 
-constexpr int kKv4StatusFull = 1;     // status[0]: an extend found too few free pages or table columns
+constexpr int kKv4StatusFull = 1;     // status[0]: an extend found too few free pages or table columns; extends and
+                                      // writes do nothing while it is set
 constexpr int kKv4StatusWait = 4;     // status[0]: an attention's wait for its copies gave up
 constexpr int kKv4StatusSequence = 2; // status[0]: a sequence or page id was out of range or repeated
 

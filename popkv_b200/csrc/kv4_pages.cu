@@ -78,7 +78,9 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Kv4View view, cons
     const int size = view.page_size();
     int refs_ahead = threadIdx.x < view.num_pages ? view.refs[threadIdx.x] : 1;
     for (int i = threadIdx.x; i < n; i += kPlanThreads) ids[i] = seqs[i];
-    if (threadIdx.x == 0) short_of_columns = 0;
+    // After an extend that found no room none succeeds until the caller has seen it: the tokens in between would be
+    // missing from the sequence.
+    if (threadIdx.x == 0) short_of_columns = view.status[0] & kKv4StatusFull;
     __syncthreads();
 
     // Pages that each entry needs: those its tokens reach, and one for the copy of
@@ -134,7 +136,7 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Kv4View view, cons
         free_pages += total;
     }
     __syncthreads();
-    if (short_of_columns || free_pages < needed) {  // all or nothing
+    if (short_of_columns || free_pages < needed) {  // all or nothing, and no writes until the bit is cleared
         for (int i = threadIdx.x; i < n; i += kPlanThreads) source[i] = -1;
         if (threadIdx.x == 0) atomicOr(view.status, kKv4StatusFull);
         return;

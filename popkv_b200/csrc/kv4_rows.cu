@@ -193,12 +193,14 @@ __global__ void __launch_bounds__(kRowsThreads, 4) write_kernel(
     const int page_mask = view.page_size() - 1, tile_bytes = view.tile_bytes();
     const uint32_t page_bytes = static_cast<uint32_t>(view.page_bytes);
     constexpr int kTogether = 2;
+    // An extend found no room, so the last tokens are not the ones to be written, and their pages may be shared.
+    const bool refused = view.status[0] & kKv4StatusFull;
 #pragma unroll 1
     for (int entry = blockIdx.y; entry < n; entry += gridDim.y) {
         const int seq = seqs[entry];
         const int count = counts ? min(counts[entry], tokens) : tokens;
         const int length = view.length_of(seq), offset = length - count;
-        if (length == 0) continue;  // an id out of range among them
+        if (length == 0 || refused) continue;  // an id out of range among them
         const int32_t* pages_of_seq = view.table + static_cast<int64_t>(seq) * view.max_pages;
         const T* rows_of_entry = rows_at + entry * seq_stride;
 #pragma unroll 1

@@ -21,7 +21,9 @@ says how many stay, and ``truncate`` drops the rest.
 
 The reference keeps a contiguous 16-bit cache of one sequence (popkv.py:965-972) and has no
 counterpart.  The byte layout is documented in ``include/popkv_b200.h``.  Sequence ids of -1
-are padding; ids out of range or repeated set an error bit that ``check`` raises on.
+are padding; ids out of range or repeated set an error bit that ``check`` raises on.  After an
+``extend`` that found no room, ``extend`` and ``write`` do nothing until ``check`` has raised: the
+cache stays as it was before that step, which can be repeated once pages are free.
 
 Streams: calls run on the current stream of the cache's device.  Calls on one cache that
 overlap in time must be ordered by the caller when one of them writes.
@@ -204,7 +206,8 @@ class Kv4Cache:
         keys, values: fp32/fp16/bf16 [n, tokens, kv_heads, 128], or [n, kv_heads, 128] for one
         token; any strides with contiguous dims (slices of a fused projection).  They are the
         last ``tokens`` (or ``counts[i]`` <= tokens, the first of the row's) of sequence
-        ``seqs[i]`` (each listed once), for which ``extend`` has made room.
+        ``seqs[i]`` (each listed once), for which ``extend`` has made room.  After an ``extend`` that
+        found none nothing is written until ``check`` has raised.
         """
         if keys.ndim == 3 and values.ndim == 3:
             keys, values = keys.unsqueeze(1), values.unsqueeze(1)
@@ -369,8 +372,9 @@ class Kv4Cache:
         """Room for ``tokens`` (an int, or int32 [n]) more tokens of each listed sequence.
 
         Takes the lowest free pages; a last page that is partly filled and shared with another
-        sequence is copied first, in every layer.  All or nothing: without enough free pages
-        nothing changes and ``check`` raises.
+        sequence is copied first, in every layer (by every listed holder, even where all of them are
+        listed).  All or nothing: without enough free pages nothing changes, further extends and
+        writes do nothing either, and ``check`` raises.
         """
         seqs, n = self._sequences(seqs)
         counts, count = None, 0

@@ -629,6 +629,51 @@ def test_extend_adds_pages_up_in_64_bits(cuda_device):
     assert cache.free_pages() == 0 and cache.table[:, :2].flatten().tolist() == list(range(64))
 
 
+def test_nothing_is_written_after_a_failed_extend(cuda_device):
+    """Branches of a pool that is too full for their copies: the shared page keeps its bytes, and the step can be repeated."""
+    cache = filled(cuda_device, 4)
+    cache.extend([0], 40)
+    cache.fork([0, 0], [1, 2])
+    cache.check()
+    host = R.HostCache.like(cache)
+    x = torch.randn(2, 2, 1, 2, 128, generator=torch.Generator().manual_seed(1))
+    keys, values = x.to(cuda_device)
+    cache.extend([1, 2], 1)  # two copies, one free page
+    for layer in range(2):
+        cache.write(keys, values, seqs=[1, 2], layer=layer)
+    cache.extend([1], 1)  # would fit, but a step that failed is not known yet
+    for layer in range(2):
+        cache.write(keys[:1], values[:1], seqs=[1], layer=layer)
+    host.same(cache)
+    cache.free([2])
+    host.truncate([2], [0])
+    with pytest.raises(RuntimeError, match="too few free pages"):
+        cache.check()
+    host.same(cache)
+    assert host.extend([1], [1])
+    cache.extend([1], 1)
+    for layer in range(2):
+        cache.write(keys[:1], values[:1], seqs=[1], layer=layer)
+        for h in range(2):
+            host.put(layer, 1, h, 40, x[0, 0, 0, h].numpy(), x[1, 0, 0, h].numpy())
+    cache.check()
+    host.same(cache)
+
+
+def test_other_errors_do_not_hold_writes_back(cuda_device):
+    cache = filled(cuda_device, 8)
+    cache.extend([0, 0, 77], 20)
+    host = R.HostCache.like(cache)
+    x = torch.randn(1, 20, 2, 128, generator=torch.Generator().manual_seed(2))
+    cache.write(x.to(cuda_device), -x.to(cuda_device), seqs=[0])
+    for t in range(20):
+        for h in range(2):
+            host.put(0, 0, h, t, x[0, t, h].numpy(), -x[0, t, h].numpy())
+    host.same(cache)
+    with pytest.raises(RuntimeError, match="out of range or repeated"):
+        cache.check()
+
+
 # -- refusals -----------------------------------------------------------------------
 def test_refusals(cuda_device):
     cache = make(cuda_device, [5, 6])
