@@ -36,7 +36,7 @@ class Kv4Decoder:
 
     Args:
         weights: the model (bf16).
-        max_seqs, max_tokens: slots, and most tokens of one.
+        max_seqs, max_tokens: slots, and most tokens of one (rounded up to whole pages).
         num_pages: pages of the pool; default enough for every slot at full length.
         retrieval: dense layers, budget and group sizes of the sparse layers' PopKV selection
             (single-token steps only); None: every layer attends over all tokens.
@@ -56,8 +56,8 @@ class Kv4Decoder:
         self.cache = Kv4Cache(pages if num_pages is None else num_pages, kv_heads=cfg.num_key_value_heads,
                               layers=cfg.num_hidden_layers, max_seqs=max_seqs, max_tokens=max_tokens,
                               page_size=page_size, dim_group_size=dim_group_size, device=self.device)
-        self.max_tokens = max_tokens
-        self.cos, self.sin = rope_tables(cfg, max_tokens, self.device)
+        self.max_tokens = self.cache.max_pages * page_size  # every token that the cache has room for has its position
+        self.cos, self.sin = rope_tables(cfg, self.max_tokens, self.device)
         self.generator = torch.Generator(device=self.device).manual_seed(seed)
         group = cfg.num_attention_heads // cfg.num_key_value_heads
         self.head_to_kv = torch.arange(cfg.num_attention_heads, device=self.device) // group

@@ -130,6 +130,33 @@ def test_a_full_pool_is_reported(weights):
         d.prefill(1, prompt(40))
 
 
+def test_room_past_max_tokens_is_room(weights, cuda_device):
+    """The cache's room is whole pages: tokens of the last page have positions of their own."""
+    short, long = Kv4Decoder(weights, max_seqs=1, max_tokens=200), Kv4Decoder(weights, max_seqs=1, max_tokens=256)
+    assert short.max_tokens == long.max_tokens == 256
+    for d in (short, long):
+        d.prefill(0, prompt(199))
+    slot = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    tokens = torch.randint(0, 503, (1, 57), generator=torch.Generator().manual_seed(4)).to(cuda_device)
+    assert torch.equal(short.forward(slot, tokens[:, :40]), long.forward(slot, tokens[:, :40]))
+    assert torch.equal(short.forward(slot, tokens[:, 40:]), long.forward(slot, tokens[:, 40:]))
+    assert short.cache.lengths.tolist() == [256]
+    whole = Kv4Decoder(weights, max_seqs=1, max_tokens=200)
+    assert torch.equal(whole.prefill(0, prompt(256)), long.prefill(0, prompt(256)))
+    with pytest.raises(RuntimeError, match="table columns"):
+        whole.prefill(0, prompt(257))
+
+
+def test_room_of_the_sparse_layers_planes(weights, cuda_device):
+    d = Kv4Decoder(weights, max_seqs=1, max_tokens=50, page_size=32,
+                   retrieval=RetrievalConfig(budget=16, full_layers=(0,)))
+    d.prefill(0, prompt(60))
+    slot = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    for i in range(4):
+        assert torch.isfinite(d.forward(slot, torch.full((1, 1), i, device=cuda_device))).all()
+    assert d.cache.lengths.tolist() == [64]
+
+
 def test_the_command_runs(cuda_device, capsys):
     main()
     text = capsys.readouterr().out

@@ -630,7 +630,7 @@ def test_extend_adds_pages_up_in_64_bits(cuda_device):
 
 
 def test_nothing_is_written_after_a_failed_extend(cuda_device):
-    """Branches of a pool that is too full for their copies: the shared page keeps its bytes, and the step can be repeated."""
+    """Branches of a pool too full for their copies: the shared page keeps its bytes, and the step can be repeated."""
     cache = filled(cuda_device, 4)
     cache.extend([0], 40)
     cache.fork([0, 0], [1, 2])
