@@ -108,8 +108,13 @@ class Kv4Decoder:
 
     @torch.inference_mode()
     def forward(self, slots: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
-        """Append tokens [n, T] to the slots (int32 [n]); returns the logits [n, T, V] after each."""
+        """Append tokens [n, T] to the slots (int32 [n]); returns the logits [n, T, V] after each.
+
+        With sparse layers T is 1.
+        """
         n, count = tokens.shape
+        if self.sparse_layers and count != 1:
+            raise ValueError("the sparse layers take one token a step")
         positions = self.cache.lengths[slots.long()].long()[:, None] + torch.arange(count, device=self.device)
         self.cache.extend(slots, count)
         hidden = self.weights.embed[tokens]

@@ -157,6 +157,19 @@ def test_room_of_the_sparse_layers_planes(weights, cuda_device):
     assert d.cache.lengths.tolist() == [64]
 
 
+def test_sparse_layers_refuse_several_tokens(weights, cuda_device):
+    d = Kv4Decoder(weights, max_seqs=2, max_tokens=100, retrieval=RetrievalConfig(budget=16, full_layers=(0,)))
+    d.prefill(0, prompt(30))
+    slots = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    for count in (0, 2, 3):
+        with pytest.raises(ValueError, match="one token a step"):
+            d.forward(slots, torch.ones((1, count), dtype=torch.int64, device=cuda_device))
+    assert d.cache.lengths.tolist() == [30, 0]
+    assert all(p.token_count == 30 for p in d.planes.values())
+    d.forward(slots, torch.ones((1, 1), dtype=torch.int64, device=cuda_device))
+    assert d.cache.lengths.tolist() == [31, 0] and all(p.token_count == 31 for p in d.planes.values())
+
+
 def test_the_command_runs(cuda_device, capsys):
     main()
     text = capsys.readouterr().out
