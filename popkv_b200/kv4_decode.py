@@ -110,13 +110,20 @@ class Kv4Decoder:
     def forward(self, slots: torch.Tensor, tokens: torch.Tensor) -> torch.Tensor:
         """Append tokens [n, T] to the slots (int32 [n]); returns the logits [n, T, V] after each.
 
-        With sparse layers T is 1.
+        With sparse layers T is 1.  Where there is no room it raises before anything is written, with
+        every slot as it was (this synchronises).
         """
         n, count = tokens.shape
         if self.sparse_layers and count != 1:
             raise ValueError("the sparse layers take one token a step")
-        positions = self.cache.lengths[slots.long()].long()[:, None] + torch.arange(count, device=self.device)
+        held = self.cache.lengths[slots.long()]
+        positions = held.long()[:, None] + torch.arange(count, device=self.device)
         self.cache.extend(slots, count)
+        try:
+            self.cache.check()
+        except RuntimeError:
+            self._back_to(slots, held)
+            raise
         hidden = self.weights.embed[tokens]
         for l, layer in enumerate(self.weights.layers):
             q, k, v = self._project(layer, hidden, positions.clamp_max(self.max_tokens - 1))
@@ -127,6 +134,11 @@ class Kv4Decoder:
                 attn = self.cache.attention(q, seqs=slots, layer=l)
             hidden = self._mlp(layer, hidden, attn)
         return self._logits(hidden)
+
+    def _back_to(self, slots: torch.Tensor, held: torch.Tensor) -> None:
+        """Take the slots back to their first ``held`` tokens, after an error that has been raised."""
+        self.cache.truncate(slots, held)
+        self.cache.status[0] = 0  # ids that the error was about are among them once more
 
     def _selected(self, slot: int, layer: int, query: torch.Tensor, key: torch.Tensor) -> torch.Tensor:
         """A sparse layer's attention [QH, D] of a slot's newest token, which its planes do not hold yet."""
@@ -172,7 +184,8 @@ class Kv4Decoder:
         """Decode at least ``steps`` tokens in every slot, after the tokens ``first`` [n] that follow
         their prompts.  ``draft``: a model whose slots of the same numbers hold the same tokens, which
         proposes ``drafts`` tokens a step.  Returns each slot's tokens (``first`` included) and the
-        tokens a slot gained per step.
+        tokens a slot gained per step.  A step without room raises and leaves both models' slots as the
+        step before left them.
         """
         if draft is not None and (self.sparse_layers or draft.sparse_layers):
             raise ValueError("drafted tokens need dense attention: the sparse layers take one token a step")
@@ -189,13 +202,17 @@ class Kv4Decoder:
             else:
                 base = self.cache.lengths[seqs.long()].clone()
                 proposed, proposals, token = [], [], pending
-                for _ in range(drafts):
-                    token, probs = draft.sample(draft.forward(seqs, token[:, None])[:, 0], temperature)
-                    proposed.append(token)
-                    proposals.append(probs)
-                draft.forward(seqs, token[:, None])  # the last draft's keys and values
-                proposed, proposals = torch.stack(proposed, 1), torch.stack(proposals, 1)
-                logits = self.forward(seqs, torch.cat([pending[:, None], proposed], 1))
+                try:
+                    for _ in range(drafts):
+                        token, probs = draft.sample(draft.forward(seqs, token[:, None])[:, 0], temperature)
+                        proposed.append(token)
+                        proposals.append(probs)
+                    draft.forward(seqs, token[:, None])  # the last draft's keys and values
+                    proposed, proposals = torch.stack(proposed, 1), torch.stack(proposals, 1)
+                    logits = self.forward(seqs, torch.cat([pending[:, None], proposed], 1))
+                except RuntimeError:
+                    draft._back_to(seqs, base)  # where the target's slots are
+                    raise
                 uniforms = torch.rand((n, drafts), device=self.device, generator=self.generator)
                 kept, accepted = verify_drafts((logits / temperature).softmax(-1), proposed, uniforms, self._noise(n),
                                                draft_probs=proposals)

@@ -170,6 +170,43 @@ def test_sparse_layers_refuse_several_tokens(weights, cuda_device):
     assert d.cache.lengths.tolist() == [31, 0] and all(p.token_count == 31 for p in d.planes.values())
 
 
+def test_a_step_without_room_changes_nothing(weights, cuda_device):
+    """Branches that find no page for their copies: the prompt they share stays, and the step can be repeated."""
+    for retrieval in (None, RetrievalConfig(budget=16, full_layers=(0,))):
+        d, other = (Kv4Decoder(weights, max_seqs=3, max_tokens=64, num_pages=n, page_size=16, retrieval=retrieval)
+                    for n in (4, 12))
+        for x in (d, other):
+            x.prefill(0, prompt(40))
+            x.fork(0, [1, 2])
+        pages, tables = d.cache.pages.clone(), d.cache.tables.clone()
+        slots = torch.tensor([1, 2], dtype=torch.int32, device=cuda_device)
+        token = torch.full((2, 1), 9, device=cuda_device)
+        with pytest.raises(RuntimeError, match="too few free pages"):
+            d.forward(slots, token)
+        assert torch.equal(d.cache.pages, pages) and torch.equal(d.cache.tables, tables)
+        assert all(p.token_count == 40 for p in d.planes.values())
+        d.release([2])
+        assert near(d.forward(slots[:1], token[:1]), other.forward(slots[:1], token[:1]))
+        assert d.cache.lengths.tolist() == [40, 41, 0]
+
+
+@pytest.mark.parametrize("short_of", ("target", "draft"))
+def test_generate_without_room_leaves_both_caches_alike(weights, short_of):
+    """The target's and the draft's slots hold the same tokens after a step that one of them had no room for."""
+    room = {"target": 5, "draft": 5, short_of: 3}
+    target, draft = (Kv4Decoder(weights, max_seqs=1, max_tokens=80, page_size=16, num_pages=room[who], seed=s)
+                     for s, who in enumerate(("target", "draft")))
+    logits = target.prefill(0, prompt(40))
+    draft.prefill(0, prompt(40))
+    first, _ = target.sample(logits[None])
+    with pytest.raises(RuntimeError, match="too few free pages"):
+        target.generate([0], first, 30, draft=draft, drafts=3)
+    held = target.cache.lengths.tolist()
+    assert held == draft.cache.lengths.tolist() and 40 < held[0] <= 48
+    target.cache.check()
+    draft.cache.check()
+
+
 def test_the_command_runs(cuda_device, capsys):
     main()
     text = capsys.readouterr().out
