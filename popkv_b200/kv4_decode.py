@@ -88,6 +88,8 @@ class Kv4Decoder:
         """Run a prompt [T] through the model into an empty slot; returns the last token's logits [V]."""
         tokens = int(ids.shape[0])
         seqs = [slot]
+        for l in self.sparse_layers:
+            self.planes.pop((slot, l), None)
         self.cache.free(seqs)
         self.cache.extend(seqs, tokens)
         self.cache.check()
@@ -116,7 +118,10 @@ class Kv4Decoder:
         n, count = tokens.shape
         if self.sparse_layers and count != 1:
             raise ValueError("the sparse layers take one token a step")
-        held = self.cache.lengths[slots.long()]
+        listed = slots.tolist() if self.sparse_layers else []
+        if any((s, l) not in self.planes for s in listed for l in self.sparse_layers):
+            raise ValueError("a slot has no prompt")
+        held = self._held(slots)
         positions = held.long()[:, None] + torch.arange(count, device=self.device)
         self.cache.extend(slots, count)
         try:
@@ -129,11 +134,15 @@ class Kv4Decoder:
             q, k, v = self._project(layer, hidden, positions.clamp_max(self.max_tokens - 1))
             self.cache.write(k, v, seqs=slots, layer=l)
             if l in self.sparse_layers:
-                attn = torch.stack([self._selected(s, l, q[i, 0], k[i, 0]) for i, s in enumerate(slots.tolist())])[:, None]
+                attn = torch.stack([self._selected(s, l, q[i, 0], k[i, 0]) for i, s in enumerate(listed)])[:, None]
             else:
                 attn = self.cache.attention(q, seqs=slots, layer=l)
             hidden = self._mlp(layer, hidden, attn)
         return self._logits(hidden)
+
+    def _held(self, slots: torch.Tensor) -> torch.Tensor:
+        """Tokens of each slot (of an id that is none, whatever: the cache refuses it)."""
+        return self.cache.lengths[slots.long().clamp(0, self.cache.max_seqs - 1)]
 
     def _back_to(self, slots: torch.Tensor, held: torch.Tensor) -> None:
         """Take the slots back to their first ``held`` tokens, after an error that has been raised."""
@@ -200,7 +209,7 @@ class Kv4Decoder:
                 pending, _ = self.sample(self.forward(seqs, pending[:, None])[:, 0], temperature)
                 kept = pending[:, None]
             else:
-                base = self.cache.lengths[seqs.long()].clone()
+                base = self._held(seqs)
                 proposed, proposals, token = [], [], pending
                 try:
                     for _ in range(drafts):

@@ -207,6 +207,35 @@ def test_generate_without_room_leaves_both_caches_alike(weights, short_of):
     draft.cache.check()
 
 
+def test_slots_out_of_range_are_refused(weights, cuda_device):
+    """An id that is no slot raises, and the other slots of the call keep what they held."""
+    for retrieval in (None, RetrievalConfig(budget=16, full_layers=(0,))):
+        d = Kv4Decoder(weights, max_seqs=3, max_tokens=100, retrieval=retrieval)
+        for s in range(2):
+            d.prefill(s, prompt(30 + s))
+        pages = d.cache.pages.clone()
+        for bad in (7, -3, 1 << 30):
+            with pytest.raises((RuntimeError, ValueError), match="out of range or repeated|no prompt"):
+                d.forward(torch.tensor([1, bad], dtype=torch.int32, device=cuda_device),
+                          torch.zeros((2, 1), dtype=torch.int64, device=cuda_device))
+            assert d.cache.lengths.tolist() == [30, 31, 0] and torch.equal(d.cache.pages, pages)
+        with pytest.raises((RuntimeError, ValueError), match="out of range or repeated|no prompt"):
+            d.generate([0, 9], torch.tensor([1, 2]), 3)
+        assert d.cache.lengths.tolist() == [30, 31, 0]
+
+
+def test_a_prompt_without_room_leaves_no_planes(weights, cuda_device):
+    d = Kv4Decoder(weights, max_seqs=1, max_tokens=64, page_size=16,
+                   retrieval=RetrievalConfig(budget=16, full_layers=(0,)))
+    d.prefill(0, prompt(40))
+    with pytest.raises(RuntimeError, match="table columns"):
+        d.prefill(0, prompt(65))
+    with pytest.raises(ValueError, match="no prompt"):
+        d.forward(torch.zeros(1, dtype=torch.int32, device=cuda_device), torch.zeros((1, 1), dtype=torch.int64,
+                                                                                     device=cuda_device))
+    assert d.cache.lengths.tolist() == [0]
+
+
 def test_the_command_runs(cuda_device, capsys):
     main()
     text = capsys.readouterr().out
