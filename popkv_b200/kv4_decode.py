@@ -52,7 +52,11 @@ class Kv4Decoder:
             retrieval.validate()
         self.weights, self.cfg, self.retrieval = weights, cfg, retrieval
         self.device = weights.embed.device
-        pages = max_seqs * -(-max_tokens // page_size)
+        pages = -(-max_tokens // page_size) * max_seqs
+        if pages == max_seqs:
+            # Slots that share their only page all copy it before it is free: one page more for every two at most.
+            # With more pages a slot, sharing the others saves at least as many.
+            pages += max_seqs // 2
         self.cache = Kv4Cache(pages if num_pages is None else num_pages, kv_heads=cfg.num_key_value_heads,
                               layers=cfg.num_hidden_layers, max_seqs=max_seqs, max_tokens=max_tokens,
                               page_size=page_size, dim_group_size=dim_group_size, device=self.device)

@@ -236,6 +236,23 @@ def test_a_prompt_without_room_leaves_no_planes(weights, cuda_device):
     assert d.cache.lengths.tolist() == [0]
 
 
+def test_the_default_pool_has_room_for_every_slots_copies(weights, cuda_device):
+    """Slots that share their last page, two by two or all four, extend together: a step copies it for each."""
+    for pairs, room, held in ((True, 16, 9), (False, 16, 9), (True, 32, 20), (False, 32, 20), (True, 32, 9)):
+        d = Kv4Decoder(weights, max_seqs=4, max_tokens=room, page_size=16)
+        for s in (0, 2) if pairs else (0,):
+            d.prefill(s, prompt(held, s))
+        if pairs:
+            d.fork(0, [1])
+            d.fork(2, [3])
+        else:
+            d.fork(0, [1, 2, 3])
+        slots = torch.arange(4, dtype=torch.int32, device=cuda_device)
+        for i in range(room - held):
+            d.forward(slots, torch.full((4, 1), i, device=cuda_device))
+        assert d.cache.lengths.tolist() == [room] * 4
+
+
 def test_the_command_runs(cuda_device, capsys):
     main()
     text = capsys.readouterr().out
