@@ -180,15 +180,20 @@ class Kv4Decoder:
             del self.planes[key]
 
     # -- decoding ------------------------------------------------------------------
-    def _noise(self, n: int) -> torch.Tensor:
-        return torch.empty((n, self.cfg.vocab_size), device=self.device).exponential_(generator=self.generator)
+    def _noise(self, n: int, generator: torch.Generator | None = None) -> torch.Tensor:
+        return torch.empty((n, self.cfg.vocab_size), device=self.device).exponential_(
+            generator=self.generator if generator is None else generator)
 
-    def sample(self, logits: torch.Tensor, temperature: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
-        """Tokens [n] drawn from logits [n, V], and the probabilities [n, V] that they were drawn from."""
+    def sample(self, logits: torch.Tensor, temperature: float = 1.0,
+               generator: torch.Generator | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """Tokens [n] drawn from logits [n, V], and the probabilities [n, V] that they were drawn from.
+
+        generator: of the random numbers, instead of the decoder's own.
+        """
         probs = (logits / temperature).softmax(-1)
         n = probs.shape[0]
         none = torch.empty((n, 0), device=self.device)
-        tokens, _ = verify_drafts(probs[:, None], none.long(), none, self._noise(n))
+        tokens, _ = verify_drafts(probs[:, None], none.long(), none, self._noise(n, generator))
         return tokens[:, 0], probs
 
     @torch.inference_mode()
@@ -217,7 +222,10 @@ class Kv4Decoder:
                 proposed, proposals, token = [], [], pending
                 try:
                     for _ in range(drafts):
-                        token, probs = draft.sample(draft.forward(seqs, token[:, None])[:, 0], temperature)
+                        # The target's random numbers: the draft's own may be the same as those that
+                        # verify it (equal seeds), and the two have to be independent.
+                        token, probs = draft.sample(draft.forward(seqs, token[:, None])[:, 0], temperature,
+                                                    self.generator)
                         proposed.append(token)
                         proposals.append(probs)
                     draft.forward(seqs, token[:, None])  # the last draft's keys and values

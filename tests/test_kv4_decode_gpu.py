@@ -253,6 +253,66 @@ def test_the_default_pool_has_room_for_every_slots_copies(weights, cuda_device):
         assert d.cache.lengths.tolist() == [room] * 4
 
 
+def test_generate_draws_independent_numbers(weights, monkeypatch):
+    """Decoders of the same (default) seed: no random number decides a draft and its verification both."""
+    target, draft = (Kv4Decoder(weights, max_seqs=2, max_tokens=200) for _ in range(2))
+    for d in (target, draft):
+        for s in range(2):
+            d.prefill(s, prompt(30))
+    drawn = []
+    noise, uniform = Kv4Decoder._noise, torch.rand
+
+    def noise_kept(self, *args):
+        drawn.append(noise(self, *args))
+        return drawn[-1]
+
+    def uniform_kept(*args, **kwargs):
+        out = uniform(*args, **kwargs)
+        drawn.append(-torch.log1p(-out))
+        drawn.append(-torch.log(out))  # either way to exponential numbers
+        return out
+
+    monkeypatch.setattr(Kv4Decoder, "_noise", noise_kept)
+    monkeypatch.setattr(torch, "rand", uniform_kept)
+    first, _ = target.sample(torch.zeros((2, 503), device=target.device))
+    target.generate([0, 1], first, 20, draft=draft, drafts=3)
+    assert len(drawn) > 20
+    for i, a in enumerate(drawn):
+        for b in drawn[:i]:
+            if a.shape == b.shape and a.shape[1] == 503:
+                # Independent fp32 numbers are equal in about one of 10^7 places.
+                assert float((a == b).float().mean()) < 0.01
+
+
+def test_generated_tokens_are_the_targets(cuda_device):
+    """First new tokens of many branches through generate, default seeds, a draft model of its own: the target's
+    probabilities within five deviations, and a bf16 rounding or two of the logits (2% of a probability)."""
+    config = replace(CONFIG, vocab_size=12)
+    target = Kv4Decoder(LlamaWeights.random(config, device=cuda_device, std=0.08, seed=5), max_seqs=64, max_tokens=64)
+    draft = Kv4Decoder(LlamaWeights.random(replace(config, num_hidden_layers=1), device=cuda_device, std=0.08, seed=6),
+                       max_seqs=64, max_tokens=64)
+    ids = torch.randint(0, 12, (20,), generator=torch.Generator().manual_seed(0))
+    slots = torch.arange(64, dtype=torch.int32, device=cuda_device)
+    for d in (target, draft):
+        d.prefill(0, ids)
+        d.fork(0, list(range(1, 64)))
+    lengths = torch.full((64,), 20, device=cuda_device)
+    first = torch.full((64,), 3, device=cuda_device)
+    logits = target.forward(slots, torch.stack([first, first, first], 1))
+    p = logits[0, 0].double().softmax(-1).cpu()
+    target.cache.truncate(slots, lengths)
+    counts = torch.zeros(12, dtype=torch.float64)
+    steps = 120
+    for _ in range(steps):
+        tokens, _ = target.generate(list(range(64)), first, 2, draft=draft, drafts=2)
+        counts += torch.bincount(torch.tensor([t[1] for t in tokens]), minlength=12)
+        for d in (target, draft):
+            d.cache.truncate(slots, lengths)
+    want = p * steps * 64
+    assert float(p.max()) < 0.9
+    assert ((counts - want).abs() <= 5 * (want * (1 - p)).sqrt() + 0.02 * want + 1).all(), (counts, want)
+
+
 def test_the_command_runs(cuda_device, capsys):
     main()
     text = capsys.readouterr().out
