@@ -162,7 +162,8 @@ class Kv4Cache:
         if ids.dtype is not torch.int32 or not ids.is_contiguous():
             if ids.dtype not in (torch.int32, torch.int64):
                 raise ValueError(f"{name} must be int32 or int64")
-            ids = ids.to(torch.int32).contiguous()
+            # What does not fit becomes the nearest number that does: out of range, or longer than any sequence.
+            ids = ids.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32).contiguous()
         if ids.ndim != 1:
             raise ValueError(f"{name} must be one-dimensional")
         if ids.device != self.device:

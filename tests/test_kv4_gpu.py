@@ -674,6 +674,34 @@ def test_other_errors_do_not_hold_writes_back(cuda_device):
         cache.check()
 
 
+def test_64_bit_ids_and_lengths_do_not_wrap(cuda_device):
+    """int64 arguments past 32 bits: a length above every sequence's, an id and a count out of range."""
+    def wide(*values):
+        return torch.tensor(values, dtype=torch.int64, device=cuda_device)
+
+    cache = filled(cuda_device, 20)
+    cache.extend([0, 1], 20)
+    host = R.HostCache.like(cache)
+    cache.truncate([0, 1], wide(2 ** 63 - 1, 2 ** 32))
+    cache.check()
+    host.same(cache)
+    for call in (lambda: cache.free(wide(2 ** 32)), lambda: cache.truncate(wide(2 ** 32 + 1), [3]),
+                 lambda: cache.fork(wide(0), wide(2 ** 32 + 1)), lambda: cache.fork(wide(2 ** 32), wide(2)),
+                 lambda: cache.extend(wide(-2 ** 32), 1)):
+        call()
+        with pytest.raises(RuntimeError, match="out of range or repeated"):
+            cache.check()
+        host.same(cache)
+    cache.extend([0, 1], wide(2 ** 32, 2 ** 62))
+    with pytest.raises(RuntimeError, match="table columns"):
+        cache.check()
+    host.same(cache)
+    cache.truncate([0], wide(-2 ** 63))
+    cache.check()
+    host.truncate([0], [0])
+    host.same(cache)
+
+
 # -- refusals -----------------------------------------------------------------------
 def test_refusals(cuda_device):
     cache = make(cuda_device, [5, 6])
