@@ -1234,7 +1234,8 @@ int check_queries(const char* what, const Kv4View& view, int64_t layer, int64_t 
     if (n < 0 || q_len < 0 || n > 65535 || q_len > (1 << 20) || q_heads > 65535 ||
         n * q_len * q_heads > (int64_t{1} << 30))
         return fail(POPKV_ERR_INVALID, "%s: sizes out of range", what);
-    if (!aligned(queries, 16) || s0 % 8 || s1 % 8 || s2 % 8)
+    // The stride of an axis with one entry is never followed, and a view may have any there.
+    if (!aligned(queries, 16) || (n > 1 && s0 % 8) || (q_len > 1 && s1 % 8) || (q_heads > 1 && s2 % 8))
         return fail(POPKV_ERR_INVALID, "%s: query rows must be 16-byte aligned", what);
     return POPKV_OK;
 }
@@ -1353,7 +1354,7 @@ extern "C" int popkv_kv4_attention_selected(const popkv_kv4_cache* cache, int64_
     const char* what = "popkv_kv4_attention_selected";
     Params p = {};
     if (int status = kv4_view(what, cache, &p.view)) return status;
-    if (int status = check_queries(what, p.view, layer, n, q_heads, 1, dtype, queries, q_seq_stride, q_head_stride, 0))
+    if (int status = check_queries(what, p.view, layer, n, q_heads, 1, dtype, queries, q_seq_stride, 0, q_head_stride))
         return status;
     if (selected < 0 || selected > (1 << 30)) return fail(POPKV_ERR_INVALID, "%s: selected out of range", what);
     if (p.view.layer_bytes / 16 > 0xFFFFFFFFll)

@@ -297,10 +297,13 @@ class Kv4Cache:
             raise RuntimeError("queries must be on the cache's device")
         strides = queries.stride()
         if strides[-1] != 1 or queries.data_ptr() % 16 or strides[0] % 8 or strides[1] % 8 or strides[-2] % 8:
-            queries = queries.contiguous()
-            if queries.data_ptr() % 16:
-                queries = queries.clone()
-            strides = queries.stride()
+            # An axis with one entry may have any stride, which contiguous() leaves as it is and nothing follows.
+            if strides[-1] != 1 or queries.data_ptr() % 16 or any(
+                    s % 8 for s, size in zip(strides[:-1], shape) if size > 1):
+                queries = queries.contiguous()
+                if queries.data_ptr() % 16:
+                    queries = queries.clone()
+                strides = queries.stride()
         return queries, strides, _lib.DTYPE_CODES[dtype]
 
     def attention(self, queries: torch.Tensor, *, seqs, layer: int = 0, counts=None,

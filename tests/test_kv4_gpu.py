@@ -702,6 +702,25 @@ def test_64_bit_ids_and_lengths_do_not_wrap(cuda_device):
     host.same(cache)
 
 
+def test_strides_of_axes_with_one_entry_do_not_matter(cuda_device):
+    """Rows that start on 16 bytes, in views whose axes of size 1 have odd strides."""
+    cache = make(cuda_device, [40], kv_heads=2, page=16)
+    wide = random_queries((1, 3 * 1028), torch.float16, cuda_device, 5)
+    plain = wide[:, :1024].clone().view(1, 8, 128)
+    want = cache.attention(plain, seqs=[0])
+    index = torch.arange(30, device=cuda_device).expand(1, 8, 30)
+    picked = cache.attention_selected(plain, index, seqs=[0])
+    one = torch.as_strided(wide, (1, 8, 128), (1028, 128, 1))
+    assert torch.equal(cache.attention(one, seqs=[0]), want)
+    assert torch.equal(cache.attention_selected(one, index, seqs=[0]), picked)
+    assert torch.equal(cache.attention(torch.as_strided(wide, (1, 1, 8, 128), (1028, 13, 128, 1)), seqs=[0])[:, 0], want)
+    few = make(cuda_device, [40], kv_heads=1, page=16)
+    head = torch.as_strided(wide, (1, 2, 1, 128), (3, 1024, 129, 1))
+    assert torch.equal(few.attention(head, seqs=[0]), few.attention(head.clone(), seqs=[0]))
+    odd = torch.as_strided(wide, (1, 2, 1, 128), (3, 1028, 129, 1))  # here the second token's row is not aligned
+    assert torch.equal(few.attention(odd, seqs=[0]), few.attention(odd.clone(), seqs=[0]))
+
+
 # -- refusals -----------------------------------------------------------------------
 def test_refusals(cuda_device):
     cache = make(cuda_device, [5, 6])
