@@ -35,7 +35,7 @@ namespace {
 constexpr int kChunk = 32;    // tokens of one stage of a warp: two tiles
 constexpr int kDim = kKv4Dim;
 constexpr int kMergeStride = kDim + 4;  // floats of a row in the warps' merge: conflict-free float2 stores
-constexpr float kNothing = -1e30f;      // `top` before any token
+constexpr float kNothing = -3e38f;      // `top` before any token: below any logit that queries in range give
 // Weights are kept below 2^(kHeadroom + kSlack): fp16's range ends at 2^16, and its
 // full precision 2^14 below 1.  The maximum is raised only when a token exceeds it by
 // kSlack (in powers of two), so the accumulators are rarely rescaled.

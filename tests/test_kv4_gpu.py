@@ -721,6 +721,27 @@ def test_strides_of_axes_with_one_entry_do_not_matter(cuda_device):
     assert torch.equal(few.attention(odd, seqs=[0]), few.attention(odd.clone(), seqs=[0]))
 
 
+def test_attention_of_logits_far_below_zero(cuda_device):
+    """bf16 queries whose every logit is below -1e30: a token is seen however small its logit."""
+    cache = Kv4Cache(8, kv_heads=1, max_seqs=1, max_tokens=100, page_size=16, device=cuda_device)
+    cache.extend([0], 70)
+    values = torch.randn(1, 70, 1, 128, generator=torch.Generator().manual_seed(1))
+    keys = torch.ones(1, 70, 1, 128)
+    keys[0, 50:] = 1.25
+    cache.write(keys.to(cuda_device), values.to(cuda_device), seqs=[0])
+    queries = torch.zeros(1, 1, 4, 128, dtype=torch.bfloat16, device=cuda_device)
+    queries[0, 0, 0] = -1e30
+    queries[0, 0, 1] = -1e32
+    queries[0, 0, 2] = -3e34
+    queries[0, 0, 3] = 1e32
+    host = R.HostCache.like(cache)
+    v = np.stack([host.get(0, 0, 0, t)[1] for t in range(70)])
+    want = np.stack([v[:50].mean(0), v[:50].mean(0), v[:50].mean(0), v[50:].mean(0)])[None, None]
+    close(cache.attention(queries, seqs=[0]), want, np.abs(v).max())
+    picked = torch.arange(70, device=cuda_device).expand(1, 4, 70)
+    close(cache.attention_selected(queries[:, 0], picked, seqs=[0]), want[:, 0], np.abs(v).max())
+
+
 # -- refusals -----------------------------------------------------------------------
 def test_refusals(cuda_device):
     cache = make(cuda_device, [5, 6])
