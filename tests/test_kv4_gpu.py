@@ -293,6 +293,76 @@ def test_attention_ignores_what_lies_past_the_end(cuda_device, stale):
     close(got, want, most)
 
 
+def chunk_coded(device, lengths, *, kv_heads, page, group):
+    """A cache whose value of a token is 1 in the dim (number of its 32 tokens + head) % 128 and 0 elsewhere, so
+    that an output is the weight of each 32 tokens and lost ones leave a hole of their own."""
+    cache = Kv4Cache(sum(-(-t // page) for t in lengths), kv_heads=kv_heads, max_seqs=len(lengths),
+                     max_tokens=max(lengths), page_size=page, dim_group_size=group, device=device)
+    gen = torch.Generator().manual_seed(len(lengths))
+    for s, tokens in enumerate(lengths):
+        if not tokens:
+            continue
+        cache.extend([s], tokens)
+        dims = (torch.arange(tokens)[:, None] // 32 + torch.arange(kv_heads)) % 128
+        values = torch.nn.functional.one_hot(dims, 128).half()
+        keys = torch.randn(tokens, kv_heads, 128, generator=gen).half()
+        cache.write(keys[None].to(device), values[None].to(device), seqs=[s])
+    cache.check()
+    return cache
+
+
+def chunk_weights(cache, seq, query, positions, group, scale=128 ** -0.5):
+    """float64 outputs of a query [128] over tokens of its KV head, and the bound on a kernel's difference.
+
+    Numbers enter the outputs as n - 8, with weights p * delta rounded to fp16: 2^-11 of |n - 8| * delta <=
+    8/15 for the tokens whose 1 lies in a dim's group (elsewhere delta is 0 and the value exact).  The output
+    rounds by 2^-11 of itself, or half an fp16 denormal.  2^-15 covers the logits (below 1e-6, see above), exp2 and the
+    products' truncated additions (2^-23 of a partial sum below 0.6 for each of up to 2000).
+    """
+    keys, values, head = query[1]
+    k, v = keys[:, head][positions], values[:, head][positions]
+    p = torch.softmax(k @ query[0] * scale, 0)
+    mass = (p @ v).view(-1, group).sum(-1).repeat_interleave(group)
+    want = p @ v
+    return want, 2.0 ** -11 * (8 / 15) * mass + 2.0 ** -11 * want + 2.0 ** -15
+
+
+@pytest.mark.parametrize("lengths,heads,per,q_len,page,group", [
+    ([20011], 1, 4, 1, 64, 32), ([9001], 1, 8, 1, 16, 64), ([6003], 1, 4, 4, 64, 128), ([6003], 1, 4, 5, 64, 32),
+    ([4099], 1, 4, 10, 32, 32), ([777, 5003, 64, 0, 3001] * 7, 2, 4, 1, 16, 32),
+    ([777, 3001, 64, 0, 2005] * 13, 2, 3, 2, 64, 64), ([777, 2001, 64, 0, 1005] * 13, 2, 4, 5, 64, 32)])
+def test_attention_leaves_no_chunk_out(cuda_device, lengths, heads, per, q_len, page, group):
+    """A bound that 32 tokens left out exceed by far wherever a segment is cut."""
+    cache = chunk_coded(cuda_device, lengths, kv_heads=heads, page=page, group=group)
+    n = len(lengths)
+    queries = 0.3 * torch.randn(n, q_len, heads * per, 128, generator=torch.Generator().manual_seed(7))
+    queries = queries.half().to(cuda_device)
+    got = cache.attention(queries, seqs=list(range(n))).double()
+    index = torch.stack([torch.randperm(max(lengths), generator=torch.Generator().manual_seed(h))
+                         for h in range(heads * per)]).to(cuda_device)
+    picked = cache.attention_selected(queries[:, 0], index.expand(n, -1, -1), seqs=list(range(n))).double()
+    for s in range(n):
+        if not lengths[s]:
+            assert not got[s].any() and not picked[s].any()
+            continue
+        keys, values = (x[0].double() for x in cache.read([s], tokens=lengths[s], dtype=torch.float32))
+        for h in range(heads * per):
+            for j in range(q_len):
+                seen = slice(0, max(0, lengths[s] - q_len + j + 1))
+                want, bound = chunk_weights(cache, s, (queries[s, j, h].double(), (keys, values, h // per)), seen, group)
+                error = (got[s, j, h] - want).abs()
+                assert (error <= bound).all(), (s, j, h, float((error / bound).max()))
+            want, bound = chunk_weights(cache, s, (queries[s, 0, h].double(), (keys, values, h // per)),
+                                        slice(0, lengths[s]), group)
+            error = (picked[s, h] - want).abs()
+            assert (error <= bound).all(), (s, h, float((error / bound).max()))
+            # What the bound is for: the largest and the smallest hole that 32 tokens would leave.
+            k = keys[:, h // per]
+            p = torch.softmax(k @ queries[s, 0, h].double() * 128 ** -0.5, 0)
+            holes = torch.stack([c.sum() for c in p.split(32) if len(c) == 32]) if lengths[s] >= 32 else p[:0]
+            assert not len(holes) or float(holes.min()) > 4 * float(bound.max())
+
+
 def test_attention_of_extreme_logits(cuda_device):
     """Large logits, equal logits, tiny and large values; a NaN query spoils its own row alone."""
     cache = make(cuda_device, [70], kv_heads=1, page=64)
