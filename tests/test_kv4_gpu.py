@@ -812,6 +812,72 @@ def test_attention_of_logits_far_below_zero(cuda_device):
     close(cache.attention_selected(queries[:, 0], picked, seqs=[0]), want[:, 0], np.abs(v).max())
 
 
+def test_one_workspace_for_calls_of_several_sizes(cuda_device):
+    """A workspace of the largest call serves smaller ones in turn, of either attention."""
+    lengths = [(211 * i) % 1500 for i in range(40)]
+    cache = make(cuda_device, lengths, kv_heads=2, page=16)
+    workspace = cache.workspace(40, 16, 5)
+    calls = []
+    for n, heads, q_len in ((40, 16, 5), (1, 2, 1), (7, 8, 1), (40, 16, 1), (3, 8, 4), (1, 16, 5)):
+        seqs = torch.arange(40 - n, 40, dtype=torch.int32, device=cuda_device)
+        q = random_queries((n, q_len, heads, 128), torch.float16, cuda_device, n + heads)
+        calls.append((cache.attention, (q,), seqs))
+        index = torch.randint(0, 1500, (n, heads, 70), generator=torch.Generator().manual_seed(n)).to(cuda_device)
+        calls.append((cache.attention_selected, (q[:, 0], index), seqs))
+    want = [call(*args, seqs=seqs) for call, args, seqs in calls]
+    for _ in range(3):
+        for (call, args, seqs), out in zip(calls, want):
+            assert torch.equal(call(*args, seqs=seqs, workspace=workspace), out)
+    with pytest.raises(RuntimeError, match="workspace"):
+        cache.attention(random_queries((1, 1, 2, 128), torch.float16, cuda_device, 0), seqs=[0],
+                        workspace=workspace[:1 << 16])
+    with pytest.raises(ValueError, match="workspace"):
+        cache.attention(random_queries((1, 1, 2, 128), torch.float16, cuda_device, 0), seqs=[0],
+                        workspace=workspace.int())
+
+
+def test_page_operations_and_selected_attention_in_a_graph(cuda_device):
+    """fork, extend, write, attention_selected, truncate, free and compact captured once and replayed."""
+    cache, twin = (make(cuda_device, [37, 50], kv_heads=2, page=16, spare=12, max_seqs=5) for _ in range(2))
+    x = torch.randn(3, 4, 8, 128, generator=torch.Generator().manual_seed(3)).half().to(cuda_device)
+    q, k, v = x[0], x[1, :, :2].contiguous(), x[2, :, :2].contiguous()
+    ids = {name: torch.tensor(value, dtype=torch.int32, device=cuda_device) for name, value in {
+        "parents": [0, 1, 0], "children": [2, 3, 4], "all": [0, 2, 3, 4], "some": [2, 0], "kept": [30, 38],
+        "gone": [3, 4]}.items()}
+    index = torch.randint(0, 60, (4, 8, 40), generator=torch.Generator().manual_seed(4)).to(cuda_device)
+    workspaces = {id(c): c.workspace(4, 8) for c in (cache, twin)}
+
+    def step(c):
+        c.fork(ids["parents"], ids["children"])
+        c.extend(ids["all"], 1)
+        c.write(k, v, seqs=ids["all"])
+        out = c.attention_selected(q, index, seqs=ids["all"], workspace=workspaces[id(c)])
+        whole = c.attention(q, seqs=ids["all"], workspace=workspaces[id(c)])
+        c.truncate(ids["some"], ids["kept"])
+        c.free(ids["gone"])
+        c.compact()
+        return out, whole
+
+    snapshot = cache.tables.clone(), cache.pages.clone()
+    step(cache)
+    cache.tables.copy_(snapshot[0])
+    cache.pages.copy_(snapshot[1])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(cache)
+    for i in range(4):
+        k.copy_(x[1, :, :2] * (i + 1))
+        graph.replay()
+        want = step(twin)
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        assert torch.equal(cache.tables, twin.tables) and torch.equal(cache.pages, twin.pages)
+        assert torch.equal(cache.status[1:3], twin.status[1:3])
+    cache.check()
+    twin.check()
+    del graph
+
+
 # -- refusals -----------------------------------------------------------------------
 def test_refusals(cuda_device):
     cache = make(cuda_device, [5, 6])

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from popkv_b200.speculative import verify_drafts
+from popkv_b200.speculative import verify_drafts, verify_workspace
 from tests import kv4_reference as R
 
 pytestmark = pytest.mark.gpu
@@ -181,3 +181,34 @@ def test_refusals_at_any_place_of_many_drafts(cuda_device, drafts, n, vocab, pro
     for _ in range(30):
         again = verify_drafts(target, tokens, uniforms, noise, draft_probs=draft)
         assert torch.equal(again[0], got) and torch.equal(again[1], accepted)
+
+
+@pytest.mark.parametrize("given", (True, False))
+def test_verification_in_a_graph(cuda_device, given):
+    """Captured with a workspace of its own or the call's, and replayed on new inputs; one workspace for several sizes."""
+    sets = [inputs(6, 4, 5003, torch.float32, cuda_device, s) for s in range(4)]
+    held = [t.clone() for t in sets[0]]
+    workspace = verify_workspace(9, cuda_device) if given else None
+
+    def call(t, d, u, e, q):
+        return verify_drafts(t, d, u, e, draft_probs=q, workspace=workspace)
+
+    call(*held)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(*held)
+    for s in sets:
+        for to, new in zip(held, s):
+            to.copy_(new)
+        graph.replay()
+        want = verify_drafts(*s[:4], draft_probs=s[4])
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        few = [t[:2] for t in s]
+        got = call(*few)
+        assert torch.equal(got[0], want[0][:2]) and torch.equal(got[1], want[1][:2])
+    if given:
+        assert not workspace.any()
+        with pytest.raises(ValueError, match="workspace"):
+            verify_drafts(*held[:4], draft_probs=held[4], workspace=workspace[:12])
+    del graph
