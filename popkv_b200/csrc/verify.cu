@@ -166,11 +166,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const __grid_
         int before;
         asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(before) : "l"(p.arrived + b) : "memory");
         is_last = before == static_cast<int>(gridDim.x) - 1;
-        if (is_last) {  // one thread reads the winner and clears the workspace, so that no warp reads it cleared
-            winner = __ldcg(p.best + b);
-            p.best[b] = 0;
-            p.arrived[b] = 0;
-        }
+        // One thread reads the winner: by the time that others would, it may have cleared the workspace.  It
+        // clears it at the end only (64 x 8 drafts: 20.0 us, and 22.6 with the stores here).
+        if (is_last) winner = __ldcg(p.best + b);
     }
     __syncthreads();
     if (!is_last) return;
@@ -186,7 +184,11 @@ __global__ void __launch_bounds__(kVerifyThreads, 4) verify_kernel(const __grid_
     const int64_t next = best ? static_cast<int64_t>(0xFFFFFFFFu - static_cast<uint32_t>(best)) : 0;
     for (int i = threadIdx.x; i <= p.drafts; i += kVerifyThreads)
         p.out[b * (p.drafts + 1) + i] = i < accepted ? tokens[i] : i == accepted ? next : -1;
-    if (threadIdx.x == 0) p.accepted[b] = accepted;
+    if (threadIdx.x == 0) {
+        p.accepted[b] = accepted;
+        p.best[b] = 0;
+        p.arrived[b] = 0;
+    }
 }
 
 template <typename T>
