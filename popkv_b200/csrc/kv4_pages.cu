@@ -77,10 +77,11 @@ __global__ void __launch_bounds__(kPlanThreads) extend_kernel(Kv4View view, cons
     int32_t* target = source + n;
     const int size = view.page_size();
     int refs_ahead = threadIdx.x < view.num_pages ? view.refs[threadIdx.x] : 1;
+    const int status = threadIdx.x == 0 ? view.status[0] : 0;
     for (int i = threadIdx.x; i < n; i += kPlanThreads) ids[i] = seqs[i];
     // After an extend that found no room none succeeds until the caller has seen it: the tokens in between would be
     // missing from the sequence.
-    if (threadIdx.x == 0) short_of_columns = view.status[0] & kKv4StatusFull;
+    if (threadIdx.x == 0) short_of_columns = status & kKv4StatusFull;
     __syncthreads();
 
     // Pages that each entry needs: those its tokens reach, and one for the copy of
