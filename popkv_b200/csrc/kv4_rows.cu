@@ -22,7 +22,7 @@ int kv4_view(const char* what, const popkv_kv4_cache* cache, Kv4View* view) {
     constexpr int64_t kMost = 1 << 30;
     if (cache->layers < 1 || cache->num_pages < 1 || cache->kv_heads < 1 || cache->max_seqs < 1 ||
         cache->max_pages < 1 || cache->layers > 65535 || cache->num_pages > kMost || cache->kv_heads > 65535 ||
-        cache->max_seqs > kMost || cache->max_pages * p > kMost)
+        cache->max_seqs > kMost || cache->max_pages > kMost / p)
         return fail(POPKV_ERR_INVALID, "%s: cache sizes out of range", what);
     view->pages = cache->pages;
     view->refs = cache->refs;

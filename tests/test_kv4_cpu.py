@@ -153,3 +153,12 @@ def test_waits_that_steer_a_warp_are_voted_on():
         text = (Path(kv4.__file__).parent / "csrc" / name).read_text()
         assert "mbar_wait(" in text
         assert not re.findall(r"(?:if|while)\s*\(\s*!?\s*mbar_wait\(|=\s*mbar_wait\(", text), name
+
+
+@pytest.mark.parametrize("max_pages,page_size", [(1 << 58, 64), (1 << 60, 16), ((1 << 56) + 3, 256), ((1 << 24) + 1, 64)])
+def test_table_widths_past_64_bits_are_refused(lib, max_pages, page_size):
+    """Widths whose product with the page size wraps to a small number."""
+    keep, c = descriptor(max_pages=max_pages, page_size=page_size)
+    refused(lib, lib.popkv_kv4_truncate(c, None, 0, None, None), "sizes out of range")
+    keep, c = descriptor(max_pages=1 << 24, page_size=64)
+    assert lib.popkv_kv4_truncate(c, None, 0, None, None) == 0
