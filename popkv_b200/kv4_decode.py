@@ -190,6 +190,8 @@ class Kv4Decoder:
 
         generator: of the random numbers, instead of the decoder's own.
         """
+        if not temperature > 0:
+            raise ValueError("temperature must be positive")
         probs = (logits / temperature).softmax(-1)
         n = probs.shape[0]
         none = torch.empty((n, 0), device=self.device)
@@ -207,6 +209,10 @@ class Kv4Decoder:
         """
         if draft is not None and (self.sparse_layers or draft.sparse_layers):
             raise ValueError("drafted tokens need dense attention: the sparse layers take one token a step")
+        if not temperature > 0:
+            raise ValueError("temperature must be positive")
+        if draft is not None and drafts < 1:
+            raise ValueError("drafts must be positive")
         n = len(slots)
         seqs = torch.tensor(slots, dtype=torch.int32, device=self.device)
         pending = first.to(self.device)

@@ -313,6 +313,20 @@ def test_generated_tokens_are_the_targets(cuda_device):
     assert ((counts - want).abs() <= 5 * (want * (1 - p)).sqrt() + 0.02 * want + 1).all(), (counts, want)
 
 
+def test_sampling_arguments_are_checked(weights):
+    """Before a token is drawn: a temperature of 0 made every probability NaN, and every token id 0."""
+    d = Kv4Decoder(weights, max_seqs=1, max_tokens=64)
+    logits = d.prefill(0, prompt(20))[None]
+    for temperature in (0.0, -1.0, float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            d.sample(logits, temperature)
+        with pytest.raises(ValueError, match="temperature"):
+            d.generate([0], torch.zeros(1, dtype=torch.int64), 3, temperature=temperature)
+    with pytest.raises(ValueError, match="drafts must be positive"):
+        d.generate([0], torch.zeros(1, dtype=torch.int64), 3, draft=d, drafts=0)
+    assert d.cache.lengths.tolist() == [20]
+
+
 def test_the_command_runs(cuda_device, capsys):
     main()
     text = capsys.readouterr().out
