@@ -213,6 +213,8 @@ class Kv4Decoder:
             raise ValueError("temperature must be positive")
         if draft is not None and drafts < 1:
             raise ValueError("drafts must be positive")
+        if draft is not None and draft.cfg.vocab_size != self.cfg.vocab_size:
+            raise ValueError("the draft model's vocabulary must be the target's")
         n = len(slots)
         seqs = torch.tensor(slots, dtype=torch.int32, device=self.device)
         pending = first.to(self.device)

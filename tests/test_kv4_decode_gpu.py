@@ -327,6 +327,18 @@ def test_sampling_arguments_are_checked(weights):
     assert d.cache.lengths.tolist() == [20]
 
 
+def test_a_draft_of_another_vocabulary_is_refused(weights, cuda_device):
+    """Before its ids reach the target's embedding."""
+    target = Kv4Decoder(weights, max_seqs=1, max_tokens=64)
+    other = Kv4Decoder(LlamaWeights.random(replace(CONFIG, vocab_size=600), device=cuda_device), max_seqs=1,
+                       max_tokens=64)
+    for d in (target, other):
+        d.prefill(0, prompt(20))
+    with pytest.raises(ValueError, match="vocabulary"):
+        target.generate([0], torch.zeros(1, dtype=torch.int64), 3, draft=other)
+    assert target.cache.lengths.tolist() == other.cache.lengths.tolist() == [20]
+
+
 def test_the_command_runs(cuda_device, capsys):
     main()
     text = capsys.readouterr().out
