@@ -708,7 +708,8 @@ POPKV_API int popkv_kv4_read(const popkv_kv4_cache* cache, int64_t layer, const 
  * queries[i, j, h, d] is read at queries + i*q_seq_stride + j*q_token_stride +
  * h*q_head_stride + d, fp16 or bf16; query head h reads KV head h / (q_heads / kv_heads).
  * out [n, q_len, q_heads, 128] of the same type; rows j >= counts[i], and rows that see no
- * token, are zeros.  Query rows are 16-byte aligned (strides multiples of 8, but
+ * token, are zeros.  Logits, weights p and sums are fp32; p * delta is rounded to fp16 (2^-11 of a
+ * value's distance from its group's middle).  Query rows are 16-byte aligned (strides multiples of 8, but
  * for axes with one entry).
  * workspace: popkv_kv4_attention_workspace bytes, 16-byte aligned, zero before the first call;
  * every call leaves it usable for the next, of any size that it holds.  Calls that overlap in

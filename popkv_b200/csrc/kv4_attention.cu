@@ -9,20 +9,25 @@
 // numbers with 16-bit rows, so the 4-bit numbers are never turned into values: a
 // number in the low bits of an fp16 is the denormal n * 2^-24, which the tensor
 // cores multiply exactly, and the pairs scale whole 16 x 8 blocks of results in
-// fp32.  The only rounding to fewer bits is that of p_t delta' to fp16.
+// fp32.  The only rounding to fewer bits is that of p_t delta' to fp16, which the second product
+// takes; p itself, its sum and the lows' share stay in fp32.  Against 64 bits the outputs are off by
+// 2.9e-4 (fp16) and 1.7e-3 (bf16) of their rms, of which their own rounding is 2.1e-4 and 1.6e-3.
 //
 // Roles in the products (mma m16n8k16, fp32 accumulators): tokens are the 16 rows
 // of the logits' product and the 16-deep axis of the outputs' product, query rows
 // are the 8 columns of both.  One pass over the cache serves every query row of a KV
 // head, and a warp needs no exchange with others until its tokens are through.
 //
-// What bounds it, measured with 32 query and 8 KV heads, groups of 32 dims: one query token over
-// 131072 tokens (168 MB) takes 41.1 us, of which about 12 us are fixed (finding the CTA's
+// What bounds it, measured with 32 query and 8 KV heads, groups of 32 dims, in graphs of passes whose
+// caches exceed L2 together: one query token over
+// 131072 tokens (168 MB) takes 40.7 us, of which about 12 us are fixed (finding the CTA's
 // share, first lookups and copies, merge, join); the loop itself runs at 84 to 91% of the
 // copy rate, with the ALU pipe, which takes the numbers apart, next at 46%.  Five query tokens
-// (20 rows) are bound by fixed-latency dependencies at 8 warps of 255 registers: 76 us.  Many
-// sequences are bound by what each costs besides its chunks (256 of 10 to 600 tokens, 104 MB: 48.7 us),
-// selected slots by three random accesses each, 45 to 50 a nanosecond (8 x 4096 of 131072 tokens: 69.3 us).
+// (20 rows) are bound by fixed-latency dependencies at 8 warps of 255 registers: 92.4 us, four such
+// sequences 300 us.  Many
+// sequences are bound by what each costs besides its chunks (256 of 10 to 600 tokens, 104 MB: 48.6 us),
+// selected slots by three random accesses each, of a layout that keeps keys, values and pairs of 16 tokens
+// apart, 45 to 50 a nanosecond (8 x 4096 of 131072 tokens: 70.4 us).
 #include <cmath>
 #include <type_traits>
 
@@ -238,7 +243,8 @@ __device__ __forceinline__ void stage_queries(const Params& p, Queries<NT>& s, c
         }
 #pragma unroll
         for (int step = 1; step < 16; step *= 2) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, step));
-        // The largest of the row to [2^13, 2^14): exact in fp16 down to 2^-38 of it.
+        // The largest of the row to [2^13, 2^14): in fp16 a bf16 value is exact down to 2^-31 of it, an fp16 one
+        // down to 2^-28, and smaller ones are off by at most 2^-38 of it.
         const int exponent = static_cast<int>(__float_as_uint(most) >> 23) - 127;  // -127 for 0 and denormals
         const int up = most == 0.0f || exponent == 128 ? 0 : min(13 - exponent, 126);
         const float by = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
@@ -725,7 +731,7 @@ __device__ Place find_place(const Params& p, int segments) {
 
 // 16-byte (or 8-byte) copy into shared memory, zeros where `there` is false.
 __device__ __forceinline__ void copy16(uint8_t* to, const uint8_t* from, bool there) {
-    // 64 bytes at a time from memory: the rows are that long (8 x 4096 slots of 131072 tokens 70.3 us, by lines
+    // 64 bytes at a time from memory: the rows are that long (8 x 4096 slots of 131072 tokens 70.4 us, by lines
     // of 128 73.6).
     asm volatile("cp.async.cg.shared.global.L2::64B [%0], [%1], 16, %2;" ::"r"(smem_addr(to)), "l"(from), "r"(there ? 16 : 0)
                  : "memory");
@@ -751,7 +757,8 @@ struct Sizes {
     // and 79.7 us with 16, 24 and 32.  Selected, 16 x 512: 28.2, 26.6 and 28.2 us with 6, 8 and 10.
     static constexpr int kSegmentCost = kWhole ? 24 : kSelected ? 8 : NC == 1 ? 12 : 16;
     // Tiles of one pass: two give the products more that does not wait (131072 tokens, 16 rows: 62.5 against
-    // 68.4 us with one; 8 x 4096 selected: 76.2 against 77.6).  With 24 rows two spill (73.7 against 74.9 us).
+    // 68.4 us with one; 8 x 4096 selected: 76.2 against 77.6).  With 24 rows the two are within 2% of each other
+    // (20 rows of one sequence 91.7 and 92.6 us, of four 74.9 and 73.7 a sequence); two spill 592 bytes a thread, one 176.
     static constexpr int kTogether = NT <= 2 ? 2 : 1;
     static constexpr int kTile = kKv4PairOffset + kKv4TileTokens * 8 * NG;
     static constexpr int kStageBytes = 2 * kTile;
