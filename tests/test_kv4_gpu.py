@@ -311,7 +311,7 @@ def chunk_coded(device, lengths, *, kv_heads, page, group):
     return cache
 
 
-def chunk_weights(cache, seq, query, positions, group, scale=128 ** -0.5):
+def chunk_weights(query, positions, group, scale=128 ** -0.5):
     """float64 outputs of a query [128] over tokens of its KV head, and the bound on a kernel's difference.
 
     Numbers enter the outputs as n - 8, with weights p * delta rounded to fp16: 2^-11 of |n - 8| * delta <=
@@ -349,11 +349,12 @@ def test_attention_leaves_no_chunk_out(cuda_device, lengths, heads, per, q_len, 
         for h in range(heads * per):
             for j in range(q_len):
                 seen = slice(0, max(0, lengths[s] - q_len + j + 1))
-                want, bound = chunk_weights(cache, s, (queries[s, j, h].double(), (keys, values, h // per)), seen, group)
+                query = queries[s, j, h].double(), (keys, values, h // per)
+                want, bound = chunk_weights(query, seen, group)
                 error = (got[s, j, h] - want).abs()
                 assert (error <= bound).all(), (s, j, h, float((error / bound).max()))
-            want, bound = chunk_weights(cache, s, (queries[s, 0, h].double(), (keys, values, h // per)),
-                                        slice(0, lengths[s]), group)
+            query = queries[s, 0, h].double(), (keys, values, h // per)
+            want, bound = chunk_weights(query, slice(0, lengths[s]), group)
             error = (picked[s, h] - want).abs()
             assert (error <= bound).all(), (s, h, float((error / bound).max()))
             # What the bound is for: the largest and the smallest hole that 32 tokens would leave.
@@ -783,7 +784,8 @@ def test_strides_of_axes_with_one_entry_do_not_matter(cuda_device):
     one = torch.as_strided(wide, (1, 8, 128), (1028, 128, 1))
     assert torch.equal(cache.attention(one, seqs=[0]), want)
     assert torch.equal(cache.attention_selected(one, index, seqs=[0]), picked)
-    assert torch.equal(cache.attention(torch.as_strided(wide, (1, 1, 8, 128), (1028, 13, 128, 1)), seqs=[0])[:, 0], want)
+    token = torch.as_strided(wide, (1, 1, 8, 128), (1028, 13, 128, 1))
+    assert torch.equal(cache.attention(token, seqs=[0])[:, 0], want)
     few = make(cuda_device, [40], kv_heads=1, page=16)
     head = torch.as_strided(wide, (1, 2, 1, 128), (3, 1024, 129, 1))
     assert torch.equal(few.attention(head, seqs=[0]), few.attention(head.clone(), seqs=[0]))
@@ -876,6 +878,75 @@ def test_page_operations_and_selected_attention_in_a_graph(cuda_device):
     cache.check()
     twin.check()
     del graph
+
+
+def test_page_operations_on_thousands_of_sequences(cuda_device):
+    """More entries than the plans' threads, and tables that a fork takes two launches for."""
+    rng = np.random.default_rng(5)
+    cache = Kv4Cache(14000, kv_heads=1, max_seqs=3000, max_tokens=20 * 16, page_size=16, dim_group_size=128,
+                     device=cuda_device)
+    cache.pages.random_(0, 256)
+    host = R.HostCache.like(cache)
+
+    def ids(values):
+        return torch.tensor(values, dtype=torch.int32, device=cuda_device)
+
+    def extend(seqs, counts):
+        assert host.extend(seqs, counts)
+        cache.extend(ids(seqs), ids(counts))
+        cache.check()
+        host.same(cache)
+
+    extend(rng.permutation(3000).tolist(), rng.integers(0, 40, 3000).tolist())
+    for n in (1400, 2000):
+        parents, children = rng.integers(0, 3000, n).tolist(), rng.permutation(3000)[:n].tolist()
+        host.fork(parents, children)
+        cache.fork(ids(parents), ids(children))
+        host.same(cache)
+        extend(rng.permutation(3000)[:2900].tolist(), rng.integers(0, 4, 2900).tolist())
+    some, lengths = rng.permutation(3000).tolist(), rng.integers(-5, 50, 3000).tolist()
+    host.truncate(some, lengths)
+    cache.truncate(ids(some), ids(lengths))
+    host.truncate(some[:1100], [0] * 1100)
+    cache.free(ids(some[:1100]))
+    host.same(cache)
+    assert cache.status[0].item() == 0
+    cache.compact()
+    assert tuple(cache.status[1:3].tolist()) == host.compact()
+    host.same(cache)
+    before = host.refs.copy()
+    assert not host.extend(some, [310 - int(host.lengths[s]) for s in some])
+    cache.extend(ids(some), ids([310 - int(host.lengths[s]) for s in some]))
+    with pytest.raises(RuntimeError, match="too few free pages"):
+        cache.check()
+    assert np.array_equal(before, host.refs)
+    host.same(cache)
+
+
+@pytest.mark.parametrize("heads,group,dtype", [(12, 32, torch.bfloat16), (9, 64, torch.float16),
+                                               (16, 128, torch.float32)])
+def test_rows_and_attention_of_many_heads(cuda_device, heads, group, dtype):
+    """More KV heads than a block has warps."""
+    cache = make(cuda_device, [37, 20], kv_heads=heads, page=16, group=group)
+    host = R.HostCache.like(cache)
+    x = torch.randn(2, 2, 7, heads, 128, generator=torch.Generator().manual_seed(heads)).to(dtype)
+    cache.write(x[0].to(cuda_device), x[1].to(cuda_device), seqs=[0, 1])
+    for s, length in enumerate((37, 20)):
+        for t in range(7):
+            for h in range(heads):
+                host.put(0, s, h, length - 7 + t, x[0, s, t, h].float().numpy(), x[1, s, t, h].float().numpy())
+    host.same(cache)
+    got = cache.read([1, 0], tokens=40, dtype=dtype)
+    for which in range(2):
+        want = np.zeros((2, 40, heads, 128))
+        for i, s in enumerate((1, 0)):
+            for t in range((37, 20)[s]):
+                for h in range(heads):
+                    want[i, t, h] = host.get(0, s, h, t)[which]
+        assert torch.equal(got[which].cpu(), torch.from_numpy(want).float().to(dtype))
+    queries = random_queries((2, 3, 2 * heads, 128), torch.float16, cuda_device, heads)
+    want, most = expect(cache, host, queries, lambda at: (at[0], range((37, 20)[at[0]] - 3 + at[1] + 1)))
+    close(cache.attention(queries, seqs=[0, 1]), want, most)
 
 
 # -- refusals -----------------------------------------------------------------------
